@@ -130,8 +130,8 @@ def _need(amax, fmt):
     """The scale of a block whose largest magnitude is amax: e4m3 the smallest power of two with amax / scale <= 448, int8 amax / 127."""
     if fmt == "int8":
         return amax / 127.0
-    m, e = torch.frexp(amax / 448.0)
-    return torch.where(amax > 0, torch.ldexp(torch.ones_like(amax), torch.where(m > 0.5, e, e - 1)), torch.zeros_like(amax))
+    m, e = torch.frexp(amax)   # 448 = 0.875 * 2^9; a division by 448 would round magnitudes that need no rounding
+    return torch.where(amax > 0, torch.ldexp(torch.ones_like(amax), torch.where(m > 0.875, e - 8, e - 9)), torch.zeros_like(amax))
 
 
 def _encode(x, fmt):
@@ -334,9 +334,10 @@ def _exact_append(st):
             full = torch.zeros(rows.shape[0], count * block, rows.shape[2], dtype=torch.float64, device="cuda")
             full[:, lead:lead + n] = rows
             full = full.view(rows.shape[0], count, block, -1)
-            need = full.abs().amax(dim=(2, 3)) / bound
-            if fmt == "e4m3":
-                need = torch.where(need > 0, 2.0 ** torch.ceil(torch.log2(need)), need)
+            need = full.abs().amax(dim=(2, 3)) / torch.full((), bound, dtype=torch.float64, device="cuda")   # by a tensor: a true quotient
+            if fmt == "e4m3":                                                                # the next power of two, itself where it is one
+                mantissa, e = torch.frexp(need)
+                need = torch.where(need > 0, torch.ldexp(torch.ones_like(need), torch.where(mantissa > 0.5, e, e - 1)), need)
             g = o // block + torch.arange(count, device="cuda")                              # block numbers along the sequence
             pg, b = st["table"][s].long()[g * block // page], g % (page // block)
             if lead:
