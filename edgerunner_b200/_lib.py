@@ -49,6 +49,35 @@ class er_step_params(C.Structure):
                 ("rms_eps", C.c_float), ("norm_weight_layer_stride", C.c_uint32), ("sliding_window", C.c_uint32), ("reserved", C.c_uint32)]
 
 
+class er_qk_norm_rope_params(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "q_out", "k", "k_out")] + [
+        (n, C.c_int64) for n in ("q_token_stride", "q_head_stride", "q_out_token_stride", "q_out_head_stride",
+                                 "k_token_stride", "k_head_stride", "k_out_token_stride", "k_out_head_stride")] + [
+        (n, C.c_void_p) for n in ("positions", "q_norm_weight", "k_norm_weight")] + [
+        (n, C.c_uint32) for n in ("num_tokens", "num_heads", "num_kv_heads", "head_dim", "type")] + [
+        (n, C.c_float) for n in ("rms_eps", "rope_theta", "rope_scaling", "partial_rotary_factor")]
+
+
+class er_kv8_cache(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("keys", "values", "key_scales", "value_scales", "block_tables", "kv_lens", "status")] + [
+        (n, C.c_uint32) for n in ("num_pages", "page_size", "scale_block", "num_kv_heads", "head_dim", "format", "num_seqs",
+                                  "block_table_width", "block_table_stride")]
+
+
+class er_kv8_append_params(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v")] + [
+        (n, C.c_int64) for n in ("k_token_stride", "k_head_stride", "v_token_stride", "v_head_stride")] + [
+        (n, C.c_void_p) for n in ("query_starts", "k_norm_weight")] + [(n, C.c_uint32) for n in ("num_tokens", "type")] + [
+        (n, C.c_float) for n in ("rms_eps", "rope_theta", "rope_scaling", "partial_rotary_factor")]
+
+
+class er_kv8_attention_params(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "out")] + [
+        (n, C.c_int64) for n in ("q_token_stride", "q_head_stride", "out_token_stride", "out_head_stride")] + [
+        ("query_starts", C.c_void_p)] + [(n, C.c_uint32) for n in ("num_tokens", "num_heads", "query_len", "max_query_len", "type")] + [
+        ("softmax_scale", C.c_float), ("sliding_window", C.c_uint32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
+
+
 # status codes (include/er_kv.h)
 ER_OK = 0
 ER_ERR_ALLOCATION_FAILED, ER_ERR_INVALID_LAYER, ER_ERR_PRECISION_MISMATCH, ER_ERR_UNSUPPORTED_STORAGE = -1, -2, -3, -4
@@ -116,6 +145,12 @@ SYMBOLS = {
     "er_kv_page_bytes": (C.c_int64, [_vp]),
     "er_kv_export_pages": (_i32, [_vp, _vp, _u32, _vp, _sz, _vp]),
     "er_kv_import_pages": (_i32, [_vp, _vp, _u32, _vp, _sz, _vp]),
+    "er_qk_norm_rope": (_i32, [C.POINTER(er_qk_norm_rope_params), _vp]),
+    "er_kv8_append": (_i32, [C.POINTER(er_kv8_cache), C.POINTER(er_kv8_append_params), _vp]),
+    "er_kv8_decode_workspace_bytes": (C.c_int64, [C.POINTER(er_kv8_cache), C.POINTER(er_kv8_attention_params)]),
+    "er_kv8_attention_decode": (_i32, [C.POINTER(er_kv8_cache), C.POINTER(er_kv8_attention_params), _vp]),
+    "er_kv8_prefill_workspace_bytes": (C.c_int64, [C.POINTER(er_kv8_cache), C.POINTER(er_kv8_attention_params)]),
+    "er_kv8_attention_prefill": (_i32, [C.POINTER(er_kv8_cache), C.POINTER(er_kv8_attention_params), _vp]),
     "er_host_alloc": (_i32, [C.POINTER(_vp), _sz]),
     "er_host_free": (_i32, [_vp]),
 }

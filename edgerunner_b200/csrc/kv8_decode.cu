@@ -1,0 +1,750 @@
+// er_kv8_attention_decode: attention of one or a few new tokens per sequence over an 8-bit block-scaled paged cache.
+//
+// Mathematics.  With codes c and block scales a (keys) and b (values), row i of a block:  s_i = (q . ck_i) a scale,  o = sum_i p_i b cv_i /
+// sum_i p_i,  p_i = exp(s_i - m).  Codes are exact in fp16, so both contractions run on mma.sync.m16n8k16 with fp16 operands and float32
+// accumulators; the key scale multiplies the score, the value scale the probability.  The probabilities that enter the second product are
+// w = p * b / R with R the largest value scale so far (so w <= 1 whatever the scales are), carried 4096 times so that small ones stay normal
+// fp16 numbers; R and m move together and rarely.
+//
+// Work.  Bound by memory: 2 D bytes a row for 4 D flops a query head.  A persistent CTA per SM; the list of 16-token units of all (sequence, kv head,
+// row tile) items is cut evenly over the CTAs whatever the lengths are, inside a CTA the units of an item go round robin to the warps.  A warp
+// streams its units through its own ring of shared-memory stages with cp.async (16 bytes a lane, no barrier between warps, several units in
+// flight: 160 to 190 KB a SM), and runs both products of a unit alone: scores as S^T = K q^T (16 tokens x 8 query rows), outputs as O^T = V^T w^T
+// (16 dims x 8 query rows), so eight query rows fill a tile and K is an A operand as it lies in memory.  The warps of a CTA are joined in shared
+// memory at the end of an item, the CTAs that share an item by a second small launch that overlaps this one's tail.
+//
+// Lane (g, t) = (lane / 4, lane % 4).  The contraction index of the scores is relabelled so that lane t owns the dims [D/4 t, D/4 (t+1)) of a
+// row: two (D = 64: one) 16-byte reads a row.  The dims of the outputs are relabelled so that lane g owns D/8 consecutive ones: 16 (8) bytes of
+// four token rows, turned into token pairs by byte permutes.  Stage layout: 16-byte chunks XORed so that both reads are free of bank conflicts.
+#include <algorithm>
+#include <cmath>
+
+#include "kv8.cuh"
+
+namespace er {
+namespace {
+
+constexpr int kWarps = 8, kThreads = kWarps * 32;
+constexpr float kWeightScale = 4096.f;
+
+struct Kv8Decode {
+    Kv8Cache cache;
+    const void* q;
+    void* out;
+    int64_t q_token, q_head, out_token, out_head;
+    float* partial;
+    const int32_t* starts;          // tokens of the sequences, or nullptr: query_len each
+    int num_tokens, group, query_len, window, tile_rows;
+    float scale_log2;
+};
+
+// ---- the work list ----
+// Query row r of a (sequence, kv head) is query r / group, head r % group of the kv head's group; tile_rows of them make an item.
+struct SeqRange {
+    int len, begin, n;              // rows in the cache, first query token, queries
+    int first_unit, units;          // first 16-token unit that a query can see, units of an item (at least 1: an empty one writes zeros)
+    int row_tiles;                  // 0 for a sequence without queries
+};
+__device__ __forceinline__ SeqRange seq_range(const Kv8Decode& p, int seq) {
+    SeqRange r;
+    if (p.starts == nullptr) {
+        r.begin = seq * p.query_len;
+        r.n = p.query_len;
+    } else {
+        r.begin = __ldg(p.starts + seq);
+        r.n = __ldg(p.starts + seq + 1) - r.begin;
+        if (r.begin < 0 || r.n < 0 || r.begin > p.num_tokens - r.n) r.n = 0;
+    }
+    r.row_tiles = (r.n * p.group + p.tile_rows - 1) / p.tile_rows;
+    r.len = max(0, min(__ldg(p.cache.lens + seq), p.cache.table_width * p.cache.page_size));   // rows behind the table have no page
+    const int lo = p.window > 0 ? max(0, r.len - r.n - p.window + 1) : 0;
+    r.first_unit = lo / kKv8Unit;
+    r.units = max(1, (r.len + kKv8Unit - 1) / kKv8Unit - r.first_unit);
+    return r;
+}
+struct Place {        // a position in the list
+    int seq, item;    // item of the sequence: kv head * row_tiles + row tile
+    int unit;         // unit of the item
+    SeqRange r;
+    __device__ __forceinline__ void next_item(const Kv8Decode& p) {   // only where there is one
+        unit = 0;
+        if (++item == p.cache.num_kv_heads * r.row_tiles) {
+            item = 0;
+            do r = seq_range(p, ++seq); while (r.row_tiles == 0);
+        }
+    }
+    // The first and the last row that some query row of the item's tile sees, without regard to the length of the cache.
+    __device__ __forceinline__ int first_query(const Kv8Decode& p) const { return item % r.row_tiles * p.tile_rows / p.group; }
+    __device__ __forceinline__ int last_query(const Kv8Decode& p) const {
+        return (min(r.n * p.group, (item % r.row_tiles + 1) * p.tile_rows) - 1) / p.group;
+    }
+    // Of the `count` units from `unit` on, those [u0, u1) that the tile sees anything of.
+    __device__ __forceinline__ void visible(const Kv8Decode& p, int count, int& u0, int& u1) const {
+        const int base = first_unit_token() / kKv8Unit, end = r.len - r.n + last_query(p) + 1;      // rows below `end`
+        const int lo = p.window > 0 ? max(0, r.len - r.n + first_query(p) - p.window + 1) / kKv8Unit : 0;
+        u0 = max(0, lo - base);
+        u1 = min(count, max(0, end + kKv8Unit - 1) / kKv8Unit - base);
+    }
+    __device__ __forceinline__ int first_unit_token() const { return (r.first_unit + unit) * kKv8Unit; }
+};
+// Total units, by every thread of the CTA (scratch: kWarps + 1 values).
+__device__ int64_t total_units(const Kv8Decode& p, int64_t* scratch) {
+    int64_t sum = 0;
+    for (int s = threadIdx.x; s < p.cache.num_seqs; s += blockDim.x) {
+        const SeqRange r = seq_range(p, s);
+        sum += static_cast<int64_t>(r.units) * r.row_tiles;
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    sum = 0;
+    for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) sum += scratch[w];
+    __syncthreads();
+    return sum * p.cache.num_kv_heads;
+}
+// The place of unit `at` (0 <= at < total), by every thread of the CTA: warp 0 walks the sequences 32 at a time.
+__device__ Place find_place(const Kv8Decode& p, int64_t at, Place* shared_place) {
+    if (threadIdx.x < 32) {
+        int64_t before = 0;
+        for (int s0 = 0; s0 < p.cache.num_seqs; s0 += 32) {
+            const int s = s0 + static_cast<int>(threadIdx.x);
+            SeqRange r{};
+            if (s < p.cache.num_seqs) r = seq_range(p, s);
+            const int64_t mine = static_cast<int64_t>(r.units) * r.row_tiles * p.cache.num_kv_heads;
+            int64_t incl = mine;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int64_t o = __shfl_up_sync(0xffffffffu, incl, off);
+                if (static_cast<int>(threadIdx.x) >= off) incl += o;
+            }
+            const int64_t start = before + incl - mine;
+            const bool here = mine > 0 && at >= start && at < start + mine;
+            if (here) {
+                Place pl;
+                pl.seq = s;
+                pl.r = r;
+                pl.item = static_cast<int>((at - start) / pl.r.units);
+                pl.unit = static_cast<int>((at - start) % pl.r.units);
+                *shared_place = pl;
+            }
+            before += __shfl_sync(0xffffffffu, incl, 31);
+            if (__any_sync(0xffffffffu, here)) break;
+        }
+    }
+    __syncthreads();
+    const Place pl = *shared_place;
+    __syncthreads();
+    return pl;
+}
+// CTA c of n takes the units [total c / n, total (c + 1) / n); at least kWarps units to a CTA, so that short work stays together.
+__device__ __forceinline__ int used_ctas(int64_t total, int ctas) { return static_cast<int>(min(static_cast<int64_t>(ctas), (total + kWarps - 1) / kWarps)); }
+__device__ __forceinline__ int64_t cta_begin(int64_t total, int n, int c) { return total * c / n; }
+__device__ __forceinline__ int cta_of(int64_t total, int n, int64_t unit) { return static_cast<int>(((unit + 1) * n - 1) / total); }
+
+// ---- instructions ----
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void split_half2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = half2_bits(a - f.x, b - f.y);
+}
+
+template <int D> struct Stage {
+    static constexpr int kSide = kKv8Unit * D, kBytes = 2 * kSide;
+    static constexpr int kChunks = kSide / 16;   // 16-byte chunks of one side
+    // byte offset of chunk c of row r inside a side
+    static __device__ __forceinline__ int at(int r, int c) {
+        if constexpr (D == 128) return r * 128 + ((c ^ (r & 7)) << 4);
+        else return (r >> 1) * 128 + (((((r & 1) << 2) | c) ^ ((r >> 1 & 3) << 1)) << 4);
+    }
+};
+template <int NT> __host__ __device__ constexpr int decode_rows() { return 8 * NT; }
+template <int D, int NT> __host__ __device__ constexpr int decode_stages() {
+    return D == 128 ? (NT == 1 ? 6 : 4) : (NT == 1 ? 12 : 10);
+}
+template <int D, int NT> __host__ __device__ constexpr int join_floats() { return kWarps * 8 * NT * (D + 4); }
+template <int D, int NT> __host__ __device__ constexpr int decode_smem() {
+    return kWarps * decode_stages<D, NT>() * (Stage<D>::kBytes + 8) + (join_floats<D, NT>() + kWarps * 8 * NT * 2) * 4 + 128;
+}
+// One partial: max, sum, -, - and the unnormalised row.
+template <int D> __host__ __device__ constexpr int partial_stride() { return D + 4; }
+
+template <typename T, int D, bool E4M3, int NT>
+__global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_constant__ Kv8Decode p) {
+    constexpr bool kSplit = sizeof(T) == 4;      // float32: queries and weights as a high and a low half
+    static_assert(!kSplit || NT == 1, "");
+    constexpr int kRows = decode_rows<NT>(), kStages = decode_stages<D, NT>();
+    constexpr int KK = D / 16, MT = D / 16, kWords = D / 16;   // k-steps of the scores; m-tiles of the outputs; 4-byte words of a lane's part of a key row
+    constexpr int kOwn = D / 8;                                 // dims of a lane g in the outputs
+    constexpr int kJoinRow = D + 4;
+    extern __shared__ __align__(16) uint8_t smem[];
+    uint8_t* stages = smem;
+    float* stage_scales = reinterpret_cast<float*>(smem + kWarps * kStages * Stage<D>::kBytes);
+    float* join = stage_scales + kWarps * kStages * 2;
+    float* join_ml = join + join_floats<D, NT>();
+    int64_t* scratch = reinterpret_cast<int64_t*>(join_ml + kWarps * kRows * 2);
+    const Kv8Cache& c = p.cache;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    const int64_t total = total_units(p, scratch);
+    const int n = used_ctas(total, gridDim.x), cta = blockIdx.x;
+    if (cta == 0) {                 // what the host cannot see
+        for (int s = threadIdx.x; s < c.num_seqs; s += kThreads) {
+            if (__ldg(c.lens + s) > c.table_width * c.page_size) kv8_report(c, ER_ERR_OUT_OF_PAGES);
+            if (__ldg(c.lens + s) < 0) kv8_report(c, ER_ERR_SHAPE);
+            if (p.starts != nullptr && seq_range(p, s).n != __ldg(p.starts + s + 1) - __ldg(p.starts + s)) kv8_report(c, ER_ERR_SHAPE);
+        }
+    }
+    if (cta >= n) return;
+    int64_t left = cta_begin(total, n, cta + 1) - cta_begin(total, n, cta);       // units of this CTA not yet walked over
+    Place at = find_place(p, cta_begin(total, n, cta), reinterpret_cast<Place*>(scratch));
+
+    // ---- producer: this warp's units, kStages - 1 ahead ----
+    uint8_t* my_stages = stages + warp * kStages * Stage<D>::kBytes;
+    float* my_scales = stage_scales + warp * kStages * 2;
+    Place pp = at;                  // segment the producer is in
+    int64_t pleft = left;           // units from pp.unit on
+    int pseg = static_cast<int>(min(static_cast<int64_t>(pp.r.units - pp.unit), pleft));   // units of the segment
+    int pu, pend;                   // next unit of the segment for this warp; end of those that are worth a look
+    int ppage = -1;                 // its page
+    bool pmore = true;
+    pp.visible(p, pseg, pu, pend);
+    pu += warp;
+    auto settle = [&]() {           // moves on to the segment that holds this warp's next unit and looks its page up
+        while (pu >= pend) {
+            pleft -= pseg;
+            if (pleft <= 0) { pmore = false; return; }
+            pp.next_item(p);
+            pseg = static_cast<int>(min(static_cast<int64_t>(pp.r.units), pleft));
+            pp.visible(p, pseg, pu, pend);
+            pu += warp;
+        }
+        ppage = kv8_page(c, pp.seq, (pp.r.first_unit + pp.unit + pu) * kKv8Unit);
+    };
+    int pstage = 0;
+    auto produce = [&]() {          // one commit group, empty when there is nothing left
+        if (pmore) {
+            const int tok = (pp.r.first_unit + pp.unit + pu) * kKv8Unit;
+            float* sc = my_scales + pstage * 2;
+            if (tok < pp.r.len && ppage >= 0) {
+                const int head = pp.item / pp.r.row_tiles, in_page = tok % c.page_size;
+                const int64_t row = (static_cast<int64_t>(ppage) * c.num_kv_heads + head) * c.page_size + in_page;
+                const uint32_t dst = smem_u32(my_stages + pstage * Stage<D>::kBytes);
+#pragma unroll
+                for (int i = 0; i < 2 * Stage<D>::kChunks / 32; ++i) {
+                    const int idx = i * 32 + lane, side = idx / Stage<D>::kChunks, k = idx % Stage<D>::kChunks;
+                    const int r = k / (D / 16), ch = k % (D / 16);
+                    cp_async16(dst + side * Stage<D>::kSide + Stage<D>::at(r, ch), c.codes[side] + row * D + k * 16);
+                }
+                if (lane < 2) cp_async4(smem_u32(sc + lane), c.scales[lane] + row / c.scale_block);
+            } else {                // nothing to see: no row yet, or no page
+                if (lane < 2) sc[lane] = -1.f;
+                if (tok < pp.r.len && lane == 0) kv8_report(c, ER_ERR_OUT_OF_PAGES);
+            }
+            pu += kWarps;
+            settle();
+        }
+        cp_async_commit();
+        pstage = pstage + 1 == kStages ? 0 : pstage + 1;
+    };
+    settle();
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) produce();
+
+    int cstage = 0;
+    bool first_segment = true;
+    while (left > 0) {
+        const int seg = static_cast<int>(min(static_cast<int64_t>(at.r.units - at.unit), left));
+        const int head = at.item / at.r.row_tiles, rt = at.item % at.r.row_tiles, rows = at.r.n * p.group;
+        const int past = at.r.len - at.r.n;            // position of query 0
+        int u0, u1;
+        at.visible(p, seg, u0, u1);
+        const int all_see_to = past + at.first_query(p), all_see_from = past + at.last_query(p) - p.window + 1;
+        // ---- queries of this lane's column g: dims [D/4 t, D/4 (t+1)), scaled to at most 1 by a power of two ----
+        uint32_t qh[NT][KK][2], ql[kSplit ? NT : 1][kSplit ? KK : 1][2];
+        float qscale[NT][2];        // of the columns 2t, 2t + 1
+        int limit[NT][2];           // last row that they see
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = rt * kRows + nt * 8 + g;
+            float x[D / 4];
+#pragma unroll
+            for (int i = 0; i < D / 4; ++i) x[i] = 0.f;
+            if (r < rows) {
+                const int qi = r / p.group, qh_ = head * p.group + r % p.group;
+                const T* src = static_cast<const T*>(p.q) + static_cast<int64_t>(at.r.begin + qi) * p.q_token + qh_ * p.q_head + (D / 4) * t;
+#pragma unroll
+                for (int i = 0; i < D / 4; i += Act<T>::kVec) Act<T>::unpack(__ldg(reinterpret_cast<const uint4*>(src + i)), x + i);
+            }
+            uint32_t mx = 0;
+#pragma unroll
+            for (int i = 0; i < D / 4; ++i) mx = max(mx, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+            mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const uint32_t ex = min(max(mx >> 23, 1u), 252u);     // an infinity or a NaN goes through as it is
+            const float down = __uint_as_float((253u - ex) << 23) , up = __uint_as_float((ex + 1u) << 23);   // 2^(126 - ex), 2^(ex - 126)
+#pragma unroll
+            for (int k = 0; k < KK; ++k) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float a = x[4 * k + 2 * j] * down, b = x[4 * k + 2 * j + 1] * down;
+                    if constexpr (kSplit) split_half2(a, b, qh[nt][k][j], ql[nt][k][j]);
+                    else qh[nt][k][j] = half2_bits(a, b);
+                }
+            }
+            const float f = up * p.scale_log2;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                qscale[nt][j] = __shfl_sync(0xffffffffu, f, (2 * t + j) * 4);
+                const int rr = rt * kRows + nt * 8 + 2 * t + j;
+                limit[nt][j] = past + min(rr, rows - 1) / p.group;
+            }
+        }
+        float o[NT][MT][4], m[NT][2], l[NT][2], R = 0.f, inv_R = 0.f;
+        float keep[kSplit ? MT : 1][4];     // float32: the tensor cores' sums are moved here every 16 units (their accumulators round towards zero)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) { o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f; }
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < (kSplit ? MT : 1); ++i) keep[i][0] = keep[i][1] = keep[i][2] = keep[i][3] = 0.f;
+        int since = 0;
+
+        for (int u = u0 + warp; u < u1; u += kWarps) {
+            cp_async_wait<kStages - 2>();
+            __syncwarp();
+            const uint8_t* ks = my_stages + cstage * Stage<D>::kBytes;
+            const uint8_t* vs = ks + Stage<D>::kSide;
+            const float kscale = my_scales[cstage * 2];
+            float vscale = my_scales[cstage * 2 + 1];
+            const int tok0 = (at.r.first_unit + at.unit + u) * kKv8Unit;
+            // ---- scores: 16 tokens x 8 NT query rows ----
+            float s[NT][4], s2[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = s2[nt][0] = s2[nt][1] = s2[nt][2] = s2[nt][3] = 0.f;
+#pragma unroll
+            for (int c16 = 0; c16 < kWords / 4; ++c16) {
+                const int ch = (kWords / 4) * t + c16;
+                const uint4 r0 = *reinterpret_cast<const uint4*>(ks + Stage<D>::at(g, ch));
+                const uint4 r1 = *reinterpret_cast<const uint4*>(ks + Stage<D>::at(g + 8, ch));
+                const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int k = 4 * c16 + i;
+                    uint32_t a0, a1, a2, a3;
+                    decode4<E4M3>(w0[i], a0, a2);
+                    decode4<E4M3>(w1[i], a1, a3);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma16816(i & 1 ? s2[nt] : s[nt], a0, a1, a2, a3, qh[nt][k][0], qh[nt][k][1]);
+                        if constexpr (kSplit) mma16816(i & 1 ? s2[nt] : s[nt], a0, a1, a2, a3, ql[nt][k][0], ql[nt][k][1]);
+                    }
+                }
+            }
+            // ---- online softmax; lane's scores: tokens g, g + 8 of the columns 2t, 2t + 1 ----
+            const bool hidden = kscale < 0.f;
+            const bool edge = hidden || tok0 + kKv8Unit - 1 > all_see_to || (p.window > 0 && tok0 < all_see_from);
+            bool rise = vscale > R;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[nt][e] = (s[nt][e] + s2[nt][e]) * (kscale * qscale[nt][e & 1]);
+                    if (edge) {
+                        const int tok = tok0 + g + 8 * (e >> 1), lim = limit[nt][e & 1];
+                        if (hidden || tok > lim || (p.window > 0 && tok <= lim - p.window)) s[nt][e] = -INFINITY;
+                    }
+                    rise |= s[nt][e] > m[nt][e & 1];
+                }
+            }
+            if (!(vscale >= 1.17549435e-38f)) vscale = isnan(vscale) ? vscale : 0.f;
+            if (__any_sync(0xffffffffu, rise)) {
+                const float R_new = fmaxf(R, vscale), down = R > 0.f ? R / R_new : 0.f;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float corr[2];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float mx = fmaxf(m[nt][j], fmaxf(s[nt][j], s[nt][2 + j]));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                        corr[j] = mx == -INFINITY ? 1.f : fast_exp2(m[nt][j] - mx);
+                        m[nt][j] = mx;
+                        l[nt][j] *= corr[j];
+                        corr[j] *= down;
+                    }
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            o[nt][i][e] *= corr[e & 1];
+                            if constexpr (kSplit) keep[i][e] *= corr[e & 1];
+                        }
+                    }
+                }
+                R = R_new;
+                inv_R = R > 0.f ? 1.f / R : 0.f;
+            }
+            const float wf = vscale * inv_R * kWeightScale;
+            uint32_t wh[NT][2], wl[kSplit ? NT : 1][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float pr = s[nt][e] == -INFINITY ? 0.f : fast_exp2(s[nt][e] - m[nt][e & 1]);
+                    l[nt][e & 1] += pr;
+                    w[e] = s[nt][e] == -INFINITY ? 0.f : pr * wf;      // a hidden row of a block with a NaN scale weighs nothing
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if constexpr (kSplit) {
+                        uint32_t hi, lo;
+                        split_half2(w[2 * h], w[2 * h + 1], hi, lo);
+                        wh[nt][h] = transpose8x8(hi);
+                        wl[nt][h] = transpose8x8(lo);
+                    } else {
+                        wh[nt][h] = transpose8x8(half2_bits(w[2 * h], w[2 * h + 1]));
+                    }
+                }
+            }
+            // ---- outputs: D dims x 8 NT query rows, token pairs (2t, 2t + 1) and 8 further ----
+            {
+                uint32_t v[4][kOwn / 4];
+#pragma unroll
+                for (int rr = 0; rr < 4; ++rr) {
+                    const int row = 2 * t + (rr & 1) + 8 * (rr >> 1);
+                    if constexpr (D == 128) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(vs + Stage<D>::at(row, g));
+                        v[rr][0] = x.x; v[rr][1] = x.y; v[rr][2 % (kOwn / 4)] = x.z; v[rr][3 % (kOwn / 4)] = x.w;
+                    } else {
+                        const uint2 x = *reinterpret_cast<const uint2*>(vs + Stage<D>::at(row, g >> 1) + (g & 1) * 8);
+                        v[rr][0] = x.x; v[rr][1] = x.y;
+                    }
+                    if (edge && (hidden || tok0 + row >= at.r.len)) {   // bytes that are nobody's row may be codes of NaN
+#pragma unroll
+                        for (int i = 0; i < kOwn / 4; ++i) v[rr][i] = 0u;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kOwn / 4; ++i) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {      // dims 4 i + 2 h, 4 i + 2 h + 1 of the lane's own
+                        uint32_t a0, a1, a2, a3;
+                        decode4<E4M3>(__byte_perm(v[0][i], v[1][i], h ? 0x7362 : 0x5140), a0, a1);
+                        decode4<E4M3>(__byte_perm(v[2][i], v[3][i], h ? 0x7362 : 0x5140), a2, a3);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma16816(o[nt][2 * i + h], a0, a1, a2, a3, wh[nt][0], wh[nt][1]);
+                            if constexpr (kSplit) mma16816(o[nt][2 * i + h], a0, a1, a2, a3, wl[nt][0], wl[nt][1]);
+                        }
+                    }
+                }
+            }
+            if constexpr (kSplit) {
+                if (++since == 16) {
+                    since = 0;
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) { keep[i][e] += o[0][i][e]; o[0][i][e] = 0.f; }
+                    }
+                }
+            }
+            __syncwarp();           // every lane has read the stage before it is filled again
+            cstage = cstage + 1 == kStages ? 0 : cstage + 1;
+            produce();
+        }
+
+        // ---- join the warps of the CTA ----
+        const float out_scale = R * (1.f / kWeightScale);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float x = l[nt][j];
+                x += __shfl_xor_sync(0xffffffffu, x, 4);
+                x += __shfl_xor_sync(0xffffffffu, x, 8);
+                x += __shfl_xor_sync(0xffffffffu, x, 16);
+                const int col = nt * 8 + 2 * t + j;
+                if (g == 0) {
+                    join_ml[(warp * kRows + col) * 2] = m[nt][j];
+                    join_ml[(warp * kRows + col) * 2 + 1] = x;
+                }
+                float* row = join + (warp * kRows + col) * kJoinRow + 2 * g;   // dim kOwn g + 2 i + e at 16 i + 2 g + e
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    float a = o[nt][i][j], b = o[nt][i][2 + j];
+                    if constexpr (kSplit) { a += keep[i][j]; b += keep[i][2 + j]; }
+                    *reinterpret_cast<float2*>(row + 16 * i) = make_float2(a * out_scale, b * out_scale);
+                }
+            }
+        }
+        __syncthreads();
+        const bool whole = at.unit == 0 && seg == at.r.units;
+        const int cols = min(kRows, rows - rt * kRows);
+        for (int e = threadIdx.x; e < cols * (D / 2); e += kThreads) {
+            const int col = e / (D / 2), d = (e % (D / 2)) * 2;
+            float M = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, join_ml[(w * kRows + col) * 2]);
+            const float M0 = M == -INFINITY ? 0.f : M;
+            float L = 0.f, x = 0.f, y = 0.f;
+            const int pos = 16 * ((d % kOwn) / 2) + 2 * (d / kOwn);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float f = fast_exp2(join_ml[(w * kRows + col) * 2] - M0);
+                const float2 v = *reinterpret_cast<const float2*>(join + (w * kRows + col) * kJoinRow + pos);
+                L = fmaf(f, join_ml[(w * kRows + col) * 2 + 1], L);
+                x = fmaf(f, v.x, x);
+                y = fmaf(f, v.y, y);
+            }
+            if (whole) {
+                const int r = rt * kRows + col;
+                const float inv = L == 0.f ? 0.f : 1.f / L;
+                T* dst = static_cast<T*>(p.out) + static_cast<int64_t>(at.r.begin + r / p.group) * p.out_token + (head * p.group + r % p.group) * p.out_head + d;
+                store_pair(dst, x * inv, y * inv);
+            } else {
+                float* dst = p.partial + ((static_cast<int64_t>(cta) * 2 + (first_segment ? 0 : 1)) * kRows + col) * partial_stride<D>();
+                if (d == 0) { dst[0] = M; dst[1] = L; }
+                store_pair(dst + 4 + d, x, y);
+            }
+        }
+        __syncthreads();
+        first_segment = false;
+        left -= seg;
+        if (left > 0) {
+            at.next_item(p);
+        }
+    }
+    cp_async_wait<0>();
+}
+
+// Joins the partials of the items that more than one CTA worked on.  At most one item begins in a CTA's range and goes on behind it: block
+// (c, row) looks for that of CTA c and, if there is one, joins query row `row` of it: its warps take the parts in turn, a lane D / 32 dims.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kThreads) kv8_decode_join_kernel(const __grid_constant__ Kv8Decode p) {
+    constexpr int kRows = decode_rows<NT>(), V = D / 32;
+    __shared__ int64_t scratch[16];
+    __shared__ float ml[kWarps][2], rows[kWarps][D];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.y;
+    // every block waits, also one with nothing to do: this grid must not end before the one whose partials it stands for
+    auto wait = [] { asm volatile("griddepcontrol.wait;" ::: "memory"); };
+    const int64_t total = total_units(p, scratch);
+    const int n = used_ctas(total, gridDim.x), cta = blockIdx.x;
+    if (cta >= n - 1) { wait(); return; }
+    const int64_t begin = cta_begin(total, n, cta), end = cta_begin(total, n, cta + 1);
+    const Place last = find_place(p, end - 1, reinterpret_cast<Place*>(scratch));
+    const int64_t item_begin = end - 1 - last.unit, item_end = item_begin + last.r.units;
+    const int head = last.item / last.r.row_tiles, r = (last.item % last.r.row_tiles) * kRows + row;
+    const int last_cta = cta_of(total, n, item_end - 1);
+    wait();
+    if (item_end <= end || item_begin < begin || r >= last.r.n * p.group) return;
+    float M = -INFINITY, L = 0.f, acc[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = 0.f;
+    for (int c = cta + warp; c <= last_cta; c += kWarps) {
+        const int slot = c == cta && item_begin > begin ? 1 : 0;
+        const float* src = p.partial + ((static_cast<int64_t>(c) * 2 + slot) * kRows + row) * partial_stride<D>();
+        const float m = __ldcg(src), m_new = fmaxf(M, m), m0 = m_new == -INFINITY ? 0.f : m_new;
+        const float f_old = fast_exp2(M - m0), f = fast_exp2(m - m0);
+        L = L * f_old + __ldcg(src + 1) * f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = acc[i] * f_old + __ldcg(src + 4 + lane * V + i) * f;
+        M = m_new;
+    }
+    if (lane == 0) { ml[warp][0] = M; ml[warp][1] = L; }
+#pragma unroll
+    for (int i = 0; i < V; ++i) rows[warp][lane * V + i] = acc[i];
+    __syncthreads();
+    if (threadIdx.x < D / 2) {
+        const int d = threadIdx.x * 2;
+        float A = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) A = fmaxf(A, ml[w][0]);
+        const float A0 = A == -INFINITY ? 0.f : A;
+        float S = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float f = fast_exp2(ml[w][0] - A0);
+            S = fmaf(f, ml[w][1], S);
+            x = fmaf(f, rows[w][d], x);
+            y = fmaf(f, rows[w][d + 1], y);
+        }
+        const float inv = S == 0.f ? 0.f : 1.f / S;
+        T* dst = static_cast<T*>(p.out) + static_cast<int64_t>(last.r.begin + r / p.group) * p.out_token + (head * p.group + r % p.group) * p.out_head + d;
+        store_pair(dst, x * inv, y * inv);
+    }
+}
+
+int sm_count() {
+    int device = 0, sms = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) sms = 0;
+    return sms;
+}
+// Two columns of eight query rows where they are needed and fit: float32 rows take two operands each and stay at eight.
+int tiles_of(uint32_t type, int rows) { return type != ER_TYPE_FLOAT32 && rows > 8 ? 2 : 1; }
+
+template <typename T, int D, bool E4M3, int NT>
+int32_t launch(Kv8Decode& p, int most_rows, int sms, cudaStream_t s) {
+    constexpr int kSmem = decode_smem<D, NT>();
+    static_assert(kSmem <= 232448, "decode kernel exceeds the shared memory of an sm_100 CTA");
+    p.tile_rows = 8 * NT;
+    cudaError_t e = cudaFuncSetAttribute(kv8_decode_kernel<T, D, E4M3, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e != cudaSuccess) return kv8_launched(e, "kv8_decode_kernel");
+    kv8_decode_kernel<T, D, E4M3, NT><<<sms, kThreads, kSmem, s>>>(p);
+    const int32_t rc = kv8_launched(cudaGetLastError(), "kv8_decode_kernel");
+    if (rc != ER_OK) return rc;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(sms, p.starts != nullptr ? 8 * NT : std::min(8 * NT, most_rows));
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, kv8_decode_join_kernel<T, D, NT>, p);
+    return kv8_launched(e, "kv8_decode_join_kernel");
+}
+template <typename T, int D, bool E4M3>
+int32_t launch_rows(Kv8Decode& p, int most_rows, int sms, cudaStream_t s) {
+    if constexpr (sizeof(T) == 2) {
+        if (tiles_of(ER_TYPE_FLOAT16, most_rows) == 2) return launch<T, D, E4M3, 2>(p, most_rows, sms, s);
+    }
+    return launch<T, D, E4M3, 1>(p, most_rows, sms, s);
+}
+template <typename T>
+int32_t launch_shape(Kv8Decode& p, int most_rows, int head_dim, bool e4m3, int sms, cudaStream_t s) {
+    if (head_dim == 128) return e4m3 ? launch_rows<T, 128, true>(p, most_rows, sms, s) : launch_rows<T, 128, false>(p, most_rows, sms, s);
+    return e4m3 ? launch_rows<T, 64, true>(p, most_rows, sms, s) : launch_rows<T, 64, false>(p, most_rows, sms, s);
+}
+
+}  // namespace
+
+// Checks shared by the two attention operators.
+int32_t kv8_check_attention(const er_kv8_cache* c, const er_kv8_attention_params* u) {
+    if (!u->q || !u->out) return report_error(ER_ERR_INVALID_ARGUMENT, "null argument");
+    if (u->type > ER_TYPE_BFLOAT16) return report_error(ER_ERR_INVALID_ARGUMENT, "type must be one of ER_TYPE_*");
+    if (u->num_heads == 0 || u->num_heads % c->num_kv_heads != 0) return report_error(ER_ERR_SHAPE, "num_heads must be a multiple of num_kv_heads");
+    if (u->num_heads > 65535u || static_cast<uint64_t>(u->num_tokens) * (u->num_heads / c->num_kv_heads) > (1u << 30))
+        return report_error(ER_ERR_UNSUPPORTED, "num_heads beyond 65535, or more than 2^30 query rows of a kv head");
+    if (!kv8_aligned(u->q) || !kv8_aligned(u->out)) return report_error(ER_ERR_INVALID_ARGUMENT, "q and out must be 16-byte aligned");
+    const int64_t vec = u->type == ER_TYPE_FLOAT32 ? 4 : 8;
+    for (const int64_t st : {u->q_token_stride, u->q_head_stride, u->out_token_stride, u->out_head_stride})
+        if (st < 0 || st % vec != 0) return report_error(ER_ERR_INVALID_ARGUMENT, "strides must be multiples of 16 bytes");
+    if (!(u->softmax_scale >= 0.f && std::isfinite(u->softmax_scale))) return report_error(ER_ERR_INVALID_ARGUMENT, "softmax_scale must be finite and not negative");
+    if (u->num_tokens > 0x7FFFFF00u || u->sliding_window > 0x7FFFFFFFu) return report_error(ER_ERR_UNSUPPORTED, "num_tokens or sliding_window beyond 2^31");
+    return ER_OK;
+}
+
+// Rows of the longest sequence, as far as the host knows.
+static int most_rows_of(const er_kv8_cache* c, const er_kv8_attention_params* u, bool ragged) {
+    uint64_t n = u->query_len;
+    if (ragged) n = u->max_query_len > 0 ? std::min(u->max_query_len, u->num_tokens) : u->num_tokens;
+    return static_cast<int>(std::min<uint64_t>(n * (u->num_heads / c->num_kv_heads), 1u << 30));
+}
+
+int64_t kv8_decode_workspace(const er_kv8_cache* c, const er_kv8_attention_params* u, bool ragged) {
+    const int sms = sm_count();
+    if (sms == 0) return report_error(ER_ERR_CUDA, "no CUDA device (no CPU fallback)");
+    return static_cast<int64_t>(sms) * 2 * 8 * tiles_of(u->type, most_rows_of(c, u, ragged)) * (c->head_dim + 4) * 4;
+}
+
+int32_t kv8_check_workspace(const er_kv8_attention_params* u, int64_t need) {
+    if (need < 0) return static_cast<int32_t>(need);
+    if (need > 0 && (!u->workspace || u->workspace_bytes < static_cast<uint64_t>(need)))
+        return report_error(ER_ERR_INVALID_ARGUMENT, "workspace is smaller than er_kv8_*_workspace_bytes");
+    if (!kv8_aligned(u->workspace)) return report_error(ER_ERR_INVALID_ARGUMENT, "workspace must be 16-byte aligned");
+    return ER_OK;
+}
+
+// The kernel over a checked call; ragged: queries by query_starts.
+int32_t kv8_launch_decode(const Kv8Cache& cache, uint32_t head_dim, bool e4m3, const er_kv8_attention_params* u, int most_rows, bool ragged, cudaStream_t s) {
+    Kv8Decode p{};
+    p.cache = cache;
+    p.q = u->q; p.out = u->out;
+    p.q_token = u->q_token_stride; p.q_head = u->q_head_stride; p.out_token = u->out_token_stride; p.out_head = u->out_head_stride;
+    p.partial = static_cast<float*>(u->workspace);
+    p.starts = ragged ? u->query_starts : nullptr;
+    p.num_tokens = static_cast<int>(u->num_tokens);
+    p.group = static_cast<int>(u->num_heads) / cache.num_kv_heads;
+    p.query_len = static_cast<int>(u->query_len); p.window = static_cast<int>(u->sliding_window);
+    p.scale_log2 = kv8_scale_log2(u->softmax_scale, head_dim);
+    const int sms = sm_count(), d = static_cast<int>(head_dim);
+    switch (u->type) {
+        case ER_TYPE_FLOAT32: return launch_shape<float>(p, most_rows, d, e4m3, sms, s);
+        case ER_TYPE_FLOAT16: return launch_shape<__half>(p, most_rows, d, e4m3, sms, s);
+        default: return launch_shape<__nv_bfloat16>(p, most_rows, d, e4m3, sms, s);
+    }
+}
+
+}  // namespace er
+
+extern "C" int64_t er_kv8_decode_workspace_bytes(const er_kv8_cache* cache, const er_kv8_attention_params* u) {
+    using namespace er;
+    if (!cache || !u || cache->num_kv_heads == 0) return report_error(ER_ERR_INVALID_ARGUMENT, "null argument");
+    return kv8_decode_workspace(cache, u, false);
+}
+
+extern "C" int32_t er_kv8_attention_decode(const er_kv8_cache* cache, const er_kv8_attention_params* u, void* stream) {
+    using namespace er;
+    if (!cache || !u) return report_error(ER_ERR_INVALID_ARGUMENT, "null argument");
+    Kv8Cache c{};
+    int32_t rc = kv8_check(cache, &c);
+    if (rc == ER_OK) rc = kv8_check_attention(cache, u);
+    if (rc != ER_OK) return rc;
+    if (u->query_len == 0 || u->query_len > 16) return report_error(ER_ERR_UNSUPPORTED, "query_len must be between 1 and 16 (longer runs: er_kv8_attention_prefill)");
+    if (u->num_tokens != static_cast<uint64_t>(cache->num_seqs) * u->query_len) return report_error(ER_ERR_SHAPE, "num_tokens must be num_seqs * query_len");
+    rc = kv8_check_device(cache);
+    if (rc == ER_OK) rc = kv8_check_workspace(u, kv8_decode_workspace(cache, u, false));
+    if (rc != ER_OK || cache->num_seqs == 0) return rc;
+    return kv8_launch_decode(c, cache->head_dim, cache->format == ER_KV8_E4M3, u, most_rows_of(cache, u, false), false, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int64_t er_kv8_prefill_workspace_bytes(const er_kv8_cache* cache, const er_kv8_attention_params* u) {
+    using namespace er;
+    if (!cache || !u || cache->num_kv_heads == 0) return report_error(ER_ERR_INVALID_ARGUMENT, "null argument");
+    return kv8_decode_workspace(cache, u, true);
+}
+
+extern "C" int32_t er_kv8_attention_prefill(const er_kv8_cache* cache, const er_kv8_attention_params* u, void* stream) {
+    using namespace er;
+    if (!cache || !u) return report_error(ER_ERR_INVALID_ARGUMENT, "null argument");
+    Kv8Cache c{};
+    int32_t rc = kv8_check(cache, &c);
+    if (rc == ER_OK) rc = kv8_check_attention(cache, u);
+    if (rc != ER_OK) return rc;
+    if (!u->query_starts) return report_error(ER_ERR_INVALID_ARGUMENT, "query_starts is needed for a ragged batch");
+    rc = kv8_check_device(cache);
+    if (rc == ER_OK) rc = kv8_check_workspace(u, kv8_decode_workspace(cache, u, true));
+    if (rc != ER_OK || cache->num_seqs == 0 || u->num_tokens == 0) return rc;
+    return kv8_launch_decode(c, cache->head_dim, cache->format == ER_KV8_E4M3, u, most_rows_of(cache, u, true), true, static_cast<cudaStream_t>(stream));
+}

@@ -436,6 +436,99 @@ int32_t er_peer_buffer_open(const uint8_t* handle /* 64 bytes */, void** device_
 int32_t er_peer_buffer_close(void* opened_ptr);
 int32_t er_peer_buffer_destroy(void* device_ptr);
 
+/* ---- activations of 16 or 32 bits; head norms with the rotation; an 8-bit paged cache with one scale per block of tokens ----
+ * No counterpart in the reference.  These operators keep no state: a paged cache is the buffers that the caller names in an
+ * er_kv8_cache, positions and lengths come from device arrays, nothing is allocated, every call may be captured into a graph, and
+ * calls on different streams are independent as long as their outputs, pages and workspaces are.  Batches are ragged: sequence s of
+ * num_seqs has the tokens query_starts[s] .. query_starts[s + 1) of the call, its newest ones.  The device that owns the buffers has
+ * to be current.  Data-dependent mistakes (a table entry without a page, starts that run backwards) cannot be seen on the host: the
+ * kernels skip what they would touch and set the cache's status word. */
+enum { ER_TYPE_FLOAT32 = 0, ER_TYPE_FLOAT16 = 1, ER_TYPE_BFLOAT16 = 2 };
+/* Code formats: E4M3 with power-of-two scales (growing a block's scale re-rounds nothing), int8 with scales amax / 127. */
+enum { ER_KV8_E4M3 = 0, ER_KV8_INT8 = 1 };
+
+/* Norms of the query and key heads and their rotation in one pass:  y = R(position) . (x / sqrt(mean(x^2) + rms_eps) * weight),
+ * the pairs (i, i + head_dim / 2) of the first head_dim / 2 * partial_rotary_factor rotated by position * rope_theta^(-2 i /
+ * head_dim) / rope_scaling (angles in 64 bits), arithmetic in 32 bits, one rounding at the end.  A NULL weight: no norm for that
+ * tensor; partial_rotary_factor 0: no rotation (positions may be NULL).  Strides are in elements; the elements of a head are
+ * contiguous.  in and out are the same buffer with the same strides, or do not overlap.  k NULL: queries only.  head_dim: a multiple of 16 up to
+ * 256.  Buffers and strides are 16-byte aligned; weights are float32. */
+typedef struct {
+    const void* q;
+    void* q_out;
+    const void* k;
+    void* k_out;
+    int64_t q_token_stride, q_head_stride, q_out_token_stride, q_out_head_stride;
+    int64_t k_token_stride, k_head_stride, k_out_token_stride, k_out_head_stride;
+    const int32_t* positions;    /* device [num_tokens], >= 0 */
+    const float* q_norm_weight;  /* device [head_dim] or NULL */
+    const float* k_norm_weight;
+    uint32_t num_tokens, num_heads, num_kv_heads, head_dim;
+    uint32_t type;               /* ER_TYPE_* of q, k and the outputs */
+    float rms_eps, rope_theta, rope_scaling, partial_rotary_factor;
+} er_qk_norm_rope_params;
+int32_t er_qk_norm_rope(const er_qk_norm_rope_params* params, void* stream);
+
+/* A batch's view of an 8-bit paged cache.  Element = code * scale; scale >= 0, one per (page, kv head, block of scale_block tokens). */
+typedef struct {
+    uint8_t* keys;               /* device [num_pages][num_kv_heads][page_size][head_dim] codes */
+    uint8_t* values;
+    float* key_scales;           /* device [num_pages][num_kv_heads][page_size / scale_block] */
+    float* value_scales;
+    const int32_t* block_tables; /* device [num_seqs][block_table_stride]: page ids, one per page_size tokens; negative = no page */
+    const int32_t* kv_lens;      /* device [num_seqs]: rows of the sequence, the call's own tokens included */
+    int32_t* status;             /* device word, set to ER_ERR_OUT_OF_PAGES / ER_ERR_SHAPE by a kernel that skipped something; NULL = none */
+    uint32_t num_pages, page_size, scale_block;  /* page_size a multiple of scale_block; scale_block 16, 32, 64 or 128 */
+    uint32_t num_kv_heads, head_dim;             /* head_dim 64 or 128 */
+    uint32_t format;                             /* ER_KV8_* */
+    uint32_t num_seqs, block_table_width, block_table_stride;
+} er_kv8_cache;
+
+/* Writes the call's tokens into their pages: token i of sequence s is row kv_lens[s] - (query_starts[s + 1] - query_starts[s]) + i.
+ * Keys are normed and rotated at that position on the way (as in er_qk_norm_rope).  The scale of a block is what its largest
+ * magnitude needs; where a block holds earlier rows its scale only grows, and when it does the earlier rows' codes are
+ * re-encoded (int8: another rounding of at most half a step).  Rows behind the newest one stay as they were.  An infinity or a
+ * NaN makes its block's scale NaN.  A page that two sequences share must not be written by either.
+ * query_starts NULL: one token per sequence (num_tokens = num_seqs). */
+typedef struct {
+    const void* k;               /* device [num_tokens][num_kv_heads][head_dim] */
+    const void* v;
+    int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;   /* elements, 16-byte multiples */
+    const int32_t* query_starts; /* device [num_seqs + 1] or NULL */
+    const float* k_norm_weight;  /* device [head_dim] or NULL */
+    uint32_t num_tokens;
+    uint32_t type;               /* ER_TYPE_* of k and v */
+    float rms_eps, rope_theta, rope_scaling, partial_rotary_factor;
+} er_kv8_append_params;
+int32_t er_kv8_append(const er_kv8_cache* cache, const er_kv8_append_params* params, void* stream);
+
+/* Attention over the cache: query i of a sequence with n queries sits at position p = kv_lens - n + i and sees the rows
+ * max(0, p - sliding_window + 1) .. p (sliding_window 0: 0 .. p).  A query that sees nothing gets zeros.  softmax_scale 0 ->
+ * 1 / sqrt(head_dim).  num_heads is a multiple of num_kv_heads, any group.
+ * er_kv8_attention_decode: query_len tokens for every sequence (1 to 16; query token s * query_len + i), the work split over the GPU
+ * along the rows; accuracy follows the type (float32: queries and probabilities enter the tensor cores as two halves each).
+ * er_kv8_attention_prefill: a ragged batch; max_query_len bounds the longest sequence's tokens (0 = num_tokens does).
+ * workspace: device memory of er_kv8_*_workspace_bytes, 16-byte aligned, no particular contents; two calls that may overlap on the
+ * GPU need two. */
+typedef struct {
+    const void* q;               /* device [num_tokens][num_heads][head_dim] */
+    void* out;
+    int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;   /* elements, 16-byte multiples */
+    const int32_t* query_starts; /* prefill: device [num_seqs + 1] */
+    uint32_t num_tokens, num_heads;
+    uint32_t query_len;          /* decode */
+    uint32_t max_query_len;      /* prefill */
+    uint32_t type;               /* ER_TYPE_* of q and out */
+    float softmax_scale;
+    uint32_t sliding_window;
+    void* workspace;
+    uint64_t workspace_bytes;
+} er_kv8_attention_params;
+int64_t er_kv8_decode_workspace_bytes(const er_kv8_cache* cache, const er_kv8_attention_params* params);
+int32_t er_kv8_attention_decode(const er_kv8_cache* cache, const er_kv8_attention_params* params, void* stream);
+int64_t er_kv8_prefill_workspace_bytes(const er_kv8_cache* cache, const er_kv8_attention_params* params);
+int32_t er_kv8_attention_prefill(const er_kv8_cache* cache, const er_kv8_attention_params* params, void* stream);
+
 /* Number of kernels this library has launched since load (all caches, this process). */
 uint64_t er_kernel_launch_count(void);
 /* Device status word of the cache (synchronises with the device): ER_OK, ER_ERR_DEVICE_TIMEOUT if a bounded wait inside a
