@@ -154,6 +154,11 @@ void count_kernel_launch();                                 // er_kv.cu: bumps e
 int32_t kv8_check(const er_kv8_cache* cache, Kv8Cache* out);                // kv8_append.cu: the fields; fills the kernels' form
 int32_t kv8_check_device(const er_kv8_cache* cache);                         // the buffers are the current device's
 int32_t kv8_launched(cudaError_t e, const char* kernel);                     // status of the launch just made
+int kv8_sm_count();                                                          // kv8_decode.cu: SMs of the current device, 0 without one
+int32_t kv8_check_attention(const er_kv8_cache* c, const er_kv8_attention_params* u);
+int32_t kv8_check_workspace(const er_kv8_attention_params* u, int64_t need);
+int64_t kv8_decode_workspace(const er_kv8_cache* c, const er_kv8_attention_params* u, bool ragged);
+int32_t kv8_launch_decode(const Kv8Cache& cache, const er_kv8_cache* c, const er_kv8_attention_params* u, bool ragged, int few_rows, cudaStream_t s);
 inline float kv8_scale_log2(float softmax_scale, uint32_t head_dim) {       // scores in units of log2
     return (softmax_scale > 0.f ? softmax_scale : 1.f / std::sqrt(static_cast<float>(head_dim))) * 1.4426950408889634f;
 }

@@ -35,6 +35,7 @@ struct Kv8Decode {
     float* partial;
     const int32_t* starts;          // tokens of the sequences, or nullptr: query_len each
     int num_tokens, group, query_len, window, tile_rows;
+    int few_rows;                   // > 0: sequences with more query rows are somebody else's
     float scale_log2;
 };
 
@@ -56,6 +57,7 @@ __device__ __forceinline__ SeqRange seq_range(const Kv8Decode& p, int seq) {
         if (r.begin < 0 || r.n < 0 || r.begin > p.num_tokens - r.n) r.n = 0;
     }
     r.row_tiles = (r.n * p.group + p.tile_rows - 1) / p.tile_rows;
+    if (p.few_rows > 0 && r.n * p.group > p.few_rows) r.row_tiles = 0;
     r.len = max(0, min(__ldg(p.cache.lens + seq), p.cache.table_width * p.cache.page_size));   // rows behind the table have no page
     const int lo = p.window > 0 ? max(0, r.len - r.n - p.window + 1) : 0;
     r.first_unit = lo / kKv8Unit;
@@ -604,11 +606,13 @@ __global__ void __launch_bounds__(kThreads) kv8_decode_join_kernel(const __grid_
     }
 }
 
-int sm_count() {
+}  // namespace
+int kv8_sm_count() {
     int device = 0, sms = 0;
     if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) sms = 0;
     return sms;
 }
+namespace {
 // Two columns of eight query rows where they are needed and fit: float32 rows take two operands each and stay at eight.
 int tiles_of(uint32_t type, int rows) { return type != ER_TYPE_FLOAT32 && rows > 8 ? 2 : 1; }
 
@@ -673,7 +677,7 @@ static int most_rows_of(const er_kv8_cache* c, const er_kv8_attention_params* u,
 }
 
 int64_t kv8_decode_workspace(const er_kv8_cache* c, const er_kv8_attention_params* u, bool ragged) {
-    const int sms = sm_count();
+    const int sms = kv8_sm_count();
     if (sms == 0) return report_error(ER_ERR_CUDA, "no CUDA device (no CPU fallback)");
     return static_cast<int64_t>(sms) * 2 * 8 * tiles_of(u->type, most_rows_of(c, u, ragged)) * (c->head_dim + 4) * 4;
 }
@@ -686,8 +690,10 @@ int32_t kv8_check_workspace(const er_kv8_attention_params* u, int64_t need) {
     return ER_OK;
 }
 
-// The kernel over a checked call; ragged: queries by query_starts.
-int32_t kv8_launch_decode(const Kv8Cache& cache, uint32_t head_dim, bool e4m3, const er_kv8_attention_params* u, int most_rows, bool ragged, cudaStream_t s) {
+// The kernel over a checked call.  ragged: queries by query_starts, of the sequences with up to `few_rows` query rows (0: all).
+int32_t kv8_launch_decode(const Kv8Cache& cache, const er_kv8_cache* c, const er_kv8_attention_params* u, bool ragged, int few_rows, cudaStream_t s) {
+    const int most_rows = few_rows > 0 ? std::min(few_rows, most_rows_of(c, u, ragged)) : most_rows_of(c, u, ragged);
+    const bool e4m3 = c->format == ER_KV8_E4M3;
     Kv8Decode p{};
     p.cache = cache;
     p.q = u->q; p.out = u->out;
@@ -695,10 +701,11 @@ int32_t kv8_launch_decode(const Kv8Cache& cache, uint32_t head_dim, bool e4m3, c
     p.partial = static_cast<float*>(u->workspace);
     p.starts = ragged ? u->query_starts : nullptr;
     p.num_tokens = static_cast<int>(u->num_tokens);
+    p.few_rows = few_rows;
     p.group = static_cast<int>(u->num_heads) / cache.num_kv_heads;
     p.query_len = static_cast<int>(u->query_len); p.window = static_cast<int>(u->sliding_window);
-    p.scale_log2 = kv8_scale_log2(u->softmax_scale, head_dim);
-    const int sms = sm_count(), d = static_cast<int>(head_dim);
+    p.scale_log2 = kv8_scale_log2(u->softmax_scale, c->head_dim);
+    const int sms = kv8_sm_count(), d = static_cast<int>(c->head_dim);
     switch (u->type) {
         case ER_TYPE_FLOAT32: return launch_shape<float>(p, most_rows, d, e4m3, sms, s);
         case ER_TYPE_FLOAT16: return launch_shape<__half>(p, most_rows, d, e4m3, sms, s);
@@ -726,25 +733,5 @@ extern "C" int32_t er_kv8_attention_decode(const er_kv8_cache* cache, const er_k
     rc = kv8_check_device(cache);
     if (rc == ER_OK) rc = kv8_check_workspace(u, kv8_decode_workspace(cache, u, false));
     if (rc != ER_OK || cache->num_seqs == 0) return rc;
-    return kv8_launch_decode(c, cache->head_dim, cache->format == ER_KV8_E4M3, u, most_rows_of(cache, u, false), false, static_cast<cudaStream_t>(stream));
-}
-
-extern "C" int64_t er_kv8_prefill_workspace_bytes(const er_kv8_cache* cache, const er_kv8_attention_params* u) {
-    using namespace er;
-    if (!cache || !u || cache->num_kv_heads == 0) return report_error(ER_ERR_INVALID_ARGUMENT, "null argument");
-    return kv8_decode_workspace(cache, u, true);
-}
-
-extern "C" int32_t er_kv8_attention_prefill(const er_kv8_cache* cache, const er_kv8_attention_params* u, void* stream) {
-    using namespace er;
-    if (!cache || !u) return report_error(ER_ERR_INVALID_ARGUMENT, "null argument");
-    Kv8Cache c{};
-    int32_t rc = kv8_check(cache, &c);
-    if (rc == ER_OK) rc = kv8_check_attention(cache, u);
-    if (rc != ER_OK) return rc;
-    if (!u->query_starts) return report_error(ER_ERR_INVALID_ARGUMENT, "query_starts is needed for a ragged batch");
-    rc = kv8_check_device(cache);
-    if (rc == ER_OK) rc = kv8_check_workspace(u, kv8_decode_workspace(cache, u, true));
-    if (rc != ER_OK || cache->num_seqs == 0 || u->num_tokens == 0) return rc;
-    return kv8_launch_decode(c, cache->head_dim, cache->format == ER_KV8_E4M3, u, most_rows_of(cache, u, true), true, static_cast<cudaStream_t>(stream));
+    return kv8_launch_decode(c, cache, u, false, 0, static_cast<cudaStream_t>(stream));
 }

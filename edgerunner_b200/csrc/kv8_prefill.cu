@@ -1,0 +1,660 @@
+// er_kv8_attention_prefill on the 5th-generation tensor cores: a ragged batch of prompts or prompt chunks, causal by position, over an 8-bit
+// block-scaled paged cache.
+//
+// Mathematics.  s = (q . ck) a scale with a the key scale of 16 or more rows, w = 2^(s log2 e - m) b / R with b the value scale and R a power of two near
+// the largest one so far, o = R sum_i w_i cv_i / sum_i (w_i R / b_i).  Codes are exact in fp16, q and w are rounded to it, sums are float32.  Neither scale
+// costs an operation a score: a multiplies the factor inside exp2's argument, log2(b / R) is part of its offset, and the sum of 16 weights is
+// divided by b / R once.
+//
+// One CTA owns two tiles of 128 query rows of a (sequence, kv head): row r is query r / group, head r % group, any group.  Bound by the tensor
+// pipe and, as closely, by exp2 (16 a clock and SM against 128 x 128 x D products in 512 clocks), so the two tiles take turns: while one is in its softmax
+// the products of the other run.
+//   warps 0-3, 4-7   softmax of tile 0, 1: a thread is a row.  Reads S from tensor memory twice (maximum, then weights), writes w as fp16 over S.  The
+//                    running maximum may lag by 2^8 before the row of O is rescaled in tensor memory, so that this is rare.
+//   warps 8-11       fetch 128 tokens of codes at a time (loads of the next half tile in registers while this one is converted), write them as
+//                    fp16 into the operand layout: a conversion in the loader reads 1 byte an element from L2 and serves 256 rows.
+//   warp 12          one lane issues the products: S_i = Q_i K^T (M128 N128 K16 steps, operands in shared memory), O_i += W_i V (A from tensor memory).
+//                    Products of one thread execute in the order of issue, so that S_i of the next tokens may overwrite W_i.
+// Tensor memory: S_0, S_1 at columns 0, 128; O_0, O_1 at 256, 384.  Shared memory: Q (2 x 128 rows), a ring of K / V tiles of 128 tokens, scales.
+// Every wait is bounded (2 s): then the status word is set, the rest of the waits are skipped, tensor memory is freed, the kernel returns.
+#include <algorithm>
+
+#include "kv8.cuh"
+#include "prefill_umma.cuh"
+
+namespace er {
+namespace {
+
+constexpr int kTok = 128;                  // tokens of a K / V tile
+constexpr int kSoftWarps = 8, kLoadWarps = 4;
+constexpr int kThreads = (kSoftWarps + kLoadWarps + 1) * 32;
+constexpr int kScaleRing = 4;
+constexpr float kLag = 8.f;                // how far (log2) a row's maximum may rise above the one in use
+constexpr float kCarry = 5.f;              // weights are carried 2^5 times: w <= 2^(8 + 2 + 5) < 65504
+template <int D> __host__ __device__ constexpr int stage_count() { return D == 128 ? 5 : 8; }
+template <int D> __host__ __device__ constexpr int tile_bytes() { return kTok * D * 2; }   // also a tile of 128 query rows
+template <int D> __host__ __device__ constexpr int prefill_smem() { return (stage_count<D>() + 2) * tile_bytes<D>() + 256 + kScaleRing * 32 * 4 + 1024; }
+
+struct Kv8Prefill {
+    Kv8Cache cache;
+    const void* q;
+    void* out;
+    int64_t q_token, q_head, out_token, out_head;
+    const int32_t* starts;
+    float* partial;             // of the split tiles: [index][256 rows][D + 4]: max, sum, -, -, unnormalised row
+    int num_tokens, group, window, min_rows;    // sequences with fewer query rows are somebody else's
+    int slots, split_from, parts;               // CTAs [0, split_from) own a tile pair, the others a part of its keys
+    float scale_log2;
+};
+
+// The sequence and the 256 query rows of slot `slot`: sequence s owns the slots from starts[s] * group / 256 + s on.
+struct Tile {
+    int seq, begin, n, len, row0, rows;        // rows: of the sequence; row0: first of the slot; rows == 0: nothing to do
+    int wrong;                                 // what the host could not see: an ER_ERR_* code, or 0
+};
+__device__ __forceinline__ Tile find_tile(const Kv8Prefill& p, int slot) {
+    int lo = 0, hi = p.cache.num_seqs;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (static_cast<int>(static_cast<int64_t>(__ldg(p.starts + mid)) * p.group / 256) + mid <= slot) lo = mid; else hi = mid;
+    }
+    Tile t;
+    t.seq = lo;
+    t.begin = __ldg(p.starts + lo);
+    t.n = __ldg(p.starts + lo + 1) - t.begin;
+    t.rows = 0;
+    t.row0 = (slot - (static_cast<int>(static_cast<int64_t>(t.begin) * p.group / 256) + lo)) * 256;
+    t.len = 0;
+    t.wrong = t.begin < 0 || t.n < 0 || t.begin > p.num_tokens - t.n ? ER_ERR_SHAPE : 0;
+    if (t.wrong != 0) return t;
+    const int rows = t.n * p.group;
+    if (rows < p.min_rows || t.row0 < 0 || t.row0 >= rows) return t;
+    t.rows = rows;
+    t.len = __ldg(p.cache.lens + lo);
+    const int most = p.cache.table_width * p.cache.page_size;     // rows behind the table have no page
+    t.wrong = t.len > most ? ER_ERR_OUT_OF_PAGES : t.len < 0 ? ER_ERR_SHAPE : 0;
+    t.len = max(0, min(t.len, most));
+    return t;
+}
+
+struct Waiter {
+    volatile int* abort_flag;
+    const Kv8Cache* cache;
+    __device__ __forceinline__ void operator()(uint64_t* bar, uint32_t parity) const {
+        if (*abort_flag || mbar_try_wait(bar, parity)) return;
+        const uint64_t start = global_timer_ns();
+        uint32_t spins = 0;
+        while (!mbar_try_wait(bar, parity)) {
+            if ((++spins & 0x3FFu) == 0u) {
+                if (*abort_flag) return;
+                if (global_timer_ns() - start > 2000000000ull) {
+                    *abort_flag = 1;
+                    kv8_report(*cache, ER_ERR_DEVICE_TIMEOUT);
+                    return;
+                }
+            }
+        }
+    }
+};
+
+// Waits for the loads of tensor memory in flight; names the registers, so that nothing that uses them moves in front.
+__device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                   "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
+                   "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]),
+                   "+r"(r[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t half2_word(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <typename T, int D, bool E4M3>
+__global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_constant__ Kv8Prefill p) {
+    constexpr int kStages = stage_count<D>(), kTile = tile_bytes<D>(), kRegion = kTok * 128;   // a region: 128 rows x 64 halves
+    constexpr int kBarFull = 0, kBarEmpty = kStages, kBarS = 2 * kStages, kBarP = kBarS + 2, kBarQ = kBarP + 2, kBarO = kBarQ + 1, kBarScale = kBarO + 1,
+                  kNumBars = kBarScale + kScaleRing;
+    static_assert(kNumBars * 8 + 8 <= 256, "");
+    extern __shared__ uint8_t raw[];
+    const Kv8Cache& c = p.cache;
+    const uint32_t sbase = (smem_u32(raw) + 1023u) & ~1023u;
+    uint8_t* gen = raw + (sbase - smem_u32(raw));
+    uint8_t* q_gen = gen + kStages * kTile;                       // two tiles of queries behind the ring
+    uint64_t* bars = reinterpret_cast<uint64_t*>(q_gen + 2 * kTile);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kNumBars);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    float* scale_ring = reinterpret_cast<float*>(q_gen + 2 * kTile + 256);   // [ring][key scale x 8, log2 of the value scale x 8, 1 / it x 8, -]
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    // ---- which rows, which keys ----
+    int unit = blockIdx.x, part = 0, parts = 1;
+    if (unit >= p.split_from) {
+        part = (unit - p.split_from) % p.parts;
+        parts = p.parts;
+        unit = p.split_from + (unit - p.split_from) / p.parts;
+    }
+    const int head = unit % c.num_kv_heads;                       // the last rows, which see most, first
+    const Tile tile = find_tile(p, p.slots - 1 - unit / c.num_kv_heads);
+    if (tile.wrong != 0 && threadIdx.x == 0) kv8_report(c, tile.wrong);
+    if (tile.rows == 0) return;
+    const int past = tile.len - tile.n, last_row = min(tile.rows, tile.row0 + 256) - 1;
+    const int hi = min(tile.len, past + last_row / p.group + 1);  // keys below it
+    const int lo = p.window > 0 ? max(0, past + tile.row0 / p.group - p.window + 1) : 0;
+    int t_begin = lo / kTok, tiles = max(0, (hi + kTok - 1) / kTok - t_begin);
+    if (parts > 1) {
+        const int per = (tiles + parts - 1) / parts, b = min(tiles, part * per);
+        tiles = min(tiles, b + per) - b;
+        t_begin += b;
+    }
+    const bool two = tile.row0 + 128 < tile.rows;
+
+    if (tid == 0) {
+        for (int i = 0; i < kNumBars; ++i) {
+            uint32_t n = 1;
+            if (i < kBarEmpty) n = kLoadWarps * 32;
+            else if (i == kBarP || i == kBarP + 1) n = 128;
+            else if (i == kBarQ) n = two ? 256 : 128;
+            else if (i >= kBarScale) n = kLoadWarps;
+            mbar_init(bars + i, n);
+        }
+        *abort_flag = 0;
+        mbar_init_fence();
+    }
+    if (warp == kSoftWarps + kLoadWarps) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const Waiter wait{abort_flag, &c};
+
+    if (warp == kSoftWarps + kLoadWarps) {
+        // ================= products =================
+        if (lane == 0 && tiles > 0) {
+            constexpr uint32_t kHi = umma_desc_hi(1024);
+            constexpr uint32_t idesc_qk = umma_idesc(128, kTok, false), idesc_pv = umma_idesc(128, D, true);
+            const uint32_t ring_lo = umma_desc_lo(sbase, 16), v_lo = umma_desc_lo(sbase, kRegion), q_lo = umma_desc_lo(sbase + kStages * kTile, 16);
+            auto scores = [&](int i, int idx) {                  // S_i = Q_i K^T, K in ring entry idx
+                const uint32_t st = static_cast<uint32_t>(idx % kStages) * (kTile >> 4);
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    const uint32_t off = ((kk >> 2) * kRegion + (kk & 3) * 32) >> 4;
+                    umma_f16(tmem + 128u * i, umma_desc_pack(q_lo + i * (kTile >> 4) + off, kHi), umma_desc_pack(ring_lo + st + off, kHi), idesc_qk, kk > 0);
+                }
+                umma_commit(smem_u32(bars + kBarS + i));
+            };
+            auto outputs = [&](int i, int idx, bool first) {     // O_i += W_i V
+                const uint32_t st = static_cast<uint32_t>(idx % kStages) * (kTile >> 4);
+#pragma unroll
+                for (int kt = 0; kt < kTok / 16; ++kt)
+                    umma_f16_ts(tmem + 256u + 128u * i, tmem + 128u * i + 8u * kt, umma_desc_pack(v_lo + st + ((kt * 2048) >> 4), kHi), idesc_pv, !first || kt > 0);
+            };
+            auto full = [&](int idx) {
+                wait(bars + kBarFull + idx % kStages, (idx / kStages) & 1);
+                tc_fence_after();
+            };
+            auto release = [&](int idx) { umma_commit(smem_u32(bars + kBarEmpty + idx % kStages)); };
+            wait(bars + kBarQ, 0);
+            full(0);
+            scores(0, 0);
+            if (two) scores(1, 0);
+            release(0);
+            for (int j = 0; j < tiles; ++j) {
+                const int vi = 2 * j + 1, ki = 2 * j + 2;
+                const bool more = j + 1 < tiles;
+                full(vi);
+                wait(bars + kBarP, j & 1);
+                tc_fence_after();
+                outputs(0, vi, j == 0);
+                if (more) {
+                    full(ki);
+                    scores(0, ki);
+                }
+                if (two) {
+                    wait(bars + kBarP + 1, j & 1);
+                    tc_fence_after();
+                    outputs(1, vi, j == 0);
+                }
+                release(vi);
+                if (more) {
+                    if (two) scores(1, ki);
+                    release(ki);
+                }
+            }
+            umma_commit(smem_u32(bars + kBarO));
+        }
+    } else if (warp >= kSoftWarps) {
+        // ================= loader: codes -> fp16 operand tiles =================
+        // A lane holds 16 codes of a row, D / 16 lanes a row; a warp fetches 32 rows, two units of 16 tokens.
+        constexpr int kLanes = D / 16, kRows = 32 / kLanes, kLoads = 32 / kRows;
+        const int w = warp - kSoftWarps, ch = lane % kLanes, sub = lane / kLanes;
+        int page_now[2] = {-1, -1}, page_next[2];
+        int64_t at_now[2] = {0, 0};            // first row of the unit in the cache
+        auto place = [&](int j) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int tok = (t_begin + j) * kTok + w * 32 + u * 16;
+                at_now[u] = (static_cast<int64_t>(max(page_now[u], 0)) * c.num_kv_heads + head) * c.page_size + tok % c.page_size;
+            }
+        };
+        auto pages = [&](int j, int (&pg)[2]) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int tok = (t_begin + j) * kTok + w * 32 + u * 16;
+                pg[u] = j < tiles && tok < tile.len ? kv8_page(c, tile.seq, tok) : -1;
+            }
+        };
+        uint4 buf[kLoads];
+        auto fetch = [&](int j, int side) {
+            const int tok0 = (t_begin + j) * kTok + w * 32;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int r = i * kRows + sub, u = i * kRows / 16;
+                buf[i] = make_uint4(0, 0, 0, 0);
+                if (page_now[u] >= 0 && tok0 + r < tile.len)
+                    buf[i] = __ldg(reinterpret_cast<const uint4*>(c.codes[side] + (at_now[u] + (r - 16 * u)) * D + ch * 16));
+            }
+        };
+        float kscale = 0.f, vscale = 0.f;      // lanes 0, 1: of their unit
+        auto fetch_scales = [&](int j) {
+            if (lane < 2) {
+                const int tok = (t_begin + j) * kTok + w * 32 + lane * 16, page = lane == 0 ? page_now[0] : page_now[1];
+                kscale = -1.f;
+                vscale = 0.f;
+                if (page >= 0) {
+                    const int64_t at = (lane == 0 ? at_now[0] : at_now[1]) / c.scale_block;
+                    kscale = __ldg(c.scales[0] + at);
+                    vscale = __ldg(c.scales[1] + at);
+                } else if (j < tiles && tok < tile.len) {
+                    kv8_report(c, ER_ERR_OUT_OF_PAGES);
+                }
+            }
+        };
+        if (tiles > 0) {
+            pages(0, page_now);
+            place(0);
+            fetch(0, 0);
+            fetch_scales(0);
+            pages(1, page_next);
+            for (int idx = 0; idx < 2 * tiles; ++idx) {
+                const int j = idx >> 1, st = idx % kStages;
+                uint4 cur[kLoads];
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) cur[i] = buf[i];
+                if ((idx & 1) == 0) {                              // keys of tile j are here; publish its scales, fetch its values
+                    if (lane < 2) {
+                        float* s = scale_ring + (j % kScaleRing) * 32 + w * 2 + lane;
+                        s[0] = kscale;
+                        s[8] = __log2f(vscale);                    // NaN stays NaN; 0 gives -inf
+                        s[16] = 1.f / vscale;
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bars + kBarScale + j % kScaleRing);
+                    fetch(j, 1);
+                } else if (j + 1 < tiles) {
+                    page_now[0] = page_next[0];
+                    page_now[1] = page_next[1];
+                    place(j + 1);
+                    fetch(j + 1, 0);
+                    fetch_scales(j + 1);
+                    pages(j + 2, page_next);
+                }
+                if (idx >= kStages) wait(bars + kBarEmpty + st, ((idx / kStages) - 1) & 1);
+                uint8_t* dst = gen + st * kTile;
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) {
+                    const int r = w * 32 + i * kRows + sub;
+                    uint4 a, b;                                    // dims 16 ch .. + 8, + 8 .. + 16
+                    decode4<E4M3>(cur[i].x, a.x, a.y);
+                    decode4<E4M3>(cur[i].y, a.z, a.w);
+                    decode4<E4M3>(cur[i].z, b.x, b.y);
+                    decode4<E4M3>(cur[i].w, b.z, b.w);
+                    uint8_t* row = dst + (ch >> 2) * kRegion;
+                    const int c0 = 2 * (ch & 3), swap = (D == 128) ? ch >> 2 : 0;   // the lanes of the second region store their odd chunk first: no bank conflict
+                    *reinterpret_cast<uint4*>(row + um_swz(r, c0 + swap)) = swap ? b : a;
+                    *reinterpret_cast<uint4*>(row + um_swz(r, c0 + 1 - swap)) = swap ? a : b;
+                }
+                fence_async_smem();
+                mbar_arrive(bars + kBarFull + st);
+            }
+        }
+    } else if (warp < 4 || two) {
+        // ================= softmax =================
+        const int i = warp >> 2, m_row = tid & 127, row = tile.row0 + i * 128 + m_row;
+        const bool row_ok = row < tile.rows;
+        const int r_use = min(row, tile.rows - 1), qi = r_use / p.group, qh = head * p.group + r_use % p.group;
+        const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t tm_s = tmem + 128u * i + lane_base, tm_o = tmem + 256u + 128u * i + lane_base;
+        float factor;                          // log2(e) * scale * the power of two that the row was divided by
+        {
+            const T* src = static_cast<const T*>(p.q) + static_cast<int64_t>(tile.begin + qi) * p.q_token + qh * p.q_head;
+            uint32_t mx = 0;
+            uint4 v[D / 8];
+#pragma unroll
+            for (int k = 0; k < D / 8; ++k) {
+                v[k] = row_ok ? __ldg(reinterpret_cast<const uint4*>(src) + k) : make_uint4(0, 0, 0, 0);
+                float f[8];
+                Act<T>::unpack(v[k], f);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) mx = max(mx, __float_as_uint(f[e]) & 0x7FFFFFFFu);
+            }
+            const uint32_t ex = min(max(mx >> 23, 1u), 252u);
+            const float down = __uint_as_float((253u - ex) << 23);
+            factor = __uint_as_float((ex + 1u) << 23) * p.scale_log2;
+            uint8_t* dst = q_gen + i * kTile;
+#pragma unroll
+            for (int k = 0; k < D / 8; ++k) {
+                float f[8];
+                Act<T>::unpack(v[k], f);
+                uint4 o;
+                o.x = half2_word(f[0] * down, f[1] * down);
+                o.y = half2_word(f[2] * down, f[3] * down);
+                o.z = half2_word(f[4] * down, f[5] * down);
+                o.w = half2_word(f[6] * down, f[7] * down);
+                *reinterpret_cast<uint4*>(dst + (k >> 3) * kRegion + um_swz(m_row, k & 7)) = o;
+            }
+            fence_async_smem();
+            mbar_arrive(bars + kBarQ);
+        }
+        const int limit = min(tile.len - 1, past + qi);
+        const int lower = p.window > 0 ? past + qi - p.window + 1 : 0;
+        float m = -INFINITY, l = 0.f, LR = -200.f;
+        for (int j = 0; j < tiles; ++j) {
+            const int t0 = (t_begin + j) * kTok;
+            wait(bars + kBarScale + j % kScaleRing, (j / kScaleRing) & 1);
+            const float* sc = scale_ring + (j % kScaleRing) * 32;
+            float ks[8], e[8], inv[8];
+            bool hidden = false;
+            float vm = -INFINITY;
+#pragma unroll
+            for (int g = 0; g < 8; ++g) {
+                ks[g] = sc[g];
+                e[g] = sc[8 + g];
+                inv[g] = sc[16 + g];
+                hidden |= ks[g] < 0.f;
+                vm = fmaxf(vm, e[g]);
+            }
+            const bool edge = __any_sync(0xffffffffu, hidden || t0 + kTok - 1 > limit || t0 < lower);
+            auto masked = [&](int g, int col) {
+                const int tok = t0 + col;
+                return tok > limit || tok < lower || ks[g] < 0.f;
+            };
+            wait(bars + kBarS + i, j & 1);
+            tc_fence_after();
+            // ---- the maximum ----
+            float mx = -INFINITY;
+            {
+                uint32_t a[32], b[32];
+                auto take = [&](const uint32_t (&s)[32], int chunk) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int g = 2 * chunk + h;
+                        float x = -INFINITY, y = -INFINITY;
+                        if (edge) {
+#pragma unroll
+                            for (int k = 0; k < 16; ++k)
+                                if (!masked(g, 16 * g + k)) x = fmaxf(x, __uint_as_float(s[16 * h + k]));
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 16; k += 2) {
+                                x = fmaxf(x, __uint_as_float(s[16 * h + k]));
+                                y = fmaxf(y, __uint_as_float(s[16 * h + k + 1]));
+                            }
+                        }
+                        mx = fmaxf(mx, ks[g] < 0.f ? -INFINITY : fmaxf(x, y) * ks[g]);   // scales are not negative
+                    }
+                };
+                tmem_ld32_nowait(tm_s, a);
+                tmem_wait32(a);
+                tmem_ld32_nowait(tm_s + 32, b);
+                take(a, 0);
+                tmem_wait32(b);
+                tmem_ld32_nowait(tm_s + 64, a);
+                take(b, 1);
+                tmem_wait32(a);
+                tmem_ld32_nowait(tm_s + 96, b);
+                take(a, 2);
+                tmem_wait32(b);
+                take(b, 3);
+            }
+            mx *= factor;
+            // ---- move to it, if it is far enough above the one in use ----
+            const bool grow = vm > LR + 2.f;
+            if (__any_sync(0xffffffffu, grow || mx > m + kLag)) {
+                const float m_new = fmaxf(m, mx), LR_new = grow ? ceilf(vm) : LR;
+                const float corr = m_new == -INFINITY ? 1.f : fast_exp2(m - m_new);
+                l *= corr;
+                const float oc = corr * fast_exp2(LR - LR_new);
+                m = m_new;
+                LR = LR_new;
+                if (j > 0) {
+#pragma unroll
+                    for (int c0 = 0; c0 < D; c0 += 32) {
+                        uint32_t o[32];
+                        tmem_ld32_nowait(tm_o + c0, o);
+                        tmem_wait32(o);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * oc);
+                        tmem_st32_words(tm_o + c0, o);
+                    }
+                }
+            }
+            // ---- weights ----
+            const float base = m == -INFINITY ? 0.f : m;
+            const float R = fast_exp2(LR - kCarry);
+            {
+                uint32_t a[32], b[32];
+                auto weigh = [&](const uint32_t (&s)[32], int chunk) {
+                    uint32_t out[16];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int g = 2 * chunk + h;
+                        const float up = e[g] - LR + kCarry, f = ks[g] * factor;
+                        const float off = (up < -60.f ? -60.f : up) - base;       // a NaN stays; below 2^-60 a weight is nothing in fp16, but counts in the sum
+                        float x = 0.f, y = 0.f;
+#pragma unroll
+                        for (int k = 0; k < 16; k += 2) {
+                            float u = fast_exp2(fmaf(__uint_as_float(s[16 * h + k]), f, off));
+                            float v = fast_exp2(fmaf(__uint_as_float(s[16 * h + k + 1]), f, off));
+                            if (edge) {
+                                u = masked(g, 16 * g + k) ? 0.f : u;
+                                v = masked(g, 16 * g + k + 1) ? 0.f : v;
+                            }
+                            x += u;
+                            y += v;
+                            out[8 * h + (k >> 1)] = half2_word(u, v);
+                        }
+                        l = fmaf(x + y, fminf(inv[g] * R, 1.152921504606846976e18f), l);
+                    }
+                    tmem_st16_words(tm_s + 16u * chunk, out);
+                };
+                tmem_ld32_nowait(tm_s, a);
+                tmem_wait32(a);
+                tmem_ld32_nowait(tm_s + 32, b);
+                tmem_wait32(b);                                    // chunk 0's weights go over columns 0-15, chunk 1's over 16-31, ...
+                weigh(a, 0);
+                tmem_ld32_nowait(tm_s + 64, a);
+                weigh(b, 1);
+                tmem_wait32(a);
+                tmem_ld32_nowait(tm_s + 96, b);
+                weigh(a, 2);
+                tmem_wait32(b);
+                weigh(b, 3);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(bars + kBarP + i);
+        }
+        // ---- the rows ----
+        if (tiles > 0) {
+            wait(bars + kBarO, 0);
+            tc_fence_after();
+        }
+        const float up = fast_exp2(LR - kCarry), f = parts > 1 ? up : (l == 0.f ? 0.f : up / l);
+        float* part_row = parts > 1 ? p.partial + (static_cast<int64_t>(static_cast<int>(blockIdx.x) - p.split_from) * 256 + i * 128 + m_row) * (D + 4) : nullptr;
+        if (parts > 1) { part_row[0] = m; part_row[1] = l; }
+        T* dst = static_cast<T*>(p.out) + static_cast<int64_t>(tile.begin + qi) * p.out_token + qh * p.out_head;
+#pragma unroll
+        for (int c0 = 0; c0 < D; c0 += 32) {
+            uint32_t o[32];
+            if (tiles > 0) {
+                tmem_ld32_nowait(tm_o + c0, o);
+                tmem_wait32(o);
+            }
+            float x[32];
+#pragma unroll
+            for (int k = 0; k < 32; ++k) x[k] = tiles > 0 && (parts > 1 || l != 0.f) ? __uint_as_float(o[k]) * f : 0.f;
+            if (parts > 1) {
+#pragma unroll
+                for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(part_row + 4 + c0 + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
+            } else if (row_ok) {
+#pragma unroll
+                for (int k = 0; k < 32; k += 8) *reinterpret_cast<uint4*>(dst + c0 + k) = Act<T>::pack(x + k);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kSoftWarps + kLoadWarps) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+// Joins the parts of the split tile pairs: a warp per query row, a lane D / 32 dims.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv8_prefill_join_kernel(const __grid_constant__ Kv8Prefill p) {
+    constexpr int V = D / 32;
+    const int lane = threadIdx.x & 31;
+    const int unit = p.split_from + static_cast<int>(blockIdx.x) / 32, r = (static_cast<int>(blockIdx.x) % 32) * 8 + (threadIdx.x >> 5);
+    const Tile tile = find_tile(p, p.slots - 1 - unit / p.cache.num_kv_heads);
+    const int row = tile.row0 + r;
+    if (tile.rows == 0 || row >= tile.rows) return;
+    const float* base = p.partial + (static_cast<int64_t>(unit - p.split_from) * p.parts * 256 + r) * (D + 4);
+    float M = -INFINITY, L = 0.f, acc[V];
+    for (int k = 0; k < p.parts; ++k) M = fmaxf(M, base[static_cast<int64_t>(k) * 256 * (D + 4)]);
+    const float M0 = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = 0.f;
+    for (int k = 0; k < p.parts; ++k) {
+        const float* src = base + static_cast<int64_t>(k) * 256 * (D + 4);
+        const float f = fast_exp2(src[0] - M0);
+        L = fmaf(src[1], f, L);
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = fmaf(src[4 + lane * V + i], f, acc[i]);
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    T* dst = static_cast<T*>(p.out) + static_cast<int64_t>(tile.begin + row / p.group) * p.out_token + (unit % p.cache.num_kv_heads * p.group + row % p.group) * p.out_head + lane * V;
+#pragma unroll
+    for (int i = 0; i < V; i += 2) store_pair(dst + i, acc[i] * inv, acc[i + 1] * inv);
+}
+
+struct Plan {
+    int slots, split_from, parts, grid;
+};
+// One CTA fits an SM, so a grid of equal CTAs takes ceil(CTAs / SMs) rounds.  The tile pairs of the last, partly filled round are cut along the
+// keys into the number of parts (up to 8, and no more CTAs than four rounds) that fills whole rounds best; a second launch joins them.
+Plan make_plan(uint32_t num_tokens, int group, int num_seqs, int kv_heads, int sms) {
+    Plan pl;
+    pl.slots = static_cast<int>(static_cast<int64_t>(num_tokens) * group / 256) + num_seqs;
+    const int units = pl.slots * kv_heads, rest = units % sms;
+    pl.split_from = units;
+    pl.parts = 1;
+    double best = 1.0;
+    for (int k = 2; k <= 8 && rest > 0 && rest * k <= 4 * sms; ++k) {
+        const double rounds = static_cast<double>((rest * k + sms - 1) / sms) / k;
+        if (rounds < best - 0.02) {
+            best = rounds;
+            pl.parts = k;
+            pl.split_from = units - rest;
+        }
+    }
+    pl.grid = pl.split_from + (units - pl.split_from) * pl.parts;
+    return pl;
+}
+
+template <typename T, int D, bool E4M3>
+int32_t launch(const Kv8Prefill& p, const Plan& pl, cudaStream_t s) {
+    constexpr int kSmem = prefill_smem<D>();
+    static_assert(kSmem <= 232448, "prefill kernel exceeds the shared memory of an sm_100 CTA");
+    const cudaError_t e = cudaFuncSetAttribute(kv8_prefill_kernel<T, D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e != cudaSuccess) return kv8_launched(e, "kv8_prefill_kernel");
+    kv8_prefill_kernel<T, D, E4M3><<<pl.grid, kThreads, kSmem, s>>>(p);
+    const int32_t rc = kv8_launched(cudaGetLastError(), "kv8_prefill_kernel");
+    if (rc != ER_OK || pl.parts == 1) return rc;
+    kv8_prefill_join_kernel<T, D><<<(pl.grid - pl.split_from) / pl.parts * 32, 256, 0, s>>>(p);
+    return kv8_launched(cudaGetLastError(), "kv8_prefill_join_kernel");
+}
+template <typename T>
+int32_t launch_shape(const Kv8Prefill& p, const Plan& pl, uint32_t head_dim, bool e4m3, cudaStream_t s) {
+    if (head_dim == 128) return e4m3 ? launch<T, 128, true>(p, pl, s) : launch<T, 128, false>(p, pl, s);
+    return e4m3 ? launch<T, 64, true>(p, pl, s) : launch<T, 64, false>(p, pl, s);
+}
+
+// Sequences with up to this many query rows run on the decode kernel, which splits their keys over the GPU: it computes 16 rows
+// at a time, the tile pair 256.
+constexpr int kFewRows = 32;
+
+struct Split {
+    bool few, many;     // which of the two kernels have sequences to work on, as far as the host knows
+};
+Split split_of(const er_kv8_cache* c, const er_kv8_attention_params* u) {
+    const uint64_t group = u->num_heads / c->num_kv_heads;
+    const uint64_t most = u->max_query_len > 0 ? std::min(u->max_query_len, u->num_tokens) : u->num_tokens;
+    const int64_t least = static_cast<int64_t>(u->num_tokens) - static_cast<int64_t>(most) * (static_cast<int64_t>(c->num_seqs) - 1);   // tokens of the shortest
+    if (u->type == ER_TYPE_FLOAT32) return {true, false};
+    return {least < 0 || static_cast<uint64_t>(least) * group <= kFewRows, most * group > kFewRows};
+}
+
+}  // namespace
+}  // namespace er
+
+extern "C" int64_t er_kv8_prefill_workspace_bytes(const er_kv8_cache* cache, const er_kv8_attention_params* u) {
+    using namespace er;
+    if (!cache || !u || cache->num_kv_heads == 0 || u->num_heads < cache->num_kv_heads) return report_error(ER_ERR_INVALID_ARGUMENT, "null argument, or no heads");
+    const int sms = kv8_sm_count();
+    if (sms == 0) return report_error(ER_ERR_CUDA, "no CUDA device (no CPU fallback)");
+    const Split sp = split_of(cache, u);
+    int64_t bytes = sp.few ? kv8_decode_workspace(cache, u, true) : 0;      // the two kernels run one after the other
+    if (sp.many) {
+        const Plan pl = make_plan(u->num_tokens, static_cast<int>(u->num_heads / cache->num_kv_heads), static_cast<int>(cache->num_seqs), static_cast<int>(cache->num_kv_heads), sms);
+        if (pl.parts > 1) bytes = std::max(bytes, static_cast<int64_t>(pl.grid - pl.split_from) * 256 * (cache->head_dim + 4) * 4);
+    }
+    return bytes;
+}
+
+extern "C" int32_t er_kv8_attention_prefill(const er_kv8_cache* cache, const er_kv8_attention_params* u, void* stream) {
+    using namespace er;
+    if (!cache || !u) return report_error(ER_ERR_INVALID_ARGUMENT, "null argument");
+    Kv8Cache c{};
+    int32_t rc = kv8_check(cache, &c);
+    if (rc == ER_OK) rc = kv8_check_attention(cache, u);
+    if (rc != ER_OK) return rc;
+    if (!u->query_starts) return report_error(ER_ERR_INVALID_ARGUMENT, "query_starts is needed for a ragged batch");
+    rc = kv8_check_device(cache);
+    if (rc == ER_OK) rc = kv8_check_workspace(u, er_kv8_prefill_workspace_bytes(cache, u));
+    if (rc != ER_OK || cache->num_seqs == 0 || u->num_tokens == 0) return rc;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool e4m3 = cache->format == ER_KV8_E4M3;
+    const Split sp = split_of(cache, u);
+    if (sp.many) {
+        Kv8Prefill p{};
+        p.cache = c;
+        p.q = u->q; p.out = u->out;
+        p.q_token = u->q_token_stride; p.q_head = u->q_head_stride; p.out_token = u->out_token_stride; p.out_head = u->out_head_stride;
+        p.starts = u->query_starts;
+        p.partial = static_cast<float*>(u->workspace);
+        p.num_tokens = static_cast<int>(u->num_tokens);
+        p.group = static_cast<int>(u->num_heads) / c.num_kv_heads;
+        p.window = static_cast<int>(u->sliding_window);
+        p.min_rows = kFewRows + 1;
+        p.scale_log2 = kv8_scale_log2(u->softmax_scale, cache->head_dim);
+        const Plan pl = make_plan(u->num_tokens, p.group, c.num_seqs, c.num_kv_heads, kv8_sm_count());
+        p.slots = pl.slots; p.split_from = pl.split_from; p.parts = pl.parts;
+        rc = u->type == ER_TYPE_FLOAT16 ? launch_shape<__half>(p, pl, cache->head_dim, e4m3, s) : launch_shape<__nv_bfloat16>(p, pl, cache->head_dim, e4m3, s);
+        if (rc != ER_OK) return rc;
+    }
+    return sp.few ? kv8_launch_decode(c, cache, u, true, u->type == ER_TYPE_FLOAT32 ? 0 : kFewRows, s) : ER_OK;
+}
