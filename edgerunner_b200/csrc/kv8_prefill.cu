@@ -27,7 +27,7 @@ namespace {
 
 constexpr int kTok = 128;                  // tokens of a K / V tile
 constexpr int kSoftWarps = 8, kLoadWarps = 4;
-constexpr int kThreads = (kSoftWarps + kLoadWarps + 1) * 32;
+constexpr int kThreads = 512;             // three of the last four warps idle: registers move between groups of four warps
 constexpr int kScaleRing = 4;
 constexpr float kLag = 8.f;                // how far (log2) a row's maximum may rise above the one in use
 constexpr float kCarry = 5.f;              // weights are carried 2^5 times: w <= 2^(8 + 2 + 5) < 65504
@@ -172,27 +172,30 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const Waiter wait{abort_flag, &c};
-
-    if (warp == kSoftWarps + kLoadWarps) {
+    // Registers of the groups of four warps: 512 threads x 128 at launch = 128 x (168 + 168 + 104 + 72).  Each branch moves its own.
+    if (warp >= kSoftWarps + kLoadWarps) {
         // ================= products =================
-        if (lane == 0 && tiles > 0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == kSoftWarps + kLoadWarps && lane == 0 && tiles > 0) {
             constexpr uint32_t kHi = umma_desc_hi(1024);
             constexpr uint32_t idesc_qk = umma_idesc(128, kTok, false), idesc_pv = umma_idesc(128, D, true);
             const uint32_t ring_lo = umma_desc_lo(sbase, 16), v_lo = umma_desc_lo(sbase, kRegion), q_lo = umma_desc_lo(sbase + kStages * kTile, 16);
             auto scores = [&](int i, int idx) {                  // S_i = Q_i K^T, K in ring entry idx
-                const uint32_t st = static_cast<uint32_t>(idx % kStages) * (kTile >> 4);
+                uint32_t kd = ring_lo + static_cast<uint32_t>(idx % kStages) * (kTile >> 4), qd = q_lo + i * (kTile >> 4);
+                asm volatile("" : "+r"(kd), "+r"(qd));           // one add an operand here, not a register a descriptor kept over the loop
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk) {
                     const uint32_t off = ((kk >> 2) * kRegion + (kk & 3) * 32) >> 4;
-                    umma_f16(tmem + 128u * i, umma_desc_pack(q_lo + i * (kTile >> 4) + off, kHi), umma_desc_pack(ring_lo + st + off, kHi), idesc_qk, kk > 0);
+                    umma_f16(tmem + 128u * i, umma_desc_pack(qd + off, kHi), umma_desc_pack(kd + off, kHi), idesc_qk, kk > 0);
                 }
                 umma_commit(smem_u32(bars + kBarS + i));
             };
             auto outputs = [&](int i, int idx, bool first) {     // O_i += W_i V
-                const uint32_t st = static_cast<uint32_t>(idx % kStages) * (kTile >> 4);
+                uint32_t vd = v_lo + static_cast<uint32_t>(idx % kStages) * (kTile >> 4), a = tmem + 128u * i;
+                asm volatile("" : "+r"(vd), "+r"(a));
 #pragma unroll
                 for (int kt = 0; kt < kTok / 16; ++kt)
-                    umma_f16_ts(tmem + 256u + 128u * i, tmem + 128u * i + 8u * kt, umma_desc_pack(v_lo + st + ((kt * 2048) >> 4), kHi), idesc_pv, !first || kt > 0);
+                    umma_f16_ts(tmem + 256u + 128u * i, a + 8u * kt, umma_desc_pack(vd + ((kt * 2048) >> 4), kHi), idesc_pv, !first || kt > 0);
             };
             auto full = [&](int idx) {
                 wait(bars + kBarFull + idx % kStages, (idx / kStages) & 1);
@@ -230,6 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         }
     } else if (warp >= kSoftWarps) {
         // ================= loader: codes -> fp16 operand tiles =================
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         // A lane holds 16 codes of a row, D / 16 lanes a row; a warp fetches 32 rows, two units of 16 tokens.
         constexpr int kLanes = D / 16, kRows = 32 / kLanes, kLoads = 32 / kRows;
         const int w = warp - kSoftWarps, ch = lane % kLanes, sub = lane / kLanes;
@@ -323,8 +327,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                 mbar_arrive(bars + kBarFull + st);
             }
         }
-    } else if (warp < 4 || two) {
+    } else {
         // ================= softmax =================
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+        if (warp < 4 || two) {
         const int i = warp >> 2, m_row = tid & 127, row = tile.row0 + i * 128 + m_row;
         const bool row_ok = row < tile.rows;
         const int r_use = min(row, tile.rows - 1), qi = r_use / p.group, qh = head * p.group + r_use % p.group;
@@ -516,6 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
 #pragma unroll
                 for (int k = 0; k < 32; k += 8) *reinterpret_cast<uint4*>(dst + c0 + k) = Act<T>::pack(x + k);
             }
+        }
         }
     }
     tc_fence_before();
