@@ -374,21 +374,24 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             const int t0 = (t_begin + j) * kTok;
             wait(bars + kBarScale + j % kScaleRing, (j / kScaleRing) & 1);
             const float* sc = scale_ring + (j % kScaleRing) * 32;
-            float ks[8], e[8], inv[8];
-            bool hidden = false;
-            float vm = -INFINITY;
+            float vm = -INFINITY, kmin = INFINITY;
 #pragma unroll
             for (int g = 0; g < 8; ++g) {
-                ks[g] = sc[g];
-                e[g] = sc[8 + g];
-                inv[g] = sc[16 + g];
-                hidden |= ks[g] < 0.f;
-                vm = fmaxf(vm, e[g]);
+                kmin = fminf(kmin, sc[g]);
+                vm = fmaxf(vm, sc[8 + g]);
             }
-            const bool edge = __any_sync(0xffffffffu, hidden || t0 + kTok - 1 > limit || t0 < lower);
-            auto masked = [&](int g, int col) {
-                const int tok = t0 + col;
-                return tok > limit || tok < lower || ks[g] < 0.f;
+            const bool edge = __any_sync(0xffffffffu, kmin < 0.f || t0 + kTok - 1 > limit || t0 < lower);
+            // The columns of chunk c0 .. c0 + 32 that this row sees, one bit each.
+            auto seen = [&](int c0) {
+                const int from = min(max(lower - t0 - c0, 0), 32), to = min(max(limit + 1 - t0 - c0, 0), 32);
+                uint32_t bits = static_cast<uint32_t>((1ull << to) - 1ull) & ~static_cast<uint32_t>((1ull << from) - 1ull);
+                if (sc[c0 / 16] < 0.f) bits &= 0xFFFF0000u;
+                if (sc[c0 / 16 + 1] < 0.f) bits &= 0x0000FFFFu;
+                return bits;
+            };
+            auto hide = [&](uint32_t (&s)[32], uint32_t bits) {
+#pragma unroll
+                for (int k = 0; k < 32; ++k) s[k] = (bits >> k & 1u) != 0u ? s[k] : 0xFF800000u;
             };
             wait(bars + kBarS + i, j & 1);
             tc_fence_after();
@@ -396,37 +399,30 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             float mx = -INFINITY;
             {
                 uint32_t a[32], b[32];
-                auto take = [&](const uint32_t (&s)[32], int chunk) {
+                auto take = [&](uint32_t (&s)[32], int c0) {
+                    if (edge) hide(s, seen(c0));
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const int g = 2 * chunk + h;
-                        float x = -INFINITY, y = -INFINITY;
-                        if (edge) {
+                        float x = __uint_as_float(s[16 * h]), y = __uint_as_float(s[16 * h + 1]);
 #pragma unroll
-                            for (int k = 0; k < 16; ++k)
-                                if (!masked(g, 16 * g + k)) x = fmaxf(x, __uint_as_float(s[16 * h + k]));
-                        } else {
-#pragma unroll
-                            for (int k = 0; k < 16; k += 2) {
-                                x = fmaxf(x, __uint_as_float(s[16 * h + k]));
-                                y = fmaxf(y, __uint_as_float(s[16 * h + k + 1]));
-                            }
+                        for (int k = 2; k < 16; k += 2) {
+                            x = fmaxf(x, __uint_as_float(s[16 * h + k]));
+                            y = fmaxf(y, __uint_as_float(s[16 * h + k + 1]));
                         }
-                        mx = fmaxf(mx, ks[g] < 0.f ? -INFINITY : fmaxf(x, y) * ks[g]);   // scales are not negative
+                        const float top = fmaxf(x, y), ks = sc[c0 / 16 + h];
+                        mx = fmaxf(mx, ks < 0.f ? -INFINITY : top * ks);          // scales are not negative but for the mark of a hidden block
                     }
                 };
                 tmem_ld32_nowait(tm_s, a);
-                tmem_wait32(a);
-                tmem_ld32_nowait(tm_s + 32, b);
-                take(a, 0);
-                tmem_wait32(b);
-                tmem_ld32_nowait(tm_s + 64, a);
-                take(b, 1);
-                tmem_wait32(a);
-                tmem_ld32_nowait(tm_s + 96, b);
-                take(a, 2);
-                tmem_wait32(b);
-                take(b, 3);
+#pragma unroll 1
+                for (int c0 = 0; c0 < kTok; c0 += 64) {
+                    tmem_wait32(a);
+                    tmem_ld32_nowait(tm_s + c0 + 32, b);
+                    take(a, c0);
+                    tmem_wait32(b);
+                    if (c0 == 0) tmem_ld32_nowait(tm_s + 64, a);
+                    take(b, c0 + 32);
+                }
             }
             mx *= factor;
             // ---- move to it, if it is far enough above the one in use ----
@@ -439,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                 m = m_new;
                 LR = LR_new;
                 if (j > 0) {
-#pragma unroll
+#pragma unroll 1
                     for (int c0 = 0; c0 < D; c0 += 32) {
                         uint32_t o[32];
                         tmem_ld32_nowait(tm_o + c0, o);
@@ -455,42 +451,49 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             const float R = fast_exp2(LR - kCarry);
             {
                 uint32_t a[32], b[32];
-                auto weigh = [&](const uint32_t (&s)[32], int chunk) {
+                auto weigh = [&](uint32_t (&s)[32], int c0) {
+                    uint32_t bits = 0xFFFFFFFFu;
+                    if (edge) {
+                        bits = seen(c0);
+                        hide(s, bits);
+                    }
                     uint32_t out[16];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const int g = 2 * chunk + h;
-                        const float up = e[g] - LR + kCarry, f = ks[g] * factor;
-                        const float off = (up < -60.f ? -60.f : up) - base;       // a NaN stays; below 2^-60 a weight is nothing in fp16, but counts in the sum
+                        const int g = c0 / 16 + h;
+                        float up = sc[8 + g] - LR + kCarry, f = sc[g] * factor;
+                        up = (up < -60.f ? -60.f : up) - base;   // a NaN stays; below 2^-60 a weight is nothing in fp16, but counts in the sum
+                        if (f == 0.f) f = 1.17549435e-38f;       // a hidden -inf stays one
+                        if ((bits >> (16 * h) & 0xFFFFu) == 0u) { f = 1.f; up = 0.f; }   // nothing seen: the scales may be anything
                         float x = 0.f, y = 0.f;
 #pragma unroll
                         for (int k = 0; k < 16; k += 2) {
-                            float u = fast_exp2(fmaf(__uint_as_float(s[16 * h + k]), f, off));
-                            float v = fast_exp2(fmaf(__uint_as_float(s[16 * h + k + 1]), f, off));
-                            if (edge) {
-                                u = masked(g, 16 * g + k) ? 0.f : u;
-                                v = masked(g, 16 * g + k + 1) ? 0.f : v;
-                            }
+                            const float u = fast_exp2(fmaf(__uint_as_float(s[16 * h + k]), f, up));
+                            const float v = fast_exp2(fmaf(__uint_as_float(s[16 * h + k + 1]), f, up));
                             x += u;
                             y += v;
                             out[8 * h + (k >> 1)] = half2_word(u, v);
                         }
-                        l = fmaf(x + y, fminf(inv[g] * R, 1.152921504606846976e18f), l);
+                        l = fmaf(x + y, fminf(sc[16 + g] * R, 1.152921504606846976e18f), l);
                     }
-                    tmem_st16_words(tm_s + 16u * chunk, out);
+                    tmem_st16_words(tm_s + static_cast<uint32_t>(c0 / 2), out);
                 };
+                // the weights of 32 columns go over 16: those of columns 0 .. 63 over the first 32, read by then
                 tmem_ld32_nowait(tm_s, a);
-                tmem_wait32(a);
                 tmem_ld32_nowait(tm_s + 32, b);
-                tmem_wait32(b);                                    // chunk 0's weights go over columns 0-15, chunk 1's over 16-31, ...
-                weigh(a, 0);
-                tmem_ld32_nowait(tm_s + 64, a);
-                weigh(b, 1);
                 tmem_wait32(a);
-                tmem_ld32_nowait(tm_s + 96, b);
-                weigh(a, 2);
                 tmem_wait32(b);
-                weigh(b, 3);
+#pragma unroll 1
+                for (int c0 = 0; c0 < kTok; c0 += 64) {
+                    weigh(a, c0);
+                    if (c0 == 0) tmem_ld32_nowait(tm_s + 64, a);
+                    weigh(b, c0 + 32);
+                    if (c0 == 0) {
+                        tmem_ld32_nowait(tm_s + 96, b);
+                        tmem_wait32(a);
+                        tmem_wait32(b);
+                    }
+                }
             }
             tmem_st_wait();
             tc_fence_before();
