@@ -121,15 +121,27 @@ struct Kv8Cache {
     const int32_t* lens;
     int* status;
     int num_pages, page_size, scale_block, num_kv_heads, num_seqs, table_width;
+    int scale_shift;        // log2(scale_block)
+    uint64_t page_magic;    // ceil(2^64 / page_size)
     int64_t table_stride;
 };
+// tok / page_size by a multiplication (exact below 2^31: the error of tok * ceil(2^64 / d) / 2^64 is under tok / 2^64 < 1 / d)
+__device__ __forceinline__ int kv8_page_index(const Kv8Cache& c, int tok) {
+    return static_cast<int>(__umul64hi(static_cast<uint64_t>(static_cast<uint32_t>(tok)), c.page_magic));
+}
+__device__ __forceinline__ int kv8_in_page(const Kv8Cache& c, int tok) { return tok - kv8_page_index(c, tok) * c.page_size; }
 // Page of token `tok` of sequence `seq`, or -1.
 __device__ __forceinline__ int kv8_page(const Kv8Cache& c, int seq, int tok) {
-    const int i = tok / c.page_size;
+    const int i = kv8_page_index(c, tok);
     if (i >= c.table_width) return -1;
     const int p = __ldg(c.tables + seq * c.table_stride + i);
     return p >= 0 && p < c.num_pages ? p : -1;
 }
+// Row of slot `in_page` of (page, head), and the scale of a row.
+__device__ __forceinline__ int64_t kv8_row(const Kv8Cache& c, int page, int head, int in_page) {
+    return (static_cast<int64_t>(page) * c.num_kv_heads + head) * c.page_size + in_page;
+}
+__device__ __forceinline__ int64_t kv8_scale_at(const Kv8Cache& c, int64_t row) { return row >> c.scale_shift; }
 __device__ __forceinline__ void kv8_report(const Kv8Cache& c, int code) {
     if (c.status != nullptr) atomicExch(c.status, code);
 }

@@ -56,6 +56,8 @@ int32_t kv8_check(const er_kv8_cache* c, Kv8Cache* out) {
     out->scale_block = static_cast<int>(c->scale_block); out->num_kv_heads = static_cast<int>(c->num_kv_heads);
     out->num_seqs = static_cast<int>(c->num_seqs); out->table_width = static_cast<int>(c->block_table_width);
     out->table_stride = c->block_table_stride;
+    out->scale_shift = c->scale_block == 16 ? 4 : c->scale_block == 32 ? 5 : c->scale_block == 64 ? 6 : 7;
+    out->page_magic = ~0ull / c->page_size + 1;   // page_size >= 16
     return ER_OK;
 }
 
@@ -220,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_append_kernel(const __grid_co
     }
     const int lead = max(0, first_pos - block_pos);        // rows of the block that were there before
     const int end = min(sb, len - block_pos);              // rows lead .. end are new
-    const int in_page = block_pos % c.page_size;
+    const int in_page = kv8_in_page(c, block_pos);
     const int token0 = begin + block_pos - first_pos;      // the call's token at row 0 of the block (negative below `lead`)
     for (int e = threadIdx.x; e < (end - lead) * p.rotated; e += kThreads) {
         const int t = e / p.rotated, pair = e - t * p.rotated;
@@ -247,8 +249,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_append_kernel(const __grid_co
                 Act<T>::unpack(__ldg(reinterpret_cast<const uint4*>(src + HALF)), b[ps]);
             }
         }
-        const int64_t at = (static_cast<int64_t>(page) * c.num_kv_heads + head) * c.page_size + in_page;
-        float* scale_at = c.scales[side] + at / sb;
+        const int64_t at = kv8_row(c, page, head, in_page);
+        float* scale_at = c.scales[side] + kv8_scale_at(c, at);
         const float old = on && lead > 0 ? *scale_at : 0.f;
         if (side == 0) {                                                // uniform over a warp
 #pragma unroll

@@ -252,8 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
             const int tok = (pp.r.first_unit + pp.unit + pu) * kKv8Unit;
             float* sc = my_scales + pstage * 2;
             if (tok < pp.r.len && ppage >= 0) {
-                const int head = pp.item / pp.r.row_tiles, in_page = tok % c.page_size;
-                const int64_t row = (static_cast<int64_t>(ppage) * c.num_kv_heads + head) * c.page_size + in_page;
+                const int64_t row = kv8_row(c, ppage, pp.item / pp.r.row_tiles, kv8_in_page(c, tok));
                 const uint32_t dst = smem_u32(my_stages + pstage * Stage<D>::kBytes);
 #pragma unroll
                 for (int i = 0; i < 2 * Stage<D>::kChunks / 32; ++i) {
@@ -261,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
                     const int r = k / (D / 16), ch = k % (D / 16);
                     cp_async16(dst + side * Stage<D>::kSide + Stage<D>::at(r, ch), c.codes[side] + row * D + k * 16);
                 }
-                if (lane < 2) cp_async4(smem_u32(sc + lane), c.scales[lane] + row / c.scale_block);
+                if (lane < 2) cp_async4(smem_u32(sc + lane), c.scales[lane] + kv8_scale_at(c, row));
             } else {                // nothing to see: no row yet, or no page
                 if (lane < 2) sc[lane] = -1.f;
                 if (tok < pp.r.len && lane == 0) kv8_report(c, ER_ERR_OUT_OF_PAGES);

@@ -11,8 +11,8 @@
 // the products of the other run.
 //   warps 0-3, 4-7   softmax of tile 0, 1: a thread is a row.  Reads S from tensor memory twice (maximum, then weights), writes w as fp16 over S.  The
 //                    running maximum may lag by 2^8 before the row of O is rescaled in tensor memory, so that this is rare.
-//   warps 8-11       fetch 128 tokens of codes at a time (loads of the next half tile in registers while this one is converted), write them as
-//                    fp16 into the operand layout: a conversion in the loader reads 1 byte an element from L2 and serves 256 rows.
+//   warps 8-11, 13-15  fetch codes and write them as fp16 into the operand layout: a conversion in the loader reads 1 byte an element from L2
+//                    and serves 256 rows.
 //   warp 12          one lane issues the products: S_i = Q_i K^T (M128 N128 K16 steps, operands in shared memory), O_i += W_i V (A from tensor memory).
 //                    Products of one thread execute in the order of issue, so that S_i of the next tokens may overwrite W_i.
 // Tensor memory: S_0, S_1 at columns 0, 128; O_0, O_1 at 256, 384.  Shared memory: Q (2 x 128 rows), a ring of K / V tiles of 128 tokens, scales.
@@ -26,8 +26,8 @@ namespace er {
 namespace {
 
 constexpr int kTok = 128;                  // tokens of a K / V tile
-constexpr int kSoftWarps = 8, kLoadWarps = 4;
-constexpr int kThreads = 512;             // three of the last four warps idle: registers move between groups of four warps
+constexpr int kSoftWarps = 8, kLoadWarps = 7, kIssueWarp = 12;   // loaders: warps 8-11 and 13-15
+constexpr int kThreads = 512;
 constexpr int kScaleRing = 4;
 constexpr float kLag = 8.f;                // how far (log2) a row's maximum may rise above the one in use
 constexpr float kCarry = 5.f;              // weights are carried 2^5 times: w <= 2^(8 + 2 + 5) < 65504
@@ -81,7 +81,7 @@ struct Waiter {
     volatile int* abort_flag;
     const Kv8Cache* cache;
     __device__ __forceinline__ void operator()(uint64_t* bar, uint32_t parity) const {
-        if (*abort_flag || mbar_try_wait(bar, parity)) return;
+        if (mbar_try_wait(bar, parity) || *abort_flag) return;
         const uint64_t start = global_timer_ns();
         uint32_t spins = 0;
         while (!mbar_try_wait(bar, parity)) {
@@ -106,6 +106,36 @@ __device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
                    "+r"(r[31])
                  :
                  : "memory");
+}
+__device__ __forceinline__ bool elect_lane() {
+    uint32_t on;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(on));
+    return on != 0u;
+}
+// Two float32 lanes in one instruction.
+struct F2 {
+    uint64_t v;
+};
+__device__ __forceinline__ F2 pack2(float a, float b) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(F2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 __device__ __forceinline__ uint32_t half2_word(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
@@ -154,16 +184,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     if (tid == 0) {
         for (int i = 0; i < kNumBars; ++i) {
             uint32_t n = 1;
-            if (i < kBarEmpty) n = kLoadWarps * 32;
-            else if (i == kBarP || i == kBarP + 1) n = 128;
+            if (i < kBarEmpty) n = kTok / 16;
+            else if (i == kBarP || i == kBarP + 1) n = 4;
             else if (i == kBarQ) n = two ? 256 : 128;
-            else if (i >= kBarScale) n = kLoadWarps;
+            else if (i >= kBarScale) n = kTok / 16;
             mbar_init(bars + i, n);
         }
         *abort_flag = 0;
         mbar_init_fence();
     }
-    if (warp == kSoftWarps + kLoadWarps) {
+    if (warp == kIssueWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -172,36 +202,120 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const Waiter wait{abort_flag, &c};
-    // Registers of the groups of four warps: 512 threads x 128 at launch = 128 x (168 + 168 + 104 + 72).  Each branch moves its own.
-    if (warp >= kSoftWarps + kLoadWarps) {
-        // ================= products =================
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (warp == kSoftWarps + kLoadWarps && lane == 0 && tiles > 0) {
+    // Codes -> fp16 operand tiles.  The 16-token units of the half tiles (keys of tile 0, values of tile 0, keys of tile 1, ...; eight to a half
+    // tile) go round robin to the loader warps, each with three units in flight in registers.  Lane: 16 codes of the rows lane / 4 and 8 further, two
+    // rows of four chunks to eight lanes, which store without bank conflicts.
+    auto load_tiles = [&](int w) {
+        constexpr int kParts = D / 64, kLoads = 2 * kParts;          // 64 codes of 8 rows at a time
+        struct Unit {
+            uint4 v[kLoads];
+            float kscale, vscale;
+            int page;
+        };
+        const int r8 = lane >> 2, c4 = lane & 3;
+        const uint32_t dst_lane = sbase + um_swz(r8, 2 * c4), dst_lane2 = sbase + um_swz(r8, 2 * c4 + 1);
+        const int64_t src_lane = static_cast<int64_t>(r8) * D + c4 * 16;
+        const int total = 16 * tiles;
+        auto token_of = [&](int q) { return (t_begin + (q >> 4)) * kTok + (q & 7) * 16; };
+        auto look_up = [&](Unit& x, int q) { x.page = q < total && token_of(q) < tile.len ? kv8_page(c, tile.seq, token_of(q)) : -1; };
+        auto fetch = [&](Unit& x, int q) {
+            const int side = (q >> 3) & 1, tok = token_of(q), valid = x.page >= 0 ? tile.len - tok : 0;
+            const int64_t row = kv8_row(c, max(x.page, 0), head, kv8_in_page(c, tok));
+            const uint8_t* src = (side ? c.codes[1] : c.codes[0]) + row * D + src_lane;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                x.v[i] = make_uint4(0, 0, 0, 0);
+                if (r8 + 8 * (i / kParts) < valid) x.v[i] = __ldg(reinterpret_cast<const uint4*>(src + (i / kParts) * 8 * D + (i % kParts) * 64));
+            }
+            if (side == 0 && lane == 0) {
+                x.kscale = -1.f;
+                x.vscale = 0.f;
+                if (valid > 0) {
+                    x.kscale = __ldg(c.scales[0] + kv8_scale_at(c, row));
+                    x.vscale = __ldg(c.scales[1] + kv8_scale_at(c, row));
+                } else if (q < total && tok < tile.len) {
+                    kv8_report(c, ER_ERR_OUT_OF_PAGES);
+                }
+            }
+        };
+        auto step = [&](Unit& x, int q) {
+            if (q >= total) return;
+            const int idx = q >> 3, st = idx % kStages, j = idx >> 1, u = q & 7;
+            if (idx >= kStages) wait(bars + kBarEmpty + st, ((idx / kStages) - 1) & 1);
+            const uint32_t at = st * kTile + u * 16 * 128;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                uint4 a, b;                                            // codes 0 .. 8, 8 .. 16 of the lane
+                decode4<E4M3>(x.v[i].x, a.x, a.y);
+                decode4<E4M3>(x.v[i].y, a.z, a.w);
+                decode4<E4M3>(x.v[i].z, b.x, b.y);
+                decode4<E4M3>(x.v[i].w, b.z, b.w);
+                const uint32_t off = at + (i / kParts) * 8 * 128 + (i % kParts) * kRegion;
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst_lane + off), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w) : "memory");
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst_lane2 + off), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w) : "memory");
+            }
+            if ((idx & 1) == 0 && lane == 0) {
+                float* s = scale_ring + (j % kScaleRing) * 32 + u;
+                s[0] = x.kscale;
+                s[8] = __log2f(x.vscale);                              // NaN stays NaN; 0 gives -inf
+                s[16] = 1.f / x.vscale;
+                mbar_arrive(bars + kBarScale + j % kScaleRing);
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bars + kBarFull + st);
+            fetch(x, q + kLoadWarps);
+            look_up(x, q + 2 * kLoadWarps);
+        };
+        Unit x;
+        look_up(x, w);
+        fetch(x, w);
+        look_up(x, w + kLoadWarps);
+        for (int q = w; q < total; q += kLoadWarps) {
+            step(x, q);
+        }
+    };
+
+    // Registers of the groups of four warps: 512 threads x 128 at launch = 128 x (168 + 168 + 88 + 88).  Each branch moves its own.
+    if (warp >= kSoftWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp != kIssueWarp) {
+            load_tiles(warp - kSoftWarps - (warp > kIssueWarp ? 1 : 0));
+        } else if (tiles > 0) {
+            // ================= products: the whole warp walks the loop, so that descriptors stay in uniform registers; one lane issues =================
+            const bool leader = elect_lane();
             constexpr uint32_t kHi = umma_desc_hi(1024);
             constexpr uint32_t idesc_qk = umma_idesc(128, kTok, false), idesc_pv = umma_idesc(128, D, true);
             const uint32_t ring_lo = umma_desc_lo(sbase, 16), v_lo = umma_desc_lo(sbase, kRegion), q_lo = umma_desc_lo(sbase + kStages * kTile, 16);
             auto scores = [&](int i, int idx) {                  // S_i = Q_i K^T, K in ring entry idx
                 uint32_t kd = ring_lo + static_cast<uint32_t>(idx % kStages) * (kTile >> 4), qd = q_lo + i * (kTile >> 4);
-                asm volatile("" : "+r"(kd), "+r"(qd));           // one add an operand here, not a register a descriptor kept over the loop
+                if (leader) {
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint32_t off = ((kk >> 2) * kRegion + (kk & 3) * 32) >> 4;
-                    umma_f16(tmem + 128u * i, umma_desc_pack(qd + off, kHi), umma_desc_pack(kd + off, kHi), idesc_qk, kk > 0);
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint32_t off = ((kk >> 2) * kRegion + (kk & 3) * 32) >> 4;
+                        umma_f16(tmem + 128u * i, umma_desc_pack(qd + off, kHi), umma_desc_pack(kd + off, kHi), idesc_qk, kk > 0);
+                    }
+                    umma_commit(smem_u32(bars + kBarS + i));
                 }
-                umma_commit(smem_u32(bars + kBarS + i));
+                __syncwarp();
             };
             auto outputs = [&](int i, int idx, bool first) {     // O_i += W_i V
                 uint32_t vd = v_lo + static_cast<uint32_t>(idx % kStages) * (kTile >> 4), a = tmem + 128u * i;
-                asm volatile("" : "+r"(vd), "+r"(a));
+                if (leader) {
 #pragma unroll
-                for (int kt = 0; kt < kTok / 16; ++kt)
-                    umma_f16_ts(tmem + 256u + 128u * i, a + 8u * kt, umma_desc_pack(vd + ((kt * 2048) >> 4), kHi), idesc_pv, !first || kt > 0);
+                    for (int kt = 0; kt < kTok / 16; ++kt)
+                        umma_f16_ts(tmem + 256u + 128u * i, a + 8u * kt, umma_desc_pack(vd + ((kt * 2048) >> 4), kHi), idesc_pv, !first || kt > 0);
+                }
+                __syncwarp();
             };
             auto full = [&](int idx) {
                 wait(bars + kBarFull + idx % kStages, (idx / kStages) & 1);
                 tc_fence_after();
             };
-            auto release = [&](int idx) { umma_commit(smem_u32(bars + kBarEmpty + idx % kStages)); };
+            auto release = [&](int idx) {
+                if (leader) umma_commit(smem_u32(bars + kBarEmpty + idx % kStages));
+                __syncwarp();
+            };
             wait(bars + kBarQ, 0);
             full(0);
             scores(0, 0);
@@ -229,103 +343,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                     release(ki);
                 }
             }
-            umma_commit(smem_u32(bars + kBarO));
-        }
-    } else if (warp >= kSoftWarps) {
-        // ================= loader: codes -> fp16 operand tiles =================
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-        // A lane holds 16 codes of a row, D / 16 lanes a row; a warp fetches 32 rows, two units of 16 tokens.
-        constexpr int kLanes = D / 16, kRows = 32 / kLanes, kLoads = 32 / kRows;
-        const int w = warp - kSoftWarps, ch = lane % kLanes, sub = lane / kLanes;
-        int page_now[2] = {-1, -1}, page_next[2];
-        int64_t at_now[2] = {0, 0};            // first row of the unit in the cache
-        auto place = [&](int j) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int tok = (t_begin + j) * kTok + w * 32 + u * 16;
-                at_now[u] = (static_cast<int64_t>(max(page_now[u], 0)) * c.num_kv_heads + head) * c.page_size + tok % c.page_size;
-            }
-        };
-        auto pages = [&](int j, int (&pg)[2]) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int tok = (t_begin + j) * kTok + w * 32 + u * 16;
-                pg[u] = j < tiles && tok < tile.len ? kv8_page(c, tile.seq, tok) : -1;
-            }
-        };
-        uint4 buf[kLoads];
-        auto fetch = [&](int j, int side) {
-            const int tok0 = (t_begin + j) * kTok + w * 32;
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                const int r = i * kRows + sub, u = i * kRows / 16;
-                buf[i] = make_uint4(0, 0, 0, 0);
-                if (page_now[u] >= 0 && tok0 + r < tile.len)
-                    buf[i] = __ldg(reinterpret_cast<const uint4*>(c.codes[side] + (at_now[u] + (r - 16 * u)) * D + ch * 16));
-            }
-        };
-        float kscale = 0.f, vscale = 0.f;      // lanes 0, 1: of their unit
-        auto fetch_scales = [&](int j) {
-            if (lane < 2) {
-                const int tok = (t_begin + j) * kTok + w * 32 + lane * 16, page = lane == 0 ? page_now[0] : page_now[1];
-                kscale = -1.f;
-                vscale = 0.f;
-                if (page >= 0) {
-                    const int64_t at = (lane == 0 ? at_now[0] : at_now[1]) / c.scale_block;
-                    kscale = __ldg(c.scales[0] + at);
-                    vscale = __ldg(c.scales[1] + at);
-                } else if (j < tiles && tok < tile.len) {
-                    kv8_report(c, ER_ERR_OUT_OF_PAGES);
-                }
-            }
-        };
-        if (tiles > 0) {
-            pages(0, page_now);
-            place(0);
-            fetch(0, 0);
-            fetch_scales(0);
-            pages(1, page_next);
-            for (int idx = 0; idx < 2 * tiles; ++idx) {
-                const int j = idx >> 1, st = idx % kStages;
-                uint4 cur[kLoads];
-#pragma unroll
-                for (int i = 0; i < kLoads; ++i) cur[i] = buf[i];
-                if ((idx & 1) == 0) {                              // keys of tile j are here; publish its scales, fetch its values
-                    if (lane < 2) {
-                        float* s = scale_ring + (j % kScaleRing) * 32 + w * 2 + lane;
-                        s[0] = kscale;
-                        s[8] = __log2f(vscale);                    // NaN stays NaN; 0 gives -inf
-                        s[16] = 1.f / vscale;
-                    }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(bars + kBarScale + j % kScaleRing);
-                    fetch(j, 1);
-                } else if (j + 1 < tiles) {
-                    page_now[0] = page_next[0];
-                    page_now[1] = page_next[1];
-                    place(j + 1);
-                    fetch(j + 1, 0);
-                    fetch_scales(j + 1);
-                    pages(j + 2, page_next);
-                }
-                if (idx >= kStages) wait(bars + kBarEmpty + st, ((idx / kStages) - 1) & 1);
-                uint8_t* dst = gen + st * kTile;
-#pragma unroll
-                for (int i = 0; i < kLoads; ++i) {
-                    const int r = w * 32 + i * kRows + sub;
-                    uint4 a, b;                                    // dims 16 ch .. + 8, + 8 .. + 16
-                    decode4<E4M3>(cur[i].x, a.x, a.y);
-                    decode4<E4M3>(cur[i].y, a.z, a.w);
-                    decode4<E4M3>(cur[i].z, b.x, b.y);
-                    decode4<E4M3>(cur[i].w, b.z, b.w);
-                    uint8_t* row = dst + (ch >> 2) * kRegion;
-                    const int c0 = 2 * (ch & 3), swap = (D == 128) ? ch >> 2 : 0;   // the lanes of the second region store their odd chunk first: no bank conflict
-                    *reinterpret_cast<uint4*>(row + um_swz(r, c0 + swap)) = swap ? b : a;
-                    *reinterpret_cast<uint4*>(row + um_swz(r, c0 + 1 - swap)) = swap ? a : b;
-                }
-                fence_async_smem();
-                mbar_arrive(bars + kBarFull + st);
-            }
+            if (leader) umma_commit(smem_u32(bars + kBarO));
+            __syncwarp();
         }
     } else {
         // ================= softmax =================
@@ -405,10 +424,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                     for (int h = 0; h < 2; ++h) {
                         float x = __uint_as_float(s[16 * h]), y = __uint_as_float(s[16 * h + 1]);
 #pragma unroll
-                        for (int k = 2; k < 16; k += 2) {
-                            x = fmaxf(x, __uint_as_float(s[16 * h + k]));
-                            y = fmaxf(y, __uint_as_float(s[16 * h + k + 1]));
+                        for (int k = 2; k < 14; k += 4) {
+                            x = max3(x, __uint_as_float(s[16 * h + k]), __uint_as_float(s[16 * h + k + 1]));
+                            y = max3(y, __uint_as_float(s[16 * h + k + 2]), __uint_as_float(s[16 * h + k + 3]));
                         }
+                        x = max3(x, __uint_as_float(s[16 * h + 14]), __uint_as_float(s[16 * h + 15]));
                         const float top = fmaxf(x, y), ks = sc[c0 / 16 + h];
                         mx = fmaxf(mx, ks < 0.f ? -INFINITY : top * ks);          // scales are not negative but for the mark of a hidden block
                     }
@@ -465,15 +485,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                         up = (up < -60.f ? -60.f : up) - base;   // a NaN stays; below 2^-60 a weight is nothing in fp16, but counts in the sum
                         if (f == 0.f) f = 1.17549435e-38f;       // a hidden -inf stays one
                         if ((bits >> (16 * h) & 0xFFFFu) == 0u) { f = 1.f; up = 0.f; }   // nothing seen: the scales may be anything
-                        float x = 0.f, y = 0.f;
+                        const F2 f2 = pack2(f, f), up2 = pack2(up, up);
+                        F2 sum = pack2(0.f, 0.f), sum2 = sum;
 #pragma unroll
                         for (int k = 0; k < 16; k += 2) {
-                            const float u = fast_exp2(fmaf(__uint_as_float(s[16 * h + k]), f, up));
-                            const float v = fast_exp2(fmaf(__uint_as_float(s[16 * h + k + 1]), f, up));
-                            x += u;
-                            y += v;
+                            float u, v;
+                            unpack2(fma2(pack2(__uint_as_float(s[16 * h + k]), __uint_as_float(s[16 * h + k + 1])), f2, up2), u, v);
+                            u = fast_exp2(u);
+                            v = fast_exp2(v);
+                            if (k & 2) sum2 = add2(sum2, pack2(u, v)); else sum = add2(sum, pack2(u, v));
                             out[8 * h + (k >> 1)] = half2_word(u, v);
                         }
+                        float x, y;
+                        unpack2(add2(sum, sum2), x, y);
                         l = fmaf(x + y, fminf(sc[16 + g] * R, 1.152921504606846976e18f), l);
                     }
                     tmem_st16_words(tm_s + static_cast<uint32_t>(c0 / 2), out);
@@ -497,7 +521,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             }
             tmem_st_wait();
             tc_fence_before();
-            mbar_arrive(bars + kBarP + i);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bars + kBarP + i);      // one arrival a warp: 128 of them would queue at the barrier
         }
         // ---- the rows ----
         if (tiles > 0) {
@@ -530,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == kSoftWarps + kLoadWarps) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    if (warp == kIssueWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
 // Joins the parts of the split tile pairs: a warp per query row, a lane D / 32 dims.
