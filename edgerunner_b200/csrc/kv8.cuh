@@ -142,6 +142,21 @@ __device__ __forceinline__ int64_t kv8_row(const Kv8Cache& c, int page, int head
     return (static_cast<int64_t>(page) * c.num_kv_heads + head) * c.page_size + in_page;
 }
 __device__ __forceinline__ int64_t kv8_scale_at(const Kv8Cache& c, int64_t row) { return row >> c.scale_shift; }
+// Work of a ragged batch is numbered without a prefix sum over it: sequence s owns the numbers from first(starts[s], s) on, `first` growing
+// with both and leaving each sequence room enough.  The sequence that owns `slot`, by whole warps: 32 probes at a time, one round of loads for
+// up to 32 sequences, two for 1024.
+template <typename First>
+__device__ __forceinline__ int kv8_find_slot(const int32_t* starts, int num_seqs, int slot, First first) {
+    int lo = 0, n = num_seqs;                    // it is one of lo .. lo + n
+    while (n > 1) {
+        const int step = (n + 31) / 32, s = lo + static_cast<int>(threadIdx.x & 31) * step;
+        const bool below = s < lo + n && first(__ldg(starts + min(s, num_seqs - 1)), s) <= slot;
+        const int k = max(__popc(__ballot_sync(0xffffffffu, below)) - 1, 0);
+        n = min(step, lo + n - (lo + k * step));
+        lo += k * step;
+    }
+    return lo;
+}
 __device__ __forceinline__ void kv8_report(const Kv8Cache& c, int code) {
     if (c.status != nullptr) atomicExch(c.status, code);
 }

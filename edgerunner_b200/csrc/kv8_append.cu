@@ -197,15 +197,10 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_append_kernel(const __grid_co
         begin = seq; count = 1; j = 0;
     } else {
         const int slot = blockIdx.x;
-        int lo = 0, hi = c.num_seqs;     // largest s with starts[s] / sb + 2 s <= slot
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (__ldg(p.starts + mid) / sb + 2 * mid <= slot) lo = mid; else hi = mid;
-        }
-        seq = lo;
+        seq = kv8_find_slot(p.starts, c.num_seqs, slot, [&](int start, int s) { return (start >> c.scale_shift) + 2 * s; });
         begin = __ldg(p.starts + seq);
         count = __ldg(p.starts + seq + 1) - begin;
-        j = slot - (begin / sb + 2 * seq);
+        j = slot - ((begin >> c.scale_shift) + 2 * seq);
     }
     if (count == 0 || j < 0) return;
     const int len = __ldg(c.lens + seq), first_pos = len - count;

@@ -53,15 +53,12 @@ struct Tile {
     int wrong;                                 // what the host could not see: an ER_ERR_* code, or 0
 };
 __device__ __forceinline__ Tile find_tile(const Kv8Prefill& p, int slot) {
-    int lo = 0, hi = p.cache.num_seqs;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (static_cast<int>(static_cast<int64_t>(__ldg(p.starts + mid)) * p.group / 256) + mid <= slot) lo = mid; else hi = mid;
-    }
+    const int lo = kv8_find_slot(p.starts, p.cache.num_seqs, slot, [&](int start, int s) { return static_cast<int>(static_cast<int64_t>(start) * p.group / 256) + s; });
     Tile t;
     t.seq = lo;
     t.begin = __ldg(p.starts + lo);
     t.n = __ldg(p.starts + lo + 1) - t.begin;
+    const int len = __ldg(p.cache.lens + lo);
     t.rows = 0;
     t.row0 = (slot - (static_cast<int>(static_cast<int64_t>(t.begin) * p.group / 256) + lo)) * 256;
     t.len = 0;
@@ -70,7 +67,7 @@ __device__ __forceinline__ Tile find_tile(const Kv8Prefill& p, int slot) {
     const int rows = t.n * p.group;
     if (rows < p.min_rows || t.row0 < 0 || t.row0 >= rows) return t;
     t.rows = rows;
-    t.len = __ldg(p.cache.lens + lo);
+    t.len = len;
     const int most = p.cache.table_width * p.cache.page_size;     // rows behind the table have no page
     t.wrong = t.len > most ? ER_ERR_OUT_OF_PAGES : t.len < 0 ? ER_ERR_SHAPE : 0;
     t.len = max(0, min(t.len, most));
@@ -414,12 +411,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             };
             wait(bars + kBarS + i, j & 1);
             tc_fence_after();
-            // ---- the maximum ----
+            // ---- the maximum; the columns 0 .. 63 last, they stay in registers ----
             float mx = -INFINITY;
-            {
-                uint32_t a[32], b[32];
-                auto take = [&](uint32_t (&s)[32], int c0) {
-                    if (edge) hide(s, seen(c0));
+            uint32_t a[32], b[32];
+            tmem_ld32_nowait(tm_s + 64, a);
+            tmem_ld32_nowait(tm_s + 96, b);
+#pragma unroll 1
+            for (int c0 = 64; c0 >= 0; c0 -= 64) {
+                const float4 ks4 = *reinterpret_cast<const float4*>(sc + c0 / 16);
+                const float ks[4] = {ks4.x, ks4.y, ks4.z, ks4.w};
+                tmem_wait32(a);
+                tmem_wait32(b);
+                if (edge) {
+                    hide(a, seen(c0));
+                    hide(b, seen(c0 + 32));
+                }
+                auto take = [&](const uint32_t (&s)[32], int g0) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         float x = __uint_as_float(s[16 * h]), y = __uint_as_float(s[16 * h + 1]);
@@ -429,20 +436,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                             y = max3(y, __uint_as_float(s[16 * h + k + 2]), __uint_as_float(s[16 * h + k + 3]));
                         }
                         x = max3(x, __uint_as_float(s[16 * h + 14]), __uint_as_float(s[16 * h + 15]));
-                        const float top = fmaxf(x, y), ks = sc[c0 / 16 + h];
-                        mx = fmaxf(mx, ks < 0.f ? -INFINITY : top * ks);          // scales are not negative but for the mark of a hidden block
+                        mx = fmaxf(mx, ks[g0 + h] < 0.f ? -INFINITY : fmaxf(x, y) * ks[g0 + h]);   // scales are not negative but for the mark of a hidden block
                     }
                 };
-                tmem_ld32_nowait(tm_s, a);
-#pragma unroll 1
-                for (int c0 = 0; c0 < kTok; c0 += 64) {
-                    tmem_wait32(a);
-                    tmem_ld32_nowait(tm_s + c0 + 32, b);
-                    take(a, c0);
-                    tmem_wait32(b);
-                    if (c0 == 0) tmem_ld32_nowait(tm_s + 64, a);
-                    take(b, c0 + 32);
-                }
+                take(a, 0);
+                if (c0 > 0) tmem_ld32_nowait(tm_s, a);
+                take(b, 2);
+                if (c0 > 0) tmem_ld32_nowait(tm_s + 32, b);
             }
             mx *= factor;
             // ---- move to it, if it is far enough above the one in use ----
@@ -466,58 +466,63 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                     }
                 }
             }
-            // ---- weights ----
+            // ---- weights: those of 64 columns go over 32, read by then ----
             const float base = m == -INFINITY ? 0.f : m;
             const float R = fast_exp2(LR - kCarry);
-            {
-                uint32_t a[32], b[32];
-                auto weigh = [&](uint32_t (&s)[32], int c0) {
-                    uint32_t bits = 0xFFFFFFFFu;
-                    if (edge) {
-                        bits = seen(c0);
-                        hide(s, bits);
+#pragma unroll 1
+            for (int c0 = 0; c0 < kTok; c0 += 64) {
+                // of the four blocks of 16: the factor of a score, the exponent's offset, what a sum of weights counts
+                const float4 k4 = *reinterpret_cast<const float4*>(sc + c0 / 16), e4 = *reinterpret_cast<const float4*>(sc + 8 + c0 / 16),
+                             i4 = *reinterpret_cast<const float4*>(sc + 16 + c0 / 16);
+                float f[4] = {k4.x, k4.y, k4.z, k4.w}, up[4] = {e4.x, e4.y, e4.z, e4.w}, count[4] = {i4.x, i4.y, i4.z, i4.w};
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    up[g] = up[g] - LR + kCarry;
+                    up[g] = (up[g] < -60.f ? -60.f : up[g]) - base;   // a NaN stays; below 2^-60 a weight is nothing in fp16, but counts in the sum
+                    f[g] *= factor;
+                    count[g] = fminf(count[g] * R, 1.152921504606846976e18f);
+                }
+                if (c0 > 0) {
+                    tmem_wait32(a);
+                    tmem_wait32(b);
+                }
+                if (edge) {
+                    const uint32_t bits[2] = {seen(c0), seen(c0 + 32)};
+                    hide(a, bits[0]);
+                    hide(b, bits[1]);
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        if (f[g] == 0.f) f[g] = 1.17549435e-38f;      // a hidden -inf stays one
+                        if ((bits[g >> 1] >> (16 * (g & 1)) & 0xFFFFu) == 0u) { f[g] = 1.f; up[g] = 0.f; }   // nothing seen: the scales may be anything
                     }
-                    uint32_t out[16];
+                }
+                uint32_t out[32];
+                auto weigh = [&](const uint32_t (&s)[32], int g0) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const int g = c0 / 16 + h;
-                        float up = sc[8 + g] - LR + kCarry, f = sc[g] * factor;
-                        up = (up < -60.f ? -60.f : up) - base;   // a NaN stays; below 2^-60 a weight is nothing in fp16, but counts in the sum
-                        if (f == 0.f) f = 1.17549435e-38f;       // a hidden -inf stays one
-                        if ((bits >> (16 * h) & 0xFFFFu) == 0u) { f = 1.f; up = 0.f; }   // nothing seen: the scales may be anything
-                        const F2 f2 = pack2(f, f), up2 = pack2(up, up);
+                        const int g = g0 + h;
+                        const F2 f2 = pack2(f[g], f[g]), up2 = pack2(up[g], up[g]);
                         F2 sum = pack2(0.f, 0.f), sum2 = sum;
 #pragma unroll
                         for (int k = 0; k < 16; k += 2) {
+                            const F2 x2 = fma2(pack2(__uint_as_float(s[16 * h + k]), __uint_as_float(s[16 * h + k + 1])), f2, up2);
                             float u, v;
-                            unpack2(fma2(pack2(__uint_as_float(s[16 * h + k]), __uint_as_float(s[16 * h + k + 1])), f2, up2), u, v);
+                            unpack2(x2, u, v);
                             u = fast_exp2(u);
                             v = fast_exp2(v);
                             if (k & 2) sum2 = add2(sum2, pack2(u, v)); else sum = add2(sum, pack2(u, v));
-                            out[8 * h + (k >> 1)] = half2_word(u, v);
+                            out[8 * g + (k >> 1)] = half2_word(u, v);
                         }
                         float x, y;
                         unpack2(add2(sum, sum2), x, y);
-                        l = fmaf(x + y, fminf(sc[16 + g] * R, 1.152921504606846976e18f), l);
+                        l = fmaf(x + y, count[g], l);
                     }
-                    tmem_st16_words(tm_s + static_cast<uint32_t>(c0 / 2), out);
                 };
-                // the weights of 32 columns go over 16: those of columns 0 .. 63 over the first 32, read by then
-                tmem_ld32_nowait(tm_s, a);
-                tmem_ld32_nowait(tm_s + 32, b);
-                tmem_wait32(a);
-                tmem_wait32(b);
-#pragma unroll 1
-                for (int c0 = 0; c0 < kTok; c0 += 64) {
-                    weigh(a, c0);
-                    if (c0 == 0) tmem_ld32_nowait(tm_s + 64, a);
-                    weigh(b, c0 + 32);
-                    if (c0 == 0) {
-                        tmem_ld32_nowait(tm_s + 96, b);
-                        tmem_wait32(a);
-                        tmem_wait32(b);
-                    }
-                }
+                weigh(a, 0);
+                if (c0 == 0) tmem_ld32_nowait(tm_s + 64, a);
+                weigh(b, 2);
+                if (c0 == 0) tmem_ld32_nowait(tm_s + 96, b);
+                tmem_st32_words(tm_s + static_cast<uint32_t>(c0 / 2), out);
             }
             tmem_st_wait();
             tc_fence_before();
