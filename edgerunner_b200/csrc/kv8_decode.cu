@@ -6,10 +6,10 @@
 // w = p * b / R with R the largest value scale so far (so w <= 1 whatever the scales are), carried 4096 times so that small ones stay normal
 // fp16 numbers; R and m move together and rarely.
 //
-// Work.  Bound by memory: 2 D bytes a row for 4 D flops a query head.  A persistent CTA per SM; the list of 16-token units of all (sequence, kv head,
+// Work.  Bound by memory: 2 D bytes a row for 4 D flops a query head.  A persistent CTA per SM; the list of 32-token units of all (sequence, kv head,
 // row tile) items is cut evenly over the CTAs whatever the lengths are, inside a CTA the units of an item go round robin to the warps.  A warp
 // streams its units through its own ring of shared-memory stages with cp.async (16 bytes a lane, no barrier between warps, several units in
-// flight: 160 to 190 KB a SM), and runs both products of a unit alone: scores as S^T = K q^T (16 tokens x 8 query rows), outputs as O^T = V^T w^T
+// flight: 160 to 190 KB a SM), and runs both products of a unit alone: scores as S^T = K q^T (2 x 16 tokens x 8 query rows), outputs as O^T = V^T w^T
 // (16 dims x 8 query rows), so eight query rows fill a tile and K is an A operand as it lies in memory.  The warps of a CTA are joined in shared
 // memory at the end of an item, the CTAs that share an item by a second small launch that overlaps this one's tail.
 //
@@ -25,6 +25,7 @@ namespace er {
 namespace {
 
 constexpr int kWarps = 8, kThreads = kWarps * 32;
+constexpr int kUnit = 2 * kKv8Unit;   // tokens that a warp takes at a time: two halves, each with a page and scales of its own
 constexpr float kWeightScale = 4096.f;
 
 struct Kv8Decode {
@@ -43,7 +44,7 @@ struct Kv8Decode {
 // Query row r of a (sequence, kv head) is query r / group, head r % group of the kv head's group; tile_rows of them make an item.
 struct SeqRange {
     int len, begin, n;              // rows in the cache, first query token, queries
-    int first_unit, units;          // first 16-token unit that a query can see, units of an item (at least 1: an empty one writes zeros)
+    int first_unit, units;          // first unit that a query can see, units of an item (at least 1: an empty one writes zeros)
     int row_tiles;                  // 0 for a sequence without queries
 };
 __device__ __forceinline__ SeqRange seq_range(const Kv8Decode& p, int seq) {
@@ -60,8 +61,8 @@ __device__ __forceinline__ SeqRange seq_range(const Kv8Decode& p, int seq) {
     if (p.few_rows > 0 && r.n * p.group > p.few_rows) r.row_tiles = 0;
     r.len = max(0, min(__ldg(p.cache.lens + seq), p.cache.table_width * p.cache.page_size));   // rows behind the table have no page
     const int lo = p.window > 0 ? max(0, r.len - r.n - p.window + 1) : 0;
-    r.first_unit = lo / kKv8Unit;
-    r.units = max(1, (r.len + kKv8Unit - 1) / kKv8Unit - r.first_unit);
+    r.first_unit = lo / kUnit;
+    r.units = max(1, (r.len + kUnit - 1) / kUnit - r.first_unit);
     return r;
 }
 struct Place {        // a position in the list
@@ -80,14 +81,16 @@ struct Place {        // a position in the list
     __device__ __forceinline__ int last_query(const Kv8Decode& p) const {
         return (min(r.n * p.group, (item % r.row_tiles + 1) * p.tile_rows) - 1) / p.group;
     }
+    // The first row that the tile sees: pages in front of it may be gone.
+    __device__ __forceinline__ int lowest(const Kv8Decode& p) const { return p.window > 0 ? max(0, r.len - r.n + first_query(p) - p.window + 1) : 0; }
     // Of the `count` units from `unit` on, those [u0, u1) that the tile sees anything of.
     __device__ __forceinline__ void visible(const Kv8Decode& p, int count, int& u0, int& u1) const {
-        const int base = first_unit_token() / kKv8Unit, end = r.len - r.n + last_query(p) + 1;      // rows below `end`
-        const int lo = p.window > 0 ? max(0, r.len - r.n + first_query(p) - p.window + 1) / kKv8Unit : 0;
+        const int base = r.first_unit + unit, end = r.len - r.n + last_query(p) + 1;      // rows below `end`
+        const int lo = lowest(p) / kUnit;
         u0 = max(0, lo - base);
-        u1 = min(count, max(0, end + kKv8Unit - 1) / kKv8Unit - base);
+        u1 = min(count, max(0, end + kUnit - 1) / kUnit - base);
     }
-    __device__ __forceinline__ int first_unit_token() const { return (r.first_unit + unit) * kKv8Unit; }
+    __device__ __forceinline__ int token(int u) const { return (r.first_unit + unit + u) * kUnit; }   // of the u-th unit from here
 };
 // Total units, by every thread of the CTA (scratch: kWarps + 1 values).
 __device__ int64_t total_units(const Kv8Decode& p, int64_t* scratch) {
@@ -173,10 +176,10 @@ __device__ __forceinline__ void split_half2(float a, float b, uint32_t& hi, uint
     lo = half2_bits(a - f.x, b - f.y);
 }
 
+// A stage: keys of the two halves, values of the two halves.
 template <int D> struct Stage {
-    static constexpr int kSide = kKv8Unit * D, kBytes = 2 * kSide;
-    static constexpr int kChunks = kSide / 16;   // 16-byte chunks of one side
-    // byte offset of chunk c of row r inside a side
+    static constexpr int kHalf = kKv8Unit * D, kSide = 2 * kHalf, kBytes = 2 * kSide;
+    // byte offset of 16-byte chunk c of row r inside a half
     static __device__ __forceinline__ int at(int r, int c) {
         if constexpr (D == 128) return r * 128 + ((c ^ (r & 7)) << 4);
         else return (r >> 1) * 128 + (((((r & 1) << 2) | c) ^ ((r >> 1 & 3) << 1)) << 4);
@@ -184,11 +187,11 @@ template <int D> struct Stage {
 };
 template <int NT> __host__ __device__ constexpr int decode_rows() { return 8 * NT; }
 template <int D, int NT> __host__ __device__ constexpr int decode_stages() {
-    return D == 128 ? (NT == 1 ? 6 : 4) : (NT == 1 ? 12 : 10);
+    return D == 128 ? (NT == 1 ? 3 : 2) : (NT == 1 ? 6 : 5);
 }
 template <int D, int NT> __host__ __device__ constexpr int join_floats() { return kWarps * 8 * NT * (D + 4); }
 template <int D, int NT> __host__ __device__ constexpr int decode_smem() {
-    return kWarps * decode_stages<D, NT>() * (Stage<D>::kBytes + 8) + (join_floats<D, NT>() + kWarps * 8 * NT * 2) * 4 + 128;
+    return kWarps * decode_stages<D, NT>() * (Stage<D>::kBytes + 16) + (join_floats<D, NT>() + kWarps * 8 * NT * 2) * 4 + 128;
 }
 // One partial: max, sum, -, - and the unnormalised row.
 template <int D> __host__ __device__ constexpr int partial_stride() { return D + 4; }
@@ -204,11 +207,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
     extern __shared__ __align__(16) uint8_t smem[];
     uint8_t* stages = smem;
     float* stage_scales = reinterpret_cast<float*>(smem + kWarps * kStages * Stage<D>::kBytes);
-    float* join = stage_scales + kWarps * kStages * 2;
+    float* join = stage_scales + kWarps * kStages * 4;
     float* join_ml = join + join_floats<D, NT>();
     int64_t* scratch = reinterpret_cast<int64_t*>(join_ml + kWarps * kRows * 2);
     const Kv8Cache& c = p.cache;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, half = lane >> 4;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     const int64_t total = total_units(p, scratch);
@@ -226,12 +229,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
 
     // ---- producer: this warp's units, kStages - 1 ahead ----
     uint8_t* my_stages = stages + warp * kStages * Stage<D>::kBytes;
-    float* my_scales = stage_scales + warp * kStages * 2;
+    float* my_scales = stage_scales + warp * kStages * 4;   // per stage: key and value scale of half 0, of half 1
     Place pp = at;                  // segment the producer is in
     int64_t pleft = left;           // units from pp.unit on
     int pseg = static_cast<int>(min(static_cast<int64_t>(pp.r.units - pp.unit), pleft));   // units of the segment
     int pu, pend;                   // next unit of the segment for this warp; end of those that are worth a look
-    int ppage = -1;                 // its page
+    int ppage = -1;                 // page of this lane's half of it
     bool pmore = true;
     pp.visible(p, pseg, pu, pend);
     pu += warp;
@@ -244,26 +247,30 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
             pp.visible(p, pseg, pu, pend);
             pu += warp;
         }
-        ppage = kv8_page(c, pp.seq, (pp.r.first_unit + pp.unit + pu) * kKv8Unit);
+        const int tok = pp.token(pu) + half * kKv8Unit;
+        ppage = tok < pp.r.len ? kv8_page(c, pp.seq, tok) : -1;
     };
     int pstage = 0;
-    auto produce = [&]() {          // one commit group, empty when there is nothing left
+    auto produce = [&]() {          // one commit group, empty when there is nothing left; lanes 0-15 fetch half 0, 16-31 half 1
         if (pmore) {
-            const int tok = (pp.r.first_unit + pp.unit + pu) * kKv8Unit;
-            float* sc = my_scales + pstage * 2;
-            if (tok < pp.r.len && ppage >= 0) {
+            const int tok = pp.token(pu) + half * kKv8Unit;
+            float* sc = my_scales + pstage * 4 + half * 2;
+            if (ppage >= 0) {
                 const int64_t row = kv8_row(c, ppage, pp.item / pp.r.row_tiles, kv8_in_page(c, tok));
-                const uint32_t dst = smem_u32(my_stages + pstage * Stage<D>::kBytes);
+                const uint32_t dst = smem_u32(my_stages + pstage * Stage<D>::kBytes + half * Stage<D>::kHalf);
 #pragma unroll
-                for (int i = 0; i < 2 * Stage<D>::kChunks / 32; ++i) {
-                    const int idx = i * 32 + lane, side = idx / Stage<D>::kChunks, k = idx % Stage<D>::kChunks;
-                    const int r = k / (D / 16), ch = k % (D / 16);
-                    cp_async16(dst + side * Stage<D>::kSide + Stage<D>::at(r, ch), c.codes[side] + row * D + k * 16);
+                for (int side = 0; side < 2; ++side) {
+                    const uint8_t* src = c.codes[side] + row * D + (lane & 15) * 16;
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        const int k = i * 16 + (lane & 15);
+                        cp_async16(dst + side * Stage<D>::kSide + Stage<D>::at(k / (D / 16), k % (D / 16)), src + i * 256);
+                    }
                 }
-                if (lane < 2) cp_async4(smem_u32(sc + lane), c.scales[lane] + kv8_scale_at(c, row));
+                if ((lane & 15) < 2) cp_async4(smem_u32(sc + (lane & 15)), ((lane & 15) == 0 ? c.scales[0] : c.scales[1]) + kv8_scale_at(c, row));
             } else {                // nothing to see: no row yet, or no page
-                if (lane < 2) sc[lane] = -1.f;
-                if (tok < pp.r.len && lane == 0) kv8_report(c, ER_ERR_OUT_OF_PAGES);
+                if ((lane & 15) < 2) sc[lane & 15] = -1.f;
+                if ((lane & 15) == 0 && tok < pp.r.len && tok + kKv8Unit > pp.lowest(p)) kv8_report(c, ER_ERR_OUT_OF_PAGES);
             }
             pu += kWarps;
             settle();
@@ -325,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
             }
         }
         float o[NT][MT][4], m[NT][2], l[NT][2], R = 0.f, inv_R = 0.f;
-        float keep[kSplit ? MT : 1][4];     // float32: the tensor cores' sums are moved here every 16 units (their accumulators round towards zero)
+        float keep[kSplit ? MT : 1][4];     // float32: the tensor cores' sums are moved here every 8 units (their accumulators round towards zero)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -342,57 +349,70 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
             __syncwarp();
             const uint8_t* ks = my_stages + cstage * Stage<D>::kBytes;
             const uint8_t* vs = ks + Stage<D>::kSide;
-            const float kscale = my_scales[cstage * 2];
-            float vscale = my_scales[cstage * 2 + 1];
-            const int tok0 = (at.r.first_unit + at.unit + u) * kKv8Unit;
-            // ---- scores: 16 tokens x 8 NT query rows ----
-            float s[NT][4], s2[NT][4];
+            const float4 sc4 = *reinterpret_cast<const float4*>(my_scales + cstage * 4);
+            const float kscale[2] = {sc4.x, sc4.z};
+            float vscale[2] = {sc4.y, sc4.w};
+            const int tok0 = at.token(u);
+            // ---- scores: 2 x 16 tokens x 8 NT query rows ----
+            float s[2][NT][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = s2[nt][0] = s2[nt][1] = s2[nt][2] = s2[nt][3] = 0.f;
+            for (int h = 0; h < 2; ++h) {
+                float s2[NT][4];
 #pragma unroll
-            for (int c16 = 0; c16 < kWords / 4; ++c16) {
-                const int ch = (kWords / 4) * t + c16;
-                const uint4 r0 = *reinterpret_cast<const uint4*>(ks + Stage<D>::at(g, ch));
-                const uint4 r1 = *reinterpret_cast<const uint4*>(ks + Stage<D>::at(g + 8, ch));
-                const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
+                for (int nt = 0; nt < NT; ++nt) s[h][nt][0] = s[h][nt][1] = s[h][nt][2] = s[h][nt][3] = s2[nt][0] = s2[nt][1] = s2[nt][2] = s2[nt][3] = 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int k = 4 * c16 + i;
-                    uint32_t a0, a1, a2, a3;
-                    decode4<E4M3>(w0[i], a0, a2);
-                    decode4<E4M3>(w1[i], a1, a3);
+                for (int c16 = 0; c16 < kWords / 4; ++c16) {
+                    const int ch = (kWords / 4) * t + c16;
+                    const uint4 r0 = *reinterpret_cast<const uint4*>(ks + h * Stage<D>::kHalf + Stage<D>::at(g, ch));
+                    const uint4 r1 = *reinterpret_cast<const uint4*>(ks + h * Stage<D>::kHalf + Stage<D>::at(g + 8, ch));
+                    const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        mma16816(i & 1 ? s2[nt] : s[nt], a0, a1, a2, a3, qh[nt][k][0], qh[nt][k][1]);
-                        if constexpr (kSplit) mma16816(i & 1 ? s2[nt] : s[nt], a0, a1, a2, a3, ql[nt][k][0], ql[nt][k][1]);
+                    for (int i = 0; i < 4; ++i) {
+                        const int k = 4 * c16 + i;
+                        uint32_t a0, a1, a2, a3;
+                        decode4<E4M3>(w0[i], a0, a2);
+                        decode4<E4M3>(w1[i], a1, a3);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma16816(i & 1 ? s2[nt] : s[h][nt], a0, a1, a2, a3, qh[nt][k][0], qh[nt][k][1]);
+                            if constexpr (kSplit) mma16816(i & 1 ? s2[nt] : s[h][nt], a0, a1, a2, a3, ql[nt][k][0], ql[nt][k][1]);
+                        }
                     }
                 }
-            }
-            // ---- online softmax; lane's scores: tokens g, g + 8 of the columns 2t, 2t + 1 ----
-            const bool hidden = kscale < 0.f;
-            const bool edge = hidden || tok0 + kKv8Unit - 1 > all_see_to || (p.window > 0 && tok0 < all_see_from);
-            bool rise = vscale > R;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[nt][e] = (s[nt][e] + s2[nt][e]) * (kscale * qscale[nt][e & 1]);
-                    if (edge) {
-                        const int tok = tok0 + g + 8 * (e >> 1), lim = limit[nt][e & 1];
-                        if (hidden || tok > lim || (p.window > 0 && tok <= lim - p.window)) s[nt][e] = -INFINITY;
-                    }
-                    rise |= s[nt][e] > m[nt][e & 1];
-                }
+                    for (int e = 0; e < 4; ++e) s[h][nt][e] = (s[h][nt][e] + s2[nt][e]) * (kscale[h] * qscale[nt][e & 1]);
             }
-            if (!(vscale >= 1.17549435e-38f)) vscale = isnan(vscale) ? vscale : 0.f;
+            // ---- online softmax; lane's scores: tokens g, g + 8 of each half, of the columns 2t, 2t + 1 ----
+            const bool edge = fminf(kscale[0], kscale[1]) < 0.f || tok0 + kUnit - 1 > all_see_to || (p.window > 0 && tok0 < all_see_from);
+            if (edge) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int tok = tok0 + h * kKv8Unit + g + 8 * (e >> 1), lim = limit[nt][e & 1];
+                            if (kscale[h] < 0.f || tok > lim || (p.window > 0 && tok <= lim - p.window)) s[h][nt][e] = -INFINITY;
+                        }
+            }
+            bool rise = fmaxf(vscale[0], vscale[1]) > R;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) rise |= fmaxf(fmaxf(s[0][nt][j], s[0][nt][2 + j]), fmaxf(s[1][nt][j], s[1][nt][2 + j])) > m[nt][j];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (!(vscale[h] >= 1.17549435e-38f)) vscale[h] = isnan(vscale[h]) ? vscale[h] : 0.f;
             if (__any_sync(0xffffffffu, rise)) {
-                const float R_new = fmaxf(R, vscale), down = R > 0.f ? R / R_new : 0.f;
+                const float R_new = fmaxf(R, fmaxf(vscale[0], vscale[1])), down = R > 0.f ? R / R_new : 0.f;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float corr[2];
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        float mx = fmaxf(m[nt][j], fmaxf(s[nt][j], s[nt][2 + j]));
+                        float mx = fmaxf(m[nt][j], fmaxf(fmaxf(s[0][nt][j], s[0][nt][2 + j]), fmaxf(s[1][nt][j], s[1][nt][2 + j])));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -413,64 +433,73 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
                 R = R_new;
                 inv_R = R > 0.f ? 1.f / R : 0.f;
             }
-            const float wf = vscale * inv_R * kWeightScale;
-            uint32_t wh[NT][2], wl[kSplit ? NT : 1][2];
+            uint32_t wh[2][NT][2], wl[2][kSplit ? NT : 1][2];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                float w[4];
+            for (int h = 0; h < 2; ++h) {
+                const float wf = vscale[h] * inv_R * kWeightScale;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float pr = s[nt][e] == -INFINITY ? 0.f : fast_exp2(s[nt][e] - m[nt][e & 1]);
-                    l[nt][e & 1] += pr;
-                    w[e] = s[nt][e] == -INFINITY ? 0.f : pr * wf;      // a hidden row of a block with a NaN scale weighs nothing
-                }
+                for (int nt = 0; nt < NT; ++nt) {
+                    float w[4];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if constexpr (kSplit) {
-                        uint32_t hi, lo;
-                        split_half2(w[2 * h], w[2 * h + 1], hi, lo);
-                        wh[nt][h] = transpose8x8(hi);
-                        wl[nt][h] = transpose8x8(lo);
-                    } else {
-                        wh[nt][h] = transpose8x8(half2_bits(w[2 * h], w[2 * h + 1]));
+                    for (int e = 0; e < 4; ++e) {
+                        const float pr = fast_exp2(s[h][nt][e] - (m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1]));
+                        l[nt][e & 1] += pr;
+                        w[e] = pr * wf;
+                        if (edge && s[h][nt][e] == -INFINITY) w[e] = 0.f;      // a hidden row of a block with a NaN scale weighs nothing
+                    }
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        if constexpr (kSplit) {
+                            uint32_t hi, lo;
+                            split_half2(w[2 * x], w[2 * x + 1], hi, lo);
+                            wh[h][nt][x] = transpose8x8(hi);
+                            wl[h][nt][x] = transpose8x8(lo);
+                        } else {
+                            wh[h][nt][x] = transpose8x8(half2_bits(w[2 * x], w[2 * x + 1]));
+                        }
                     }
                 }
             }
             // ---- outputs: D dims x 8 NT query rows, token pairs (2t, 2t + 1) and 8 further ----
-            {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
                 uint32_t v[4][kOwn / 4];
 #pragma unroll
                 for (int rr = 0; rr < 4; ++rr) {
                     const int row = 2 * t + (rr & 1) + 8 * (rr >> 1);
                     if constexpr (D == 128) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(vs + Stage<D>::at(row, g));
+                        const uint4 x = *reinterpret_cast<const uint4*>(vs + h * Stage<D>::kHalf + Stage<D>::at(row, g));
                         v[rr][0] = x.x; v[rr][1] = x.y; v[rr][2 % (kOwn / 4)] = x.z; v[rr][3 % (kOwn / 4)] = x.w;
                     } else {
-                        const uint2 x = *reinterpret_cast<const uint2*>(vs + Stage<D>::at(row, g >> 1) + (g & 1) * 8);
+                        const uint2 x = *reinterpret_cast<const uint2*>(vs + h * Stage<D>::kHalf + Stage<D>::at(row, g >> 1) + (g & 1) * 8);
                         v[rr][0] = x.x; v[rr][1] = x.y;
                     }
-                    if (edge && (hidden || tok0 + row >= at.r.len)) {   // bytes that are nobody's row may be codes of NaN
+                }
+                if (edge) {             // bytes that are nobody's row may be codes of NaN
 #pragma unroll
-                        for (int i = 0; i < kOwn / 4; ++i) v[rr][i] = 0u;
+                    for (int rr = 0; rr < 4; ++rr) {
+                        const bool nobody = kscale[h] < 0.f || tok0 + h * kKv8Unit + 2 * t + (rr & 1) + 8 * (rr >> 1) >= at.r.len;
+#pragma unroll
+                        for (int i = 0; i < kOwn / 4; ++i) v[rr][i] = nobody ? 0u : v[rr][i];
                     }
                 }
 #pragma unroll
                 for (int i = 0; i < kOwn / 4; ++i) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {      // dims 4 i + 2 h, 4 i + 2 h + 1 of the lane's own
+                    for (int x = 0; x < 2; ++x) {      // dims 4 i + 2 x, 4 i + 2 x + 1 of the lane's own
                         uint32_t a0, a1, a2, a3;
-                        decode4<E4M3>(__byte_perm(v[0][i], v[1][i], h ? 0x7362 : 0x5140), a0, a1);
-                        decode4<E4M3>(__byte_perm(v[2][i], v[3][i], h ? 0x7362 : 0x5140), a2, a3);
+                        decode4<E4M3>(__byte_perm(v[0][i], v[1][i], x ? 0x7362 : 0x5140), a0, a1);
+                        decode4<E4M3>(__byte_perm(v[2][i], v[3][i], x ? 0x7362 : 0x5140), a2, a3);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            mma16816(o[nt][2 * i + h], a0, a1, a2, a3, wh[nt][0], wh[nt][1]);
-                            if constexpr (kSplit) mma16816(o[nt][2 * i + h], a0, a1, a2, a3, wl[nt][0], wl[nt][1]);
+                            mma16816(o[nt][2 * i + x], a0, a1, a2, a3, wh[h][nt][0], wh[h][nt][1]);
+                            if constexpr (kSplit) mma16816(o[nt][2 * i + x], a0, a1, a2, a3, wl[h][nt][0], wl[h][nt][1]);
                         }
                     }
                 }
             }
             if constexpr (kSplit) {
-                if (++since == 16) {
+                if (++since == 8) {
                     since = 0;
 #pragma unroll
                     for (int i = 0; i < MT; ++i) {

@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                 if (valid > 0) {
                     x.kscale = __ldg(c.scales[0] + kv8_scale_at(c, row));
                     x.vscale = __ldg(c.scales[1] + kv8_scale_at(c, row));
-                } else if (q < total && tok < tile.len) {
+                } else if (q < total && tok < tile.len && tok + kKv8Unit > lo) {   // pages in front of the window may be gone
                     kv8_report(c, ER_ERR_OUT_OF_PAGES);
                 }
             }

@@ -360,6 +360,25 @@ def test_pages_that_are_missing_are_hidden(er, torch, fmt, t):
     check_attention(torch, cache.attention_prefill(q, ints(torch, [0, long]), table, ints(torch, [long])), want, big, t)
 
 
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_pages_in_front_of_the_window_may_be_gone(er, torch, t):
+    """A sliding window that begins in the second page of 16 rows of a larger unit of work: freed pages before it are no mistake."""
+    lens, window = [16 * 23 + 5, 700], 100
+    cache, table, rows = fill(er, torch, "e4m3", lens, 16, 2, 128, 16)
+    q = torch.randn(2 * 70, 4, 128, generator=gen(torch, 3), device="cuda").to(dtype(torch, t))
+    for n in (1, 70):
+        freed = table.clone()
+        for s in range(2):
+            freed[s, :(lens[s] - n - window + 1) // 16] = -1
+        mine = torch.cat([q[:n], q[70:70 + n]])
+        got = cache.attention_decode(mine, freed, ints(torch, lens), sliding_window=window) if n == 1 else cache.attention_prefill(
+            mine, ints(torch, [0, n, 2 * n]), freed, ints(torch, lens), sliding_window=window)
+        assert cache.device_status() == 0
+        for s in range(2):
+            want, big = ref_attention(torch, mine[s * n:(s + 1) * n], *rows[s], lens[s], 128 ** -0.5, window)
+            check_attention(torch, got[s * n:(s + 1) * n], want, big, t)
+
+
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
 def test_values_that_are_not_finite_reach_only_those_who_see_them(er, torch, t):
     """A NaN among the newest rows: earlier queries of the same call, and other sequences, stay finite; later ones are NaN."""
