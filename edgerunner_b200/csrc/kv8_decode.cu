@@ -24,7 +24,7 @@
 namespace er {
 namespace {
 
-constexpr int kWarps = 8, kThreads = kWarps * 32;
+constexpr int kMinUnits = 8;          // units of a CTA, so that short work stays together
 constexpr int kUnit = 2 * kKv8Unit;   // tokens that a warp takes at a time: two halves, each with a page and scales of its own
 constexpr float kWeightScale = 4096.f;
 
@@ -92,7 +92,7 @@ struct Place {        // a position in the list
     }
     __device__ __forceinline__ int token(int u) const { return (r.first_unit + unit + u) * kUnit; }   // of the u-th unit from here
 };
-// Total units, by every thread of the CTA (scratch: kWarps + 1 values).
+// Total units, by every thread of the CTA (scratch: a value a warp).
 __device__ int64_t total_units(const Kv8Decode& p, int64_t* scratch) {
     int64_t sum = 0;
     for (int s = threadIdx.x; s < p.cache.num_seqs; s += blockDim.x) {
@@ -142,8 +142,8 @@ __device__ Place find_place(const Kv8Decode& p, int64_t at, Place* shared_place)
     __syncthreads();
     return pl;
 }
-// CTA c of n takes the units [total c / n, total (c + 1) / n); at least kWarps units to a CTA, so that short work stays together.
-__device__ __forceinline__ int used_ctas(int64_t total, int ctas) { return static_cast<int>(min(static_cast<int64_t>(ctas), (total + kWarps - 1) / kWarps)); }
+// CTA c of n takes the units [total c / n, total (c + 1) / n).
+__device__ __forceinline__ int used_ctas(int64_t total, int ctas) { return static_cast<int>(min(static_cast<int64_t>(ctas), (total + kMinUnits - 1) / kMinUnits)); }
 __device__ __forceinline__ int64_t cta_begin(int64_t total, int n, int c) { return total * c / n; }
 __device__ __forceinline__ int cta_of(int64_t total, int n, int64_t unit) { return static_cast<int>(((unit + 1) * n - 1) / total); }
 
@@ -186,21 +186,27 @@ template <int D> struct Stage {
     }
 };
 template <int NT> __host__ __device__ constexpr int decode_rows() { return 8 * NT; }
-template <int D, int NT> __host__ __device__ constexpr int decode_stages() {
-    return D == 128 ? (NT == 1 ? 3 : 2) : (NT == 1 ? 6 : 5);
+// Warps of a CTA.  A unit costs a warp about 570 instructions, most of them in chains: with two warps to a scheduler it waits for itself a
+// quarter of the time.  Three fit where 168 registers do: one column tile of 16-bit rows (64 ragged sequences: 237 -> WWW us).
+template <typename T, int NT> __host__ __device__ constexpr int decode_warps() { return sizeof(T) == 2 && NT == 1 ? 12 : 8; }
+// Warps that meet in shared memory at the end of an item; those beyond hand theirs to a partner first.
+template <typename T, int NT> __host__ __device__ constexpr int join_warps() { return decode_warps<T, NT>() == 12 ? 6 : 8; }
+template <typename T, int D, int NT> __host__ __device__ constexpr int decode_stages() {
+    constexpr int n = decode_warps<T, NT>() == 12 ? 2 : NT == 1 ? 3 : 2;
+    return D == 128 ? n : 2 * n;
 }
-template <int D, int NT> __host__ __device__ constexpr int join_floats() { return kWarps * 8 * NT * (D + 4); }
-template <int D, int NT> __host__ __device__ constexpr int decode_smem() {
-    return kWarps * decode_stages<D, NT>() * (Stage<D>::kBytes + 16) + (join_floats<D, NT>() + kWarps * 8 * NT * 2) * 4 + 128;
+template <typename T, int D, int NT> __host__ __device__ constexpr int join_floats() { return join_warps<T, NT>() * 8 * NT * (D + 4); }
+template <typename T, int D, int NT> __host__ __device__ constexpr int decode_smem() {
+    return decode_warps<T, NT>() * decode_stages<T, D, NT>() * (Stage<D>::kBytes + 16) + (join_floats<T, D, NT>() + join_warps<T, NT>() * 8 * NT * 2) * 4 + 128;
 }
 // One partial: max, sum, -, - and the unnormalised row.
 template <int D> __host__ __device__ constexpr int partial_stride() { return D + 4; }
 
 template <typename T, int D, bool E4M3, int NT>
-__global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_constant__ Kv8Decode p) {
+__global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kernel(const __grid_constant__ Kv8Decode p) {
     constexpr bool kSplit = sizeof(T) == 4;      // float32: queries and weights as a high and a low half
     static_assert(!kSplit || NT == 1, "");
-    constexpr int kRows = decode_rows<NT>(), kStages = decode_stages<D, NT>();
+    constexpr int kRows = decode_rows<NT>(), kStages = decode_stages<T, D, NT>(), kWarps = decode_warps<T, NT>(), kThreads = kWarps * 32, kJoin = join_warps<T, NT>();
     constexpr int KK = D / 16, MT = D / 16, kWords = D / 16;   // k-steps of the scores; m-tiles of the outputs; 4-byte words of a lane's part of a key row
     constexpr int kOwn = D / 8;                                 // dims of a lane g in the outputs
     constexpr int kJoinRow = D + 4;
@@ -208,8 +214,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
     uint8_t* stages = smem;
     float* stage_scales = reinterpret_cast<float*>(smem + kWarps * kStages * Stage<D>::kBytes);
     float* join = stage_scales + kWarps * kStages * 4;
-    float* join_ml = join + join_floats<D, NT>();
-    int64_t* scratch = reinterpret_cast<int64_t*>(join_ml + kWarps * kRows * 2);
+    float* join_ml = join + join_floats<T, D, NT>();
+    int64_t* scratch = reinterpret_cast<int64_t*>(join_ml + kJoin * kRows * 2);
     const Kv8Cache& c = p.cache;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, half = lane >> 4;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -346,7 +352,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
 
         for (int u = u0 + warp; u < u1; u += kWarps) {
             cp_async_wait<kStages - 2>();
-            __syncwarp();
+            __syncwarp();           // the unit is here for every lane, and every lane has read the one before, whose stage is filled next
+            produce();
             const uint8_t* ks = my_stages + cstage * Stage<D>::kBytes;
             const uint8_t* vs = ks + Stage<D>::kSide;
             const float4 sc4 = *reinterpret_cast<const float4*>(my_scales + cstage * 4);
@@ -508,9 +515,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
                     }
                 }
             }
-            __syncwarp();           // every lane has read the stage before it is filled again
             cstage = cstage + 1 == kStages ? 0 : cstage + 1;
-            produce();
         }
 
         // ---- join the warps of the CTA ----
@@ -519,24 +524,59 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                float x = l[nt][j];
-                x += __shfl_xor_sync(0xffffffffu, x, 4);
-                x += __shfl_xor_sync(0xffffffffu, x, 8);
-                x += __shfl_xor_sync(0xffffffffu, x, 16);
-                const int col = nt * 8 + 2 * t + j;
-                if (g == 0) {
-                    join_ml[(warp * kRows + col) * 2] = m[nt][j];
-                    join_ml[(warp * kRows + col) * 2 + 1] = x;
-                }
-                float* row = join + (warp * kRows + col) * kJoinRow + 2 * g;   // dim kOwn g + 2 i + e at 16 i + 2 g + e
+                l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 4);
+                l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 8);
+                l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 16);
+            }
 #pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    float a = o[nt][i][j], b = o[nt][i][2 + j];
-                    if constexpr (kSplit) { a += keep[i][j]; b += keep[i][2 + j]; }
-                    *reinterpret_cast<float2*>(row + 16 * i) = make_float2(a * out_scale, b * out_scale);
+            for (int i = 0; i < MT; ++i) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (kSplit) o[nt][i][e] += keep[i][e];
+                    o[nt][i][e] *= out_scale;
                 }
             }
         }
+        auto leave = [&](int slot) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int col = nt * 8 + 2 * t + j;
+                    if (g == 0) *reinterpret_cast<float2*>(join_ml + (slot * kRows + col) * 2) = make_float2(m[nt][j], l[nt][j]);
+                    float* row = join + (slot * kRows + col) * kJoinRow + 2 * g;   // dim kOwn g + 2 i + e at 16 i + 2 g + e
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) *reinterpret_cast<float2*>(row + 16 * i) = make_float2(o[nt][i][j], o[nt][i][2 + j]);
+                }
+            }
+        };
+        if constexpr (kWarps > kJoin) {
+            if (warp >= kJoin) leave(warp - kJoin);
+            __syncthreads();
+            if (warp < kJoin) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int col = nt * 8 + 2 * t + j;
+                        const float2 ml = *reinterpret_cast<const float2*>(join_ml + (warp * kRows + col) * 2);
+                        const float M = fmaxf(m[nt][j], ml.x), M0 = M == -INFINITY ? 0.f : M;
+                        const float mine = fast_exp2(m[nt][j] - M0), other = fast_exp2(ml.x - M0);
+                        m[nt][j] = M;
+                        l[nt][j] = l[nt][j] * mine + ml.y * other;
+                        const float* row = join + (warp * kRows + col) * kJoinRow + 2 * g;
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) {
+                            const float2 v = *reinterpret_cast<const float2*>(row + 16 * i);
+                            o[nt][i][j] = o[nt][i][j] * mine + v.x * other;
+                            o[nt][i][2 + j] = o[nt][i][2 + j] * mine + v.y * other;
+                        }
+                    }
+                }
+            }
+            __syncwarp();            // the slot is read by the warp that fills it next
+        }
+        if (warp < kJoin) leave(warp);
         __syncthreads();
         const bool whole = at.unit == 0 && seg == at.r.units;
         const int cols = min(kRows, rows - rt * kRows);
@@ -544,12 +584,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
             const int col = e / (D / 2), d = (e % (D / 2)) * 2;
             float M = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, join_ml[(w * kRows + col) * 2]);
+            for (int w = 0; w < kJoin; ++w) M = fmaxf(M, join_ml[(w * kRows + col) * 2]);
             const float M0 = M == -INFINITY ? 0.f : M;
             float L = 0.f, x = 0.f, y = 0.f;
             const int pos = 16 * ((d % kOwn) / 2) + 2 * (d / kOwn);
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
+            for (int w = 0; w < kJoin; ++w) {
                 const float f = fast_exp2(join_ml[(w * kRows + col) * 2] - M0);
                 const float2 v = *reinterpret_cast<const float2*>(join + (w * kRows + col) * kJoinRow + pos);
                 L = fmaf(f, join_ml[(w * kRows + col) * 2 + 1], L);
@@ -579,9 +619,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
 
 // Joins the partials of the items that more than one CTA worked on.  At most one item begins in a CTA's range and goes on behind it: block
 // (c, row) looks for that of CTA c and, if there is one, joins query row `row` of it: its warps take the parts in turn, a lane D / 32 dims.
+constexpr int kJoinThreads = 256;
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads) kv8_decode_join_kernel(const __grid_constant__ Kv8Decode p) {
-    constexpr int kRows = decode_rows<NT>(), V = D / 32;
+__global__ void __launch_bounds__(kJoinThreads) kv8_decode_join_kernel(const __grid_constant__ Kv8Decode p) {
+    constexpr int kWarps = kJoinThreads / 32, kRows = decode_rows<NT>(), V = D / 32;
     __shared__ int64_t scratch[16];
     __shared__ float ml[kWarps][2], rows[kWarps][D];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.y;
@@ -646,17 +687,17 @@ int tiles_of(uint32_t type, int rows) { return type != ER_TYPE_FLOAT32 && rows >
 
 template <typename T, int D, bool E4M3, int NT>
 int32_t launch(Kv8Decode& p, int most_rows, int sms, cudaStream_t s) {
-    constexpr int kSmem = decode_smem<D, NT>();
+    constexpr int kSmem = decode_smem<T, D, NT>();
     static_assert(kSmem <= 232448, "decode kernel exceeds the shared memory of an sm_100 CTA");
     p.tile_rows = 8 * NT;
     cudaError_t e = cudaFuncSetAttribute(kv8_decode_kernel<T, D, E4M3, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return kv8_launched(e, "kv8_decode_kernel");
-    kv8_decode_kernel<T, D, E4M3, NT><<<sms, kThreads, kSmem, s>>>(p);
+    kv8_decode_kernel<T, D, E4M3, NT><<<sms, decode_warps<T, NT>() * 32, kSmem, s>>>(p);
     const int32_t rc = kv8_launched(cudaGetLastError(), "kv8_decode_kernel");
     if (rc != ER_OK) return rc;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(sms, p.starts != nullptr ? 8 * NT : std::min(8 * NT, most_rows));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
