@@ -48,6 +48,8 @@ int32_t kv8_check(const er_kv8_cache* c, Kv8Cache* out) {
     if (c->block_table_width > c->block_table_stride) return report_error(ER_ERR_SHAPE, "block_table_width exceeds block_table_stride");
     if (static_cast<uint64_t>(c->block_table_width) * c->page_size > 0x7FFFFF00ull)
         return report_error(ER_ERR_UNSUPPORTED, "block tables address more than 2^31 rows of a sequence");
+    if (static_cast<uint64_t>(c->num_pages) * c->num_kv_heads * c->page_size > 0x7FFFFFFFull)
+        return report_error(ER_ERR_UNSUPPORTED, "the cache has more than 2^31 rows (pages * kv heads * page_size)");
     if (!kv8_aligned(c->keys) || !kv8_aligned(c->values)) return report_error(ER_ERR_INVALID_ARGUMENT, "keys and values must be 16-byte aligned");
     out->codes[0] = c->keys; out->codes[1] = c->values;
     out->scales[0] = c->key_scales; out->scales[1] = c->value_scales;

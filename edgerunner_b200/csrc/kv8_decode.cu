@@ -8,8 +8,7 @@
 //
 // Work.  Bound by memory: 2 D bytes a row for 4 D flops a query head.  A persistent CTA per SM; the list of 32-token units of all (sequence, kv head,
 // row tile) items is cut evenly over the CTAs whatever the lengths are, inside a CTA the units of an item go round robin to the warps.  A warp
-// streams its units through its own ring of shared-memory stages with cp.async (16 bytes a lane, no barrier between warps, several units in
-// flight: 160 to 190 KB a SM), and runs both products of a unit alone: scores as S^T = K q^T (2 x 16 tokens x 8 query rows), outputs as O^T = V^T w^T
+// streams its units through its own ring of shared-memory stages with TMA (boxes of 16 rows; no barrier between warps, 96 to 130 KB in flight a SM), and runs both products of a unit alone: scores as S^T = K q^T (2 x 16 tokens x 8 query rows), outputs as O^T = V^T w^T
 // (16 dims x 8 query rows), so eight query rows fill a tile and K is an A operand as it lies in memory.  The warps of a CTA are joined in shared
 // memory at the end of an item, the CTAs that share an item by a second small launch that overlaps this one's tail.
 //
@@ -20,6 +19,7 @@
 #include <cmath>
 
 #include "kv8.cuh"
+#include "tmap.h"
 
 namespace er {
 namespace {
@@ -29,6 +29,7 @@ constexpr int kUnit = 2 * kKv8Unit;   // tokens that a warp takes at a time: two
 constexpr float kWeightScale = 4096.f;
 
 struct Kv8Decode {
+    CUtensorMap maps[2];            // codes of the keys, values as [rows][head_dim], boxes of 16 rows
     Kv8Cache cache;
     const void* q;
     void* out;
@@ -148,8 +149,10 @@ __device__ __forceinline__ int64_t cta_begin(int64_t total, int n, int c) { retu
 __device__ __forceinline__ int cta_of(int64_t total, int n, int64_t unit) { return static_cast<int>(((unit + 1) * n - 1) / total); }
 
 // ---- instructions ----
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, int row, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(0), "r"(row),
+                 "r"(smem_u32(bar))
+                 : "memory");
 }
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
@@ -179,10 +182,10 @@ __device__ __forceinline__ void split_half2(float a, float b, uint32_t& hi, uint
 // A stage: keys of the two halves, values of the two halves.
 template <int D> struct Stage {
     static constexpr int kHalf = kKv8Unit * D, kSide = 2 * kHalf, kBytes = 2 * kSide;
-    // byte offset of 16-byte chunk c of row r inside a half
+    // byte offset of 16-byte chunk c of row r inside a half: the 128-byte (64-byte) swizzle of the tensor map
     static __device__ __forceinline__ int at(int r, int c) {
         if constexpr (D == 128) return r * 128 + ((c ^ (r & 7)) << 4);
-        else return (r >> 1) * 128 + (((((r & 1) << 2) | c) ^ ((r >> 1 & 3) << 1)) << 4);
+        else return r * 64 + ((c ^ (r >> 1 & 3)) << 4);
     }
 };
 template <int NT> __host__ __device__ constexpr int decode_rows() { return 8 * NT; }
@@ -190,17 +193,34 @@ template <int NT> __host__ __device__ constexpr int decode_rows() { return 8 * N
 // quarter of the time.  Three fit where 168 registers do: one column tile of 16-bit rows (64 ragged sequences: 237 -> WWW us).
 template <typename T, int NT> __host__ __device__ constexpr int decode_warps() { return sizeof(T) == 2 && NT == 1 ? 12 : 8; }
 // Warps that meet in shared memory at the end of an item; those beyond hand theirs to a partner first.
-template <typename T, int NT> __host__ __device__ constexpr int join_warps() { return decode_warps<T, NT>() == 12 ? 6 : 8; }
+template <typename T, int NT> __host__ __device__ constexpr int join_warps() { return decode_warps<T, NT>() / 2; }
 template <typename T, int D, int NT> __host__ __device__ constexpr int decode_stages() {
     constexpr int n = decode_warps<T, NT>() == 12 ? 2 : NT == 1 ? 3 : 2;
     return D == 128 ? n : 2 * n;
 }
 template <typename T, int D, int NT> __host__ __device__ constexpr int join_floats() { return join_warps<T, NT>() * 8 * NT * (D + 4); }
 template <typename T, int D, int NT> __host__ __device__ constexpr int decode_smem() {
-    return decode_warps<T, NT>() * decode_stages<T, D, NT>() * (Stage<D>::kBytes + 16) + (join_floats<T, D, NT>() + join_warps<T, NT>() * 8 * NT * 2) * 4 + 128;
+    return decode_warps<T, NT>() * decode_stages<T, D, NT>() * (Stage<D>::kBytes + 16 + 8) + (join_floats<T, D, NT>() + join_warps<T, NT>() * 8 * NT * 2) * 4 + 128 + 1024;
 }
 // One partial: max, sum, -, - and the unnormalised row.
 template <int D> __host__ __device__ constexpr int partial_stride() { return D + 4; }
+
+// A wait of at most 2 s: then the status word is set, later waits are skipped and the kernel runs to its end.
+__device__ __forceinline__ void bounded_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, const Kv8Cache& c) {
+    if (mbar_try_wait(bar, parity) || *abort_flag) return;
+    const uint64_t start = global_timer_ns();
+    uint32_t spins = 0;
+    while (!mbar_try_wait(bar, parity)) {
+        if ((++spins & 0x3FFu) == 0u) {
+            if (*abort_flag) return;
+            if (global_timer_ns() - start > 2000000000ull) {
+                *abort_flag = 1;
+                kv8_report(c, ER_ERR_DEVICE_TIMEOUT);
+                return;
+            }
+        }
+    }
+}
 
 template <typename T, int D, bool E4M3, int NT>
 __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kernel(const __grid_constant__ Kv8Decode p) {
@@ -210,15 +230,22 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
     constexpr int KK = D / 16, MT = D / 16, kWords = D / 16;   // k-steps of the scores; m-tiles of the outputs; 4-byte words of a lane's part of a key row
     constexpr int kOwn = D / 8;                                 // dims of a lane g in the outputs
     constexpr int kJoinRow = D + 4;
-    extern __shared__ __align__(16) uint8_t smem[];
-    uint8_t* stages = smem;
-    float* stage_scales = reinterpret_cast<float*>(smem + kWarps * kStages * Stage<D>::kBytes);
+    extern __shared__ uint8_t raw[];
+    uint8_t* stages = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);     // the swizzle goes by the address
+    float* stage_scales = reinterpret_cast<float*>(stages + kWarps * kStages * Stage<D>::kBytes);
     float* join = stage_scales + kWarps * kStages * 4;
     float* join_ml = join + join_floats<T, D, NT>();
-    int64_t* scratch = reinterpret_cast<int64_t*>(join_ml + kJoin * kRows * 2);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(join_ml + kJoin * kRows * 2);
+    int64_t* scratch = reinterpret_cast<int64_t*>(bars + kWarps * kStages);   // 96 bytes
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(scratch + 14);
     const Kv8Cache& c = p.cache;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, half = lane >> 4;
+    const int odd = D == 64 ? t & 1 : 0;
+    const uint32_t pairs_lo = odd ? 0x1504u : 0x5140u, pairs_hi = odd ? 0x3726u : 0x7362u;   // bytes 0, 1 (2, 3) of a row pair, the lower row first
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (threadIdx.x < kWarps * kStages) mbar_init(bars + threadIdx.x, 2);    // a lane of each half arrives with the bytes of its copies
+    if (threadIdx.x == 0) *abort_flag = 0;
+    mbar_init_fence();
 
     const int64_t total = total_units(p, scratch);
     const int n = used_ctas(total, gridDim.x), cta = blockIdx.x;
@@ -235,6 +262,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
 
     // ---- producer: this warp's units, kStages - 1 ahead ----
     uint8_t* my_stages = stages + warp * kStages * Stage<D>::kBytes;
+    uint64_t* my_bars = bars + warp * kStages;
     float* my_scales = stage_scales + warp * kStages * 4;   // per stage: key and value scale of half 0, of half 1
     Place pp = at;                  // segment the producer is in
     int64_t pleft = left;           // units from pp.unit on
@@ -257,26 +285,24 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
         ppage = tok < pp.r.len ? kv8_page(c, pp.seq, tok) : -1;
     };
     int pstage = 0;
-    auto produce = [&]() {          // one commit group, empty when there is nothing left; lanes 0-15 fetch half 0, 16-31 half 1
+    auto produce = [&]() {          // the next unit, if there is one: lanes 0-15 see to half 0, 16-31 to half 1
         if (pmore) {
             const int tok = pp.token(pu) + half * kKv8Unit;
             float* sc = my_scales + pstage * 4 + half * 2;
-            if (ppage >= 0) {
-                const int64_t row = kv8_row(c, ppage, pp.item / pp.r.row_tiles, kv8_in_page(c, tok));
-                const uint32_t dst = smem_u32(my_stages + pstage * Stage<D>::kBytes + half * Stage<D>::kHalf);
-#pragma unroll
-                for (int side = 0; side < 2; ++side) {
-                    const uint8_t* src = c.codes[side] + row * D + (lane & 15) * 16;
-#pragma unroll
-                    for (int i = 0; i < D / 16; ++i) {
-                        const int k = i * 16 + (lane & 15);
-                        cp_async16(dst + side * Stage<D>::kSide + Stage<D>::at(k / (D / 16), k % (D / 16)), src + i * 256);
-                    }
+            const int64_t row = kv8_row(c, max(ppage, 0), pp.item / pp.r.row_tiles, kv8_in_page(c, tok));
+            if ((lane & 15) == 0) {
+                mbar_arrive_expect_tx(my_bars + pstage, ppage >= 0 ? 2 * Stage<D>::kHalf : 0);
+                if (ppage >= 0) {
+                    const uint32_t dst = smem_u32(my_stages + pstage * Stage<D>::kBytes + half * Stage<D>::kHalf);
+                    tma_rows(dst, &p.maps[0], static_cast<int>(row), my_bars + pstage);
+                    tma_rows(dst + Stage<D>::kSide, &p.maps[1], static_cast<int>(row), my_bars + pstage);
+                } else if (tok < pp.r.len && tok + kKv8Unit > pp.lowest(p)) {
+                    kv8_report(c, ER_ERR_OUT_OF_PAGES);
                 }
-                if ((lane & 15) < 2) cp_async4(smem_u32(sc + (lane & 15)), ((lane & 15) == 0 ? c.scales[0] : c.scales[1]) + kv8_scale_at(c, row));
-            } else {                // nothing to see: no row yet, or no page
-                if ((lane & 15) < 2) sc[lane & 15] = -1.f;
-                if ((lane & 15) == 0 && tok < pp.r.len && tok + kKv8Unit > pp.lowest(p)) kv8_report(c, ER_ERR_OUT_OF_PAGES);
+            }
+            if ((lane & 15) < 2) {
+                if (ppage >= 0) cp_async4(smem_u32(sc + (lane & 15)), ((lane & 15) == 0 ? c.scales[0] : c.scales[1]) + kv8_scale_at(c, row));
+                else sc[lane & 15] = -1.f;      // nothing to see: no row yet, or no page
             }
             pu += kWarps;
             settle();
@@ -288,7 +314,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) produce();
 
-    int cstage = 0;
+    int cstage = 0, cphase = 0;
     bool first_segment = true;
     while (left > 0) {
         const int seg = static_cast<int>(min(static_cast<int64_t>(at.r.units - at.unit), left));
@@ -352,6 +378,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
 
         for (int u = u0 + warp; u < u1; u += kWarps) {
             cp_async_wait<kStages - 2>();
+            bounded_wait(my_bars + cstage, cphase, abort_flag, c);
             __syncwarp();           // the unit is here for every lane, and every lane has read the one before, whose stage is filled next
             produce();
             const uint8_t* ks = my_stages + cstage * Stage<D>::kBytes;
@@ -473,7 +500,8 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
                 uint32_t v[4][kOwn / 4];
 #pragma unroll
                 for (int rr = 0; rr < 4; ++rr) {
-                    const int row = 2 * t + (rr & 1) + 8 * (rr >> 1);
+                    // D = 64: two rows share 128 bytes, so every other lane takes its pair of rows the other way round
+                    const int row = 2 * t + ((rr ^ odd) & 1) + 8 * (rr >> 1);
                     if constexpr (D == 128) {
                         const uint4 x = *reinterpret_cast<const uint4*>(vs + h * Stage<D>::kHalf + Stage<D>::at(row, g));
                         v[rr][0] = x.x; v[rr][1] = x.y; v[rr][2 % (kOwn / 4)] = x.z; v[rr][3 % (kOwn / 4)] = x.w;
@@ -485,7 +513,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
                 if (edge) {             // bytes that are nobody's row may be codes of NaN
 #pragma unroll
                     for (int rr = 0; rr < 4; ++rr) {
-                        const bool nobody = kscale[h] < 0.f || tok0 + h * kKv8Unit + 2 * t + (rr & 1) + 8 * (rr >> 1) >= at.r.len;
+                        const bool nobody = kscale[h] < 0.f || tok0 + h * kKv8Unit + 2 * t + ((rr ^ odd) & 1) + 8 * (rr >> 1) >= at.r.len;
 #pragma unroll
                         for (int i = 0; i < kOwn / 4; ++i) v[rr][i] = nobody ? 0u : v[rr][i];
                     }
@@ -495,8 +523,8 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {      // dims 4 i + 2 x, 4 i + 2 x + 1 of the lane's own
                         uint32_t a0, a1, a2, a3;
-                        decode4<E4M3>(__byte_perm(v[0][i], v[1][i], x ? 0x7362 : 0x5140), a0, a1);
-                        decode4<E4M3>(__byte_perm(v[2][i], v[3][i], x ? 0x7362 : 0x5140), a2, a3);
+                        decode4<E4M3>(__byte_perm(v[0][i], v[1][i], x ? pairs_hi : pairs_lo), a0, a1);
+                        decode4<E4M3>(__byte_perm(v[2][i], v[3][i], x ? pairs_hi : pairs_lo), a2, a3);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             mma16816(o[nt][2 * i + x], a0, a1, a2, a3, wh[h][nt][0], wh[h][nt][1]);
@@ -516,6 +544,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
                 }
             }
             cstage = cstage + 1 == kStages ? 0 : cstage + 1;
+            cphase ^= cstage == 0 ? 1 : 0;
         }
 
         // ---- join the warps of the CTA ----
@@ -550,33 +579,31 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
                 }
             }
         };
-        if constexpr (kWarps > kJoin) {
-            if (warp >= kJoin) leave(warp - kJoin);
-            __syncthreads();
-            if (warp < kJoin) {
+        if (warp >= kJoin) leave(warp - kJoin);
+        __syncthreads();
+        if (warp < kJoin) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
+            for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const int col = nt * 8 + 2 * t + j;
-                        const float2 ml = *reinterpret_cast<const float2*>(join_ml + (warp * kRows + col) * 2);
-                        const float M = fmaxf(m[nt][j], ml.x), M0 = M == -INFINITY ? 0.f : M;
-                        const float mine = fast_exp2(m[nt][j] - M0), other = fast_exp2(ml.x - M0);
-                        m[nt][j] = M;
-                        l[nt][j] = l[nt][j] * mine + ml.y * other;
-                        const float* row = join + (warp * kRows + col) * kJoinRow + 2 * g;
+                for (int j = 0; j < 2; ++j) {
+                    const int col = nt * 8 + 2 * t + j;
+                    const float2 ml = *reinterpret_cast<const float2*>(join_ml + (warp * kRows + col) * 2);
+                    const float M = fmaxf(m[nt][j], ml.x), M0 = M == -INFINITY ? 0.f : M;
+                    const float mine = fast_exp2(m[nt][j] - M0), other = fast_exp2(ml.x - M0);
+                    m[nt][j] = M;
+                    l[nt][j] = l[nt][j] * mine + ml.y * other;
+                    const float* row = join + (warp * kRows + col) * kJoinRow + 2 * g;
 #pragma unroll
-                        for (int i = 0; i < MT; ++i) {
-                            const float2 v = *reinterpret_cast<const float2*>(row + 16 * i);
-                            o[nt][i][j] = o[nt][i][j] * mine + v.x * other;
-                            o[nt][i][2 + j] = o[nt][i][2 + j] * mine + v.y * other;
-                        }
+                    for (int i = 0; i < MT; ++i) {
+                        const float2 v = *reinterpret_cast<const float2*>(row + 16 * i);
+                        o[nt][i][j] = o[nt][i][j] * mine + v.x * other;
+                        o[nt][i][2 + j] = o[nt][i][2 + j] * mine + v.y * other;
                     }
                 }
             }
-            __syncwarp();            // the slot is read by the warp that fills it next
+            __syncwarp();            // the slot has been read before it is filled again
+            leave(warp);
         }
-        if (warp < kJoin) leave(warp);
         __syncthreads();
         const bool whole = at.unit == 0 && seg == at.r.units;
         const int cols = min(kRows, rows - rt * kRows);
@@ -685,6 +712,17 @@ namespace {
 // Two columns of eight query rows where they are needed and fit: float32 rows take two operands each and stay at eight.
 int tiles_of(uint32_t type, int rows) { return type != ER_TYPE_FLOAT32 && rows > 8 ? 2 : 1; }
 
+// Codes as a 2-D tensor of bytes, swizzled as the kernel reads them: rows of 128 (64) bytes, 16-byte chunk c of row r at c ^ (r % 8) (c ^ (r / 2 % 4)).
+bool encode_rows(CUtensorMap* map, const uint8_t* codes, const Kv8Cache& c, int head_dim) {
+    const EncodeTiledFn fn = tensor_map_encode_entry();
+    if (fn == nullptr) return false;
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(c.num_pages) * c.num_kv_heads * c.page_size};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(head_dim)};
+    const cuuint32_t box[2] = {static_cast<cuuint32_t>(head_dim), kKv8Unit}, one[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(codes), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int D, bool E4M3, int NT>
 int32_t launch(Kv8Decode& p, int most_rows, int sms, cudaStream_t s) {
     constexpr int kSmem = decode_smem<T, D, NT>();
@@ -773,6 +811,8 @@ int32_t kv8_launch_decode(const Kv8Cache& cache, const er_kv8_cache* c, const er
     p.few_rows = few_rows;
     p.group = static_cast<int>(u->num_heads) / cache.num_kv_heads;
     p.query_len = static_cast<int>(u->query_len); p.window = static_cast<int>(u->sliding_window);
+    if (!encode_rows(&p.maps[0], cache.codes[0], cache, static_cast<int>(c->head_dim)) || !encode_rows(&p.maps[1], cache.codes[1], cache, static_cast<int>(c->head_dim)))
+        return report_error(ER_ERR_CUDA, "cuTensorMapEncodeTiled refused the cache's shape");
     p.scale_log2 = kv8_scale_log2(u->softmax_scale, c->head_dim);
     const int sms = kv8_sm_count(), d = static_cast<int>(c->head_dim);
     switch (u->type) {
