@@ -145,12 +145,12 @@ SYMBOLS = {
     "er_kv_page_bytes": (C.c_int64, [_vp]),
     "er_kv_export_pages": (_i32, [_vp, _vp, _u32, _vp, _sz, _vp]),
     "er_kv_import_pages": (_i32, [_vp, _vp, _u32, _vp, _sz, _vp]),
-    "er_qk_norm_rope": (_i32, [C.POINTER(er_qk_norm_rope_params), _vp]),
-    "er_kv8_append": (_i32, [C.POINTER(er_kv8_cache), C.POINTER(er_kv8_append_params), _vp]),
-    "er_kv8_decode_workspace_bytes": (C.c_int64, [C.POINTER(er_kv8_cache), C.POINTER(er_kv8_attention_params)]),
-    "er_kv8_attention_decode": (_i32, [C.POINTER(er_kv8_cache), C.POINTER(er_kv8_attention_params), _vp]),
-    "er_kv8_prefill_workspace_bytes": (C.c_int64, [C.POINTER(er_kv8_cache), C.POINTER(er_kv8_attention_params)]),
-    "er_kv8_attention_prefill": (_i32, [C.POINTER(er_kv8_cache), C.POINTER(er_kv8_attention_params), _vp]),
+    "er_qk_norm_rope": (_i32, [_vp, _vp]),
+    "er_kv8_append": (_i32, [_vp, _vp, _vp]),
+    "er_kv8_decode_workspace_bytes": (C.c_int64, [_vp, _vp]),
+    "er_kv8_attention_decode": (_i32, [_vp, _vp, _vp]),
+    "er_kv8_prefill_workspace_bytes": (C.c_int64, [_vp, _vp]),
+    "er_kv8_attention_prefill": (_i32, [_vp, _vp, _vp]),
     "er_host_alloc": (_i32, [C.POINTER(_vp), _sz]),
     "er_host_free": (_i32, [_vp]),
 }

@@ -9,62 +9,77 @@ torch stream of the tensors' device; nothing waits, and every call may be captur
     cache.append(k, v, block_tables, kv_lens, query_starts, k_norm_weight=kw, rope_theta=theta)
     out = cache.attention_prefill(q, query_starts, block_tables, kv_lens)                 # or attention_decode for single tokens
 """
-import ctypes as C
 import enum
+import struct
 
-from ._lib import (check, er_kv8_append_params, er_kv8_attention_params, er_kv8_cache, er_qk_norm_rope_params, lib, stream_ptr)
+from ._lib import check, lib, stream_ptr
+
+# The parameter structures of include/er_kv.h as packed bytes: one call instead of some thirty attribute writes, which cost more than a
+# small kernel runs for.  Field order as in the header (tests compare the sizes with the compiler's).
+_NORM_ROPE = struct.Struct("@4P8q3P5I4f4x")
+_CACHE = struct.Struct("@7P9I4x")
+_APPEND = struct.Struct("@2P4q2P2I4f")
+_ATTENTION = struct.Struct("@2P4qP5IfIPQ")
 
 _TYPE = {}
+_torch = None    # imported with the first tensor, like everywhere in this package
 
 
 def _types():
-    if not _TYPE:
+    global _torch
+    if _torch is None:
         import torch
         _TYPE.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+        _torch = torch
     return _TYPE
 
 
-def _stream(stream, device):
-    if stream is not None:
-        return stream_ptr(stream)
-    import torch
-    return torch.cuda.current_stream(device).cuda_stream
+def _stream(stream, index):
+    return _torch.cuda.current_stream(index).cuda_stream if stream is None else stream_ptr(stream)
 
 
-def _call(fn, device, *args):
+def _call(fn, index, *args):
     """fn(*args) with the tensors' device current (the C ABI wants it to be)."""
-    import torch
-    if torch.cuda.current_device() != device.index:
-        with torch.cuda.device(device):
+    if _torch.cuda.current_device() != index:
+        with _torch.cuda.device(index):
             return check(fn(*args))
-    return check(fn(*args))
+    rc = fn(*args)
+    return rc if rc >= 0 else check(rc)
 
 
-def _rows(x, name, device=None, dtype=None, dim=None):
-    if x.dim() != 3 or x.stride(2) != 1:
+def _rows(x, name, index=None, dtype=None, dim=None):
+    """(address, token stride, head stride, tokens, heads) of [tokens, heads, head_dim] rows."""
+    shape, stride = x.shape, x.stride()
+    if len(shape) != 3 or (stride[2] != 1 and shape[2] != 1):
         raise ValueError("%s must be [tokens, heads, head_dim] with a contiguous last dimension" % name)
-    if x.dtype not in _types():
-        raise ValueError("%s must be float32, float16 or bfloat16" % name)
-    if not x.is_cuda or (device is not None and x.device != device):
+    at = x.get_device()
+    if at < 0 or (index is not None and at != index):
         raise ValueError("%s must be a CUDA tensor on the device of the others" % name)
-    if dtype is not None and x.dtype != dtype:
+    if dtype is not None and x.dtype is not dtype:
         raise ValueError("%s must have the type of the other rows" % name)
-    if dim is not None and x.shape[2] != dim:
+    if dim is not None and shape[2] != dim:
         raise ValueError("%s must have %d elements a head" % (name, dim))
-    return x
+    return x.data_ptr(), stride[0], stride[1], shape[0], shape[1]
 
 
-def _ints(x, name, shape, device):
-    if x.dtype.is_floating_point or x.element_size() != 4 or tuple(x.shape) != shape or x.device != device or x.stride(-1) != 1:
-        raise ValueError("%s must be int32 %r, contiguous, on %s" % (name, list(shape), device))
+def _type(x, name):
+    t = _types().get(x.dtype)
+    if t is None:
+        raise ValueError("%s must be float32, float16 or bfloat16" % name)
+    return t
+
+
+def _ints(x, name, shape, index):
+    if x.dtype is not _torch.int32 or x.shape != shape or x.get_device() != index or (x.stride(-1) != 1 and shape[-1] > 1):
+        raise ValueError("%s must be int32 %r, contiguous, on CUDA device %d" % (name, list(shape), index))
     return x.data_ptr()
 
 
-def _weight(w, name, dim, device):
+def _weight(w, name, dim, index):
     if w is None:
-        return None
-    if str(w.dtype) != "torch.float32" or tuple(w.shape) != (dim,) or not w.is_contiguous() or w.device != device:
-        raise ValueError("%s must be float32 [%d] on %s" % (name, dim, device))
+        return 0
+    if w.dtype is not _torch.float32 or w.shape != (dim,) or not w.is_contiguous() or w.get_device() != index:
+        raise ValueError("%s must be float32 [%d] on CUDA device %d" % (name, dim, index))
     return w.data_ptr()
 
 
@@ -73,34 +88,27 @@ class QKNormRopeKernel:
                rope_scaling=1.0, partial_rotary_factor=1.0, stream=None):
         """er_qk_norm_rope: every head of q (and k) normed by its root mean square (weight None: not) and rotated at its token's
         position.  An output may be its own input.  positions: int32 [tokens] (None with partial_rotary_factor 0)."""
-        _rows(q, "q")
-        dev, (tokens, heads, dim) = q.device, q.shape
-        p = er_qk_norm_rope_params()
-        p.num_tokens, p.num_heads, p.head_dim, p.type = tokens, heads, dim, _types()[q.dtype]
-        for name, x, y, at in (("q", q, q_out, 0), ("k", k, k_out, 1)):
-            if x is None and y is None and at == 1:
-                break
-            if x is None or y is None:
-                raise ValueError("%s and %s_out come together" % (name, name))
-            _rows(x, name, dev, q.dtype, dim)
-            _rows(y, name + "_out", dev, q.dtype, dim)
-            if x.shape[0] != tokens or y.shape != x.shape:
-                raise ValueError("%s_out must have the shape of %s, with as many tokens as q" % (name, name))
-            if at == 0:
-                p.q, p.q_out = x.data_ptr(), y.data_ptr()
-                p.q_token_stride, p.q_head_stride, _ = x.stride()
-                p.q_out_token_stride, p.q_out_head_stride, _ = y.stride()
-            else:
-                p.k, p.k_out, p.num_kv_heads = x.data_ptr(), y.data_ptr(), x.shape[1]
-                p.k_token_stride, p.k_head_stride, _ = x.stride()
-                p.k_out_token_stride, p.k_out_head_stride, _ = y.stride()
-        if positions is not None:
-            p.positions = _ints(positions, "positions", (tokens,), dev)
-        p.q_norm_weight = _weight(q_norm_weight, "q_norm_weight", dim, dev)
-        p.k_norm_weight = _weight(k_norm_weight, "k_norm_weight", dim, dev)
-        p.rms_eps, p.rope_theta, p.rope_scaling, p.partial_rotary_factor = rms_eps, rope_theta, rope_scaling, partial_rotary_factor
+        kind = _type(q, "q")
+        dt, index, dim = q.dtype, q.get_device(), q.shape[-1]
+        qp, qt, qh, tokens, heads = _rows(q, "q")
+        op, ot, oh, *shape = _rows(q_out, "q_out", index, dt, dim)
+        if shape != [tokens, heads]:
+            raise ValueError("q_out must have the shape of q")
+        kp = kt = kh = kop = kot = koh = kv_heads = 0
+        if k is not None or k_out is not None:
+            if k is None or k_out is None:
+                raise ValueError("k and k_out come together")
+            kp, kt, kh, *shape = _rows(k, "k", index, dt, dim)
+            kop, kot, koh, *out_shape = _rows(k_out, "k_out", index, dt, dim)
+            kv_heads = shape[1]
+            if shape != out_shape or shape[0] != tokens:
+                raise ValueError("k_out must have the shape of k, with as many tokens as q")
+        pos = 0 if positions is None else _ints(positions, "positions", (tokens,), index)
         if tokens:
-            _call(lib().er_qk_norm_rope, dev, C.byref(p), _stream(stream, dev))
+            _call(lib().er_qk_norm_rope, index, _NORM_ROPE.pack(
+                qp, op, kp, kop, qt, qh, ot, oh, kt, kh, kot, koh, pos, _weight(q_norm_weight, "q_norm_weight", dim, index),
+                _weight(k_norm_weight, "k_norm_weight", dim, index), tokens, heads, kv_heads, dim, kind, rms_eps, rope_theta, rope_scaling,
+                partial_rotary_factor), _stream(stream, index))
 
 
 class BlockScaledFormat(enum.IntEnum):
@@ -146,72 +154,70 @@ class BlockScaledKVCache:
         self.scale_block = page_size // key_scales.shape[2]
         self.device = keys.device
         self._status = torch.zeros(1, dtype=torch.int32, device=keys.device)
+        self._index = keys.get_device()
+        self._buffers = tuple(x.data_ptr() for x in (keys, values, key_scales, value_scales))
+        self._status_ptr = self._status.data_ptr()
+        self._shape = (pages, page_size, self.scale_block, heads, dim, int(self.format))
+        self._workspace_bytes = {}     # by the shape of a call
 
     def _view(self, block_tables, kv_lens):
-        n = kv_lens.shape[0]
-        if block_tables.dim() != 2 or block_tables.shape[0] != n:
+        """(er_kv8_cache bytes, sequences)"""
+        n, index = kv_lens.shape[0], self._index
+        shape, stride = block_tables.shape, block_tables.stride()
+        if len(shape) != 2 or shape[0] != n:
             raise ValueError("block_tables must be [sequences, pages], kv_lens [sequences]")
-        v = er_kv8_cache()
-        v.keys, v.values, v.key_scales, v.value_scales = (x.data_ptr() for x in (self.keys, self.values, self.key_scales, self.value_scales))
-        v.block_tables = _ints(block_tables, "block_tables", tuple(block_tables.shape), self.device)
-        v.kv_lens = _ints(kv_lens, "kv_lens", (n,), self.device)
-        v.status = self._status.data_ptr()
-        v.num_pages, v.page_size, v.scale_block, v.num_kv_heads, v.head_dim = self.num_pages, self.page_size, self.scale_block, self.num_kv_heads, self.head_dim
-        v.format, v.num_seqs, v.block_table_width = int(self.format), n, block_tables.shape[1]
-        v.block_table_stride = max(block_tables.stride(0), block_tables.shape[1])
-        if n > 1 and block_tables.stride(0) < block_tables.shape[1]:
+        if n > 1 and stride[0] < shape[1]:
             raise ValueError("rows of block_tables overlap")
-        return v
+        return _CACHE.pack(*self._buffers, _ints(block_tables, "block_tables", shape, index), _ints(kv_lens, "kv_lens", (n,), index), self._status_ptr,
+                           *self._shape, n, shape[1], max(stride[0], shape[1])), n
 
     def append(self, k, v, block_tables, kv_lens, query_starts=None, *, k_norm_weight=None, rms_eps=1e-6, rope_theta=10000.0, rope_scaling=1.0,
                partial_rotary_factor=1.0, stream=None):
         """er_kv8_append: the call's tokens as the newest rows of their sequences.  query_starts: int32 [sequences + 1], the tokens of
         each sequence; None: one each.  partial_rotary_factor 0: keys come rotated already."""
-        _rows(k, "k", self.device, None, self.head_dim)
-        _rows(v, "v", self.device, k.dtype, self.head_dim)
-        if v.shape != k.shape or k.shape[1] != self.num_kv_heads:
+        index = self._index
+        kind = _type(k, "k")
+        kp, kt, kh, tokens, heads = _rows(k, "k", index, None, self.head_dim)
+        vp, vt, vh, *shape = _rows(v, "v", index, k.dtype, self.head_dim)
+        if shape != [tokens, heads] or heads != self.num_kv_heads:
             raise ValueError("k and v must be [tokens, %d, %d]" % (self.num_kv_heads, self.head_dim))
-        view = self._view(block_tables, kv_lens)
-        p = er_kv8_append_params()
-        p.k, p.v = k.data_ptr(), v.data_ptr()
-        p.k_token_stride, p.k_head_stride, _ = k.stride()
-        p.v_token_stride, p.v_head_stride, _ = v.stride()
-        if query_starts is not None:
-            p.query_starts = _ints(query_starts, "query_starts", (view.num_seqs + 1,), self.device)
-        p.k_norm_weight = _weight(k_norm_weight, "k_norm_weight", self.head_dim, self.device)
-        p.num_tokens, p.type = k.shape[0], _types()[k.dtype]
-        p.rms_eps, p.rope_theta, p.rope_scaling, p.partial_rotary_factor = rms_eps, rope_theta, rope_scaling, partial_rotary_factor
-        if k.shape[0]:
-            _call(lib().er_kv8_append, self.device, C.byref(view), C.byref(p), _stream(stream, self.device))
+        view, n = self._view(block_tables, kv_lens)
+        starts = 0 if query_starts is None else _ints(query_starts, "query_starts", (n + 1,), index)
+        if tokens:
+            _call(lib().er_kv8_append, index, view, _APPEND.pack(
+                kp, vp, kt, kh, vt, vh, starts, _weight(k_norm_weight, "k_norm_weight", self.head_dim, index), tokens, kind, rms_eps, rope_theta,
+                rope_scaling, partial_rotary_factor), _stream(stream, index))
 
     def _attention(self, fn, size_fn, q, out, block_tables, kv_lens, query_starts, query_len, max_query_len, softmax_scale, sliding_window, stream):
-        import torch
-        _rows(q, "q", self.device, None, self.head_dim)
+        index = self._index
+        kind = _type(q, "q")
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        _rows(out, "out", self.device, q.dtype, self.head_dim)
-        if out.shape != q.shape:
+            out = _torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        qp, qt, qh, tokens, heads = _rows(q, "q", index, None, self.head_dim)
+        op, ot, oh, *shape = _rows(out, "out", index, q.dtype, self.head_dim)
+        if shape != [tokens, heads]:
             raise ValueError("out must have the shape of q")
-        view = self._view(block_tables, kv_lens)
-        p = er_kv8_attention_params()
-        p.q, p.out = q.data_ptr(), out.data_ptr()
-        p.q_token_stride, p.q_head_stride, _ = q.stride()
-        p.out_token_stride, p.out_head_stride, _ = out.stride()
-        if query_starts is not None:
-            p.query_starts = _ints(query_starts, "query_starts", (view.num_seqs + 1,), self.device)
-        p.num_tokens, p.num_heads, p.query_len, p.max_query_len, p.type = q.shape[0], q.shape[1], query_len, max_query_len, _types()[q.dtype]
-        p.softmax_scale, p.sliding_window = softmax_scale, sliding_window
-        if q.shape[0] == 0:
+        view, n = self._view(block_tables, kv_lens)
+        starts = 0 if query_starts is None else _ints(query_starts, "query_starts", (n + 1,), index)
+        if tokens == 0:
             return out
-        size = _call(size_fn, self.device, C.byref(view), C.byref(p))
         # a fresh block of the caching allocator for each call: calls on different streams never share one, and a captured call keeps its own
-        if stream is None:
-            work = torch.empty(size, dtype=torch.uint8, device=self.device)
-        else:
-            with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self.device) if isinstance(stream, int) else stream):
-                work = torch.empty(size, dtype=torch.uint8, device=self.device)
-        p.workspace, p.workspace_bytes = work.data_ptr(), size
-        _call(fn, self.device, C.byref(view), C.byref(p), _stream(stream, self.device))
+        key = (n, tokens, heads, query_len, max_query_len, kind)
+        size = self._workspace_bytes.get(key)
+        if size is None:
+            if len(self._workspace_bytes) > 256:
+                self._workspace_bytes.clear()
+            size = self._workspace_bytes[key] = _call(size_fn, index, view, _ATTENTION.pack(
+                qp, op, qt, qh, ot, oh, starts, tokens, heads, query_len, max_query_len, kind, softmax_scale, sliding_window, 0, 0))
+        work = None
+        if size:
+            if stream is None:
+                work = _torch.empty(size, dtype=_torch.uint8, device=self.device)
+            else:
+                with _torch.cuda.stream(_torch.cuda.ExternalStream(stream, device=self.device) if isinstance(stream, int) else stream):
+                    work = _torch.empty(size, dtype=_torch.uint8, device=self.device)
+        _call(fn, index, view, _ATTENTION.pack(qp, op, qt, qh, ot, oh, starts, tokens, heads, query_len, max_query_len, kind, softmax_scale, sliding_window,
+                                               work.data_ptr() if size else 0, size), _stream(stream, index))
         return out
 
     def attention_decode(self, q, block_tables, kv_lens, out=None, query_len=1, softmax_scale=0.0, sliding_window=0, stream=None):

@@ -80,25 +80,20 @@ struct NormRope {
     double log2_theta, inv_scaling;
 };
 
-// The two vectors of a row in registers -> normed and rotated.  `turns`: the row's token's table, nullptr: no rotation.
+// The turns of the pairs `first` .. of a row; pairs from `rotated` on stay.
 template <int VEC>
-__device__ __forceinline__ void norm_rotate(float (&a)[VEC], float (&b)[VEC], int first, int half, int rotated, int lanes, const float* weight,
-                                            float eps, const float2* turns) {
-    if (weight != nullptr) {
-        float ss = 0.f;
+__device__ __forceinline__ void rotate(float (&a)[VEC], float (&b)[VEC], int first, int rotated, const float2* turns) {
+    if (first + VEC <= rotated) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
-        for (int off = lanes >> 1; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-        const float f = rsqrtf(ss / static_cast<float>(2 * half) + eps);
-        if (first < half) {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                a[i] *= f * __ldg(weight + first + i);
-                b[i] *= f * __ldg(weight + half + first + i);
-            }
+        for (int i = 0; i < VEC; i += 2) {
+            const float4 cs = *reinterpret_cast<const float4*>(turns + first + i);
+            const float x0 = a[i], y0 = b[i], x1 = a[i + 1], y1 = b[i + 1];
+            a[i] = x0 * cs.x - y0 * cs.y;
+            b[i] = x0 * cs.y + y0 * cs.x;
+            a[i + 1] = x1 * cs.z - y1 * cs.w;
+            b[i + 1] = x1 * cs.w + y1 * cs.z;
         }
-    }
-    if (turns != nullptr && first < rotated) {
+    } else {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             if (first + i < rotated) {
@@ -110,12 +105,34 @@ __device__ __forceinline__ void norm_rotate(float (&a)[VEC], float (&b)[VEC], in
         }
     }
 }
+__device__ __forceinline__ void load_weights(float* f, const float* w, int n) {
+    for (int i = 0; i < n; i += 4) *reinterpret_cast<float4*>(f + i) = *reinterpret_cast<const float4*>(w + i);
+}
+// Rows of a table start on 16 bytes.  A frequency takes a 64-bit exp2, some 150 instructions of the slow pipe: once a pair, not once a turn.
+__host__ __device__ __forceinline__ int turn_stride(int rotated) { return (rotated + 1) & ~1; }
+__host__ __device__ __forceinline__ int table_bytes(int tokens, int rotated) { return (tokens + 1) * turn_stride(rotated) * 8; }
+// (cos, sin) of `tokens` tokens at turns[t * turn_stride + pair], by the whole CTA; the caller synchronises behind it.
+template <typename Position>
+__device__ __forceinline__ void build_turns(float2* turns, double* frequencies, int tokens, int rotated, int half, double log2_theta, double inv_scaling, Position position) {
+    if (rotated == 0) return;
+    for (int i = threadIdx.x; i < rotated; i += kThreads) frequencies[i] = rope_frequency(i, half, log2_theta, inv_scaling);
+    __syncthreads();
+    const int stride = turn_stride(rotated);
+    for (int e = threadIdx.x; e < tokens * rotated; e += kThreads) {
+        const int t = e / rotated, pair = e - t * rotated;
+        turns[t * stride + pair] = rope_turn(position(t), frequencies[pair]);
+    }
+}
 
+// A warp works on kBatch sets of rows at a time, so that the loads of all are in flight together.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const __grid_constant__ NormRope p) {
-    extern __shared__ float2 turns[];   // [tokens_per_cta][rotated]
-    constexpr int VEC = Act<T>::kVec;
-    const int half = p.head_dim >> 1;
+    extern __shared__ float4 shared4[];                            // weights [2][head_dim], turns [tokens_per_cta][turn_stride], frequencies
+    constexpr int VEC = Act<T>::kVec, kBatch = 2;
+    float* weights = reinterpret_cast<float*>(shared4);
+    float2* turns = reinterpret_cast<float2*>(weights + 2 * p.head_dim);
+    double* frequencies = reinterpret_cast<double*>(turns + p.tokens_per_cta * turn_stride(p.rotated));
+    const int half = p.head_dim >> 1, stride = turn_stride(p.rotated);
     const int t0 = static_cast<int>(blockIdx.x) * p.tokens_per_cta;
     const int nt = min(p.tokens_per_cta, p.num_tokens - t0);
     const int rows_per_warp = 32 / p.lanes;
@@ -123,46 +140,68 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const __grid_con
     const int sub = lane / p.lanes, first = (lane & (p.lanes - 1)) * VEC;
     const int heads = p.heads[0] + p.heads[1], rows = nt * heads;
     const int step = (kThreads / 32) * rows_per_warp * gridDim.y;
-    for (int e = threadIdx.x; e < nt * p.rotated; e += kThreads) {
-        const int t = e / p.rotated, pair = e - t * p.rotated;
-        turns[e] = rope_turn(__ldg(p.positions + t0 + t), rope_frequency(pair, half, p.log2_theta, p.inv_scaling));
-    }
-    __syncthreads();
-    for (int r0 = (static_cast<int>(blockIdx.y) * (kThreads / 32) + warp) * rows_per_warp; r0 < rows; r0 += step) {
-        const int r = r0 + sub;
-        const bool on = r < rows && first < half;
-        const int t = on ? r / heads : 0;
-        int h = on ? r - t * heads : 0;
-        const int side = h >= p.heads[0] ? 1 : 0;
-        h -= side ? p.heads[0] : 0;
-        float a[VEC] = {}, b[VEC] = {};
-        if (on) {
-            const T* src = static_cast<const T*>(p.in[side]) + (t0 + t) * p.in_token[side] + h * p.in_head[side] + first;
-            Act<T>::unpack(*reinterpret_cast<const uint4*>(src), a);
-            Act<T>::unpack(*reinterpret_cast<const uint4*>(src + half), b);
+    const bool any_norm = p.weight[0] != nullptr || p.weight[1] != nullptr;
+    if (any_norm) {
+        for (int e = threadIdx.x; e < 2 * p.head_dim; e += kThreads) {
+            const float* w = p.weight[e >= p.head_dim ? 1 : 0];
+            weights[e] = w != nullptr ? __ldg(w + (e >= p.head_dim ? e - p.head_dim : e)) : 1.f;
         }
-        // lanes of one warp may hold a query and a key row: a missing weight is a factor of one
-        const bool any_norm = p.weight[0] != nullptr || p.weight[1] != nullptr;
-        if (any_norm) {
-            float ss = 0.f;
+    }
+    build_turns(turns, frequencies, nt, p.rotated, half, p.log2_theta, p.inv_scaling, [&](int t) { return __ldg(p.positions + t0 + t); });
+    bool ready = false;
+    for (int r0 = (static_cast<int>(blockIdx.y) * (kThreads / 32) + warp) * rows_per_warp; r0 < rows || !ready; r0 += kBatch * step) {
+        uint4 va[kBatch], vb[kBatch];
+        int t[kBatch], h[kBatch], side[kBatch];
+        bool on[kBatch];
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
-            for (int off = p.lanes >> 1; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-            const float* w = p.weight[side];
-            if (on && w != nullptr) {
-                const float f = rsqrtf(ss / static_cast<float>(p.head_dim) + p.eps);
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    a[i] *= f * __ldg(w + first + i);
-                    b[i] *= f * __ldg(w + half + first + i);
-                }
+        for (int k = 0; k < kBatch; ++k) {
+            const int r = r0 + k * step + sub;
+            on[k] = r < rows && first < half;
+            t[k] = on[k] ? r / heads : 0;
+            h[k] = on[k] ? r - t[k] * heads : 0;
+            side[k] = h[k] >= p.heads[0] ? 1 : 0;
+            h[k] -= side[k] ? p.heads[0] : 0;
+            va[k] = vb[k] = make_uint4(0, 0, 0, 0);
+            if (on[k]) {
+                const T* src = static_cast<const T*>(side[k] ? p.in[1] : p.in[0]) + (t0 + t[k]) * (side[k] ? p.in_token[1] : p.in_token[0]) +
+                               h[k] * (side[k] ? p.in_head[1] : p.in_head[0]) + first;
+                va[k] = *reinterpret_cast<const uint4*>(src);
+                vb[k] = *reinterpret_cast<const uint4*>(src + half);
             }
         }
-        if (on) {
-            norm_rotate<VEC>(a, b, first, half, p.rotated, 1, nullptr, 0.f, p.rotated > 0 ? turns + t * p.rotated : nullptr);
-            T* dst = static_cast<T*>(p.out[side]) + (t0 + t) * p.out_token[side] + h * p.out_head[side] + first;
-            *reinterpret_cast<uint4*>(dst) = Act<T>::pack(a);
-            *reinterpret_cast<uint4*>(dst + half) = Act<T>::pack(b);
+        if (!ready) {                                              // the tables are built while the first rows are on their way
+            __syncthreads();
+            ready = true;
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            float a[VEC], b[VEC];
+            Act<T>::unpack(va[k], a);
+            Act<T>::unpack(vb[k], b);
+            if (any_norm) {
+                float ss = 0.f;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
+                for (int off = p.lanes >> 1; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+                if (on[k] && (side[k] ? p.weight[1] : p.weight[0]) != nullptr) {
+                    const float f = rsqrtf(ss / static_cast<float>(p.head_dim) + p.eps);
+                    float wa[VEC], wb[VEC];
+                    load_weights(wa, weights + side[k] * p.head_dim + first, VEC);
+                    load_weights(wb, weights + side[k] * p.head_dim + half + first, VEC);
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        a[i] *= f * wa[i];
+                        b[i] *= f * wb[i];
+                    }
+                }
+            }
+            if (on[k]) {
+                rotate<VEC>(a, b, first, p.rotated, turns + t[k] * stride);
+                T* dst = static_cast<T*>(side[k] ? p.out[1] : p.out[0]) + (t0 + t[k]) * (side[k] ? p.out_token[1] : p.out_token[0]) +
+                         h[k] * (side[k] ? p.out_head[1] : p.out_head[0]) + first;
+                *reinterpret_cast<uint4*>(dst) = Act<T>::pack(a);
+                *reinterpret_cast<uint4*>(dst + half) = Act<T>::pack(b);
+            }
         }
     }
 }
@@ -178,19 +217,28 @@ struct Kv8Append {
     double log2_theta, inv_scaling;
 };
 
-// CTA = one block of scale_block tokens of one sequence; its warps walk the (side, kv head) pairs, scale_block / 16 warps to a pair, a
-// warp holding up to 16 rows of it in registers (16 * D / 32 values a lane) between the maximum and the encoding, so that a row is read
-// once.  blockIdx.x numbers the blocks a sequence can touch without a prefix sum over the batch: sequence s owns the numbers from
-// starts[s] / scale_block + 2 s on, always enough for a run of tokens that begins and ends inside a block; the rest return at once.
-// blockIdx.y spreads the pairs over more CTAs when there are few blocks.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {   // a NaN wins
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// CTA = one block of scale_block tokens of one sequence; its warps walk the (kv head, side) pairs, scale_block / 16 warps to a pair, a warp
+// holding up to 16 rows of it in registers between the maximum and the encoding, so that a row is read once; 16-bit rows stay packed there and the
+// loads of the warp's next pair are in flight meanwhile (float32: no room for both).  The norm factor of a row is positive, so it
+// multiplies the row's maximum and the reciprocal of the scale, not the elements.  blockIdx.x numbers the blocks a sequence can touch (kv8_find_slot):
+// sequence s owns the numbers from starts[s] / scale_block + 2 s on, always enough for a run of tokens that begins and ends inside a block; the rest
+// return at once.  blockIdx.y spreads the pairs over more CTAs when there are few blocks.
 template <typename T, int D, bool E4M3>
-__global__ void __launch_bounds__(kThreads, 2) kv8_append_kernel(const __grid_constant__ Kv8Append p) {
-    extern __shared__ float2 turns[];   // [scale_block][rotated]
-    __shared__ uint32_t warp_max[kThreads / 32];
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) kv8_append_kernel(const __grid_constant__ Kv8Append p) {
+    extern __shared__ float4 shared4[];        // [scale_block][turn_stride], frequencies
+    float2* turns = reinterpret_cast<float2*>(shared4);
+    __shared__ float warp_max[2][kThreads / 32];
     constexpr int VEC = Act<T>::kVec, HALF = D / 2;
     constexpr int kLanes = HALF / VEC, kRowsPerPass = 32 / kLanes, kPasses = 16 / kRowsPerPass;
+    constexpr bool kAhead = sizeof(T) == 2;
     const Kv8Cache& c = p.cache;
-    const int sb = c.scale_block;
+    const int sb = c.scale_block, stride = turn_stride(p.rotated);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // ---- which sequence, which block ----
     int seq, begin, count, j;
@@ -210,8 +258,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_append_kernel(const __grid_co
         if (threadIdx.x == 0) kv8_report(c, ER_ERR_SHAPE);
         return;
     }
-    const int block_pos = (first_pos / sb + j) * sb;       // first position of the block
-    if (block_pos >= len) return;
+    const int block_pos = ((first_pos >> c.scale_shift) + j) << c.scale_shift;       // first position of the block
+    if (block_pos >= len || block_pos < 0) return;
     const int page = kv8_page(c, seq, block_pos);
     if (page < 0) {
         if (threadIdx.x == 0) kv8_report(c, ER_ERR_OUT_OF_PAGES);
@@ -219,99 +267,142 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_append_kernel(const __grid_co
     }
     const int lead = max(0, first_pos - block_pos);        // rows of the block that were there before
     const int end = min(sb, len - block_pos);              // rows lead .. end are new
-    const int in_page = kv8_in_page(c, block_pos);
     const int token0 = begin + block_pos - first_pos;      // the call's token at row 0 of the block (negative below `lead`)
-    for (int e = threadIdx.x; e < (end - lead) * p.rotated; e += kThreads) {
-        const int t = e / p.rotated, pair = e - t * p.rotated;
-        turns[e] = rope_turn(block_pos + lead + t, rope_frequency(pair, HALF, p.log2_theta, p.inv_scaling));
-    }
-    if (p.rotated > 0) __syncthreads();
-    const int wpp = sb / 16, groups = (kThreads / 32) / wpp;           // warps per pair, pairs at a time
+    const int64_t block_row = kv8_row(c, page, 0, kv8_in_page(c, block_pos));
+    const int wpp = sb / 16, groups = (kThreads / 32) / wpp, group = warp / wpp;     // warps per pair, pairs at a time
     const int pairs = 2 * c.num_kv_heads;
     const int row0 = (warp % wpp) * 16, sub = lane / kLanes, first = (lane % kLanes) * VEC;
-    for (int base = static_cast<int>(blockIdx.y) * groups; base < pairs; base += groups * gridDim.y) {   // uniform over the CTA
-        const int pr = base + warp / wpp;
-        const bool on = pr < pairs;
-        const int side = on ? pr & 1 : 0, head = on ? pr >> 1 : 0;
-        float a[kPasses][VEC], b[kPasses][VEC];
-        uint32_t mx = 0;
+    uint4 va[kPasses], vb[kPasses];
+    float old = 0.f;
+    // keys and values take turns in a warp, keys cost more: pairs 2 m, 2 m + 1 are the sides of a head, swapped every other time round
+    auto side_of = [&](int it, int pr) { return groups > 1 ? (pr ^ it) & 1 : pr & 1; };
+    auto load = [&](int it, uint4 (&a)[kPasses], uint4 (&b)[kPasses]) {
+        const int pr = it * groups + group, side = side_of(it, pr), head = pr >> 1;
+        const T* base = static_cast<const T*>(side ? p.in[1] : p.in[0]) + head * (side ? p.in_head[1] : p.in_head[0]) + first;
+        const int64_t token = side ? p.in_token[1] : p.in_token[0];
 #pragma unroll
         for (int ps = 0; ps < kPasses; ++ps) {
             const int row = row0 + ps * kRowsPerPass + sub;
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) a[ps][i] = b[ps][i] = 0.f;
-            if (on && row >= lead && row < end) {
-                const T* src = static_cast<const T*>(p.in[side]) + (token0 + row) * p.in_token[side] + head * p.in_head[side] + first;
-                Act<T>::unpack(__ldg(reinterpret_cast<const uint4*>(src)), a[ps]);
-                Act<T>::unpack(__ldg(reinterpret_cast<const uint4*>(src + HALF)), b[ps]);
+            a[ps] = b[ps] = make_uint4(0, 0, 0, 0);
+            if (pr < pairs && row >= lead && row < end) {
+                const T* src = base + (token0 + row) * token;
+                a[ps] = __ldg(reinterpret_cast<const uint4*>(src));
+                b[ps] = __ldg(reinterpret_cast<const uint4*>(src + HALF));
             }
         }
-        const int64_t at = kv8_row(c, page, head, in_page);
-        float* scale_at = c.scales[side] + kv8_scale_at(c, at);
-        const float old = on && lead > 0 ? *scale_at : 0.f;
-        if (side == 0) {                                                // uniform over a warp
+        if (pr < pairs && lead > 0) old = (side ? c.scales[1] : c.scales[0])[kv8_scale_at(c, block_row + static_cast<int64_t>(head) * c.page_size)];
+    };
+    const int its = (pairs + groups - 1) / groups;
+    int it = blockIdx.y;
+    load(it, va, vb);
+    build_turns(turns, reinterpret_cast<double*>(turns + sb * stride), end - lead, p.rotated, HALF, p.log2_theta, p.inv_scaling, [&](int t) { return block_pos + lead + t; });
+    float wa[VEC], wb[VEC];
+    if (p.weight != nullptr) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            wa[i] = __ldg(p.weight + first + i);
+            wb[i] = __ldg(p.weight + HALF + first + i);
+        }
+    }
+    __syncthreads();
+    for (int turn = 0; it < its; it += gridDim.y, turn ^= 1) {         // uniform over the CTA
+        const int pr = it * groups + group, side = side_of(it, pr), head = pr >> 1;
+        uint4 ca[kPasses], cb[kPasses];
+#pragma unroll
+        for (int ps = 0; ps < kPasses; ++ps) { ca[ps] = va[ps]; cb[ps] = vb[ps]; }
+        const float before = lead > 0 ? old : 0.f;
+        if (kAhead && it + static_cast<int>(gridDim.y) < its) load(it + gridDim.y, va, vb);
+        // ---- the largest magnitude ----
+        float factor[kPasses], mx = 0.f;
+        auto element = [&](int ps, float (&a)[VEC], float (&b)[VEC]) {      // a row without its norm factor
+            Act<T>::unpack(ca[ps], a);
+            Act<T>::unpack(cb[ps], b);
+            if (side == 0) {
+                if (p.weight != nullptr) {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) { a[i] *= wa[i]; b[i] *= wb[i]; }
+                }
+                // rows of zeros turn by some token's angle
+                rotate<VEC>(a, b, first, p.rotated, turns + min(max(row0 + ps * kRowsPerPass + sub - lead, 0), end - lead - 1) * stride);
+            }
+        };
+#pragma unroll
+        for (int ps = 0; ps < kPasses; ++ps) {
+            float a[VEC], b[VEC];
+            factor[ps] = 1.f;
+            if (side == 0 && p.weight != nullptr) {                         // uniform over a warp
+                Act<T>::unpack(ca[ps], a);
+                Act<T>::unpack(cb[ps], b);
+                float ss = 0.f;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
+#pragma unroll
+                for (int off = kLanes / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+                factor[ps] = rsqrtf(ss / static_cast<float>(D) + p.eps);
+            }
+            element(ps, a, b);
+            float m = 0.f;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) m = max3_nan(m, fabsf(a[i]), fabsf(b[i]));
+            mx = max3_nan(mx, m * factor[ps], 0.f);
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) mx = max3_nan(mx, __shfl_xor_sync(0xffffffffu, mx, off), 0.f);
+        if (wpp > 1) {
+            if (lane == 0) warp_max[turn][warp] = mx;
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(wpp * 32) : "memory");      // the warps of the pair; the other half of the array is for the next pair
+            for (int w = 0; w < wpp; ++w) mx = max3_nan(mx, warp_max[turn][group * wpp + w], 0.f);
+        }
+        if (pr < pairs) {
+            const float need = needed_scale<E4M3>(mx);
+            const float scale = (before >= need) ? before : (isnan(before) ? before : need);  // a NaN on either side stays
+            const float inv = scale > 0.f ? __frcp_rn(scale) : 0.f;
+            const bool grown = lead > 0 && scale > before;
+            const float ratio = grown ? __fdiv_rn(before, scale) : 1.f;
+            const int64_t at = block_row + static_cast<int64_t>(head) * c.page_size;
+            uint8_t* dst = (side ? c.codes[1] : c.codes[0]) + at * D + first;
 #pragma unroll
             for (int ps = 0; ps < kPasses; ++ps) {
                 const int row = row0 + ps * kRowsPerPass + sub;
-                const int t = min(max(row - lead, 0), end - lead - 1);  // rows of zeros turn by some token's angle
-                norm_rotate<VEC>(a[ps], b[ps], first, HALF, p.rotated, kLanes, p.weight, p.eps, p.rotated > 0 ? turns + t * p.rotated : nullptr);
-            }
-        }
+                uint8_t* d = dst + row * D;
+                float a[VEC], b[VEC];
+                if (row >= lead && row < end) {
+                    element(ps, a, b);
+                    const float f = factor[ps] * inv;
 #pragma unroll
-        for (int ps = 0; ps < kPasses; ++ps)
+                    for (int i = 0; i < VEC; ++i) { a[i] *= f; b[i] *= f; }
+                    if (!(inv > 0.f)) {                                     // zeros, or a NaN scale: codes of zeros
 #pragma unroll
-            for (int i = 0; i < VEC; ++i)   // magnitudes compare like integers, infinities and NaN above all others
-                mx = max(mx, max(__float_as_uint(a[ps][i]) & 0x7FFFFFFFu, __float_as_uint(b[ps][i]) & 0x7FFFFFFFu));
-        mx = __reduce_max_sync(0xffffffffu, mx);
-        if (wpp > 1) {
-            if (lane == 0) warp_max[warp] = mx;
-            __syncthreads();
-            for (int w = 0; w < wpp; ++w) mx = max(mx, warp_max[warp / wpp * wpp + w]);
-            __syncthreads();                                            // read by all before the next pair's maxima
-        }
-        if (!on) continue;
-        const float need = needed_scale<E4M3>(__uint_as_float(mx));
-        const float scale = (old >= need) ? old : (isnan(old) ? old : need);   // a NaN on either side stays
-        const float inv = scale > 0.f ? __frcp_rn(scale) : 0.f;         // NaN scale: codes of zeros
-        uint8_t* dst = c.codes[side] + at * D;
-        const bool grown = lead > 0 && scale > old;
-        const float ratio = grown ? __fdiv_rn(old, scale) : 1.f;
+                        for (int i = 0; i < VEC; ++i) a[i] = b[i] = 0.f;
+                    }
+                } else if (row < lead && grown) {
 #pragma unroll
-        for (int ps = 0; ps < kPasses; ++ps) {
-            const int row = row0 + ps * kRowsPerPass + sub;
-            uint8_t* d = dst + row * D + first;
-            if (row >= lead && row < end) {
+                    for (int i = 0; i < VEC; i += 4) {
+                        decode4f<E4M3>(*reinterpret_cast<const uint32_t*>(d + i), a + i);
+                        decode4f<E4M3>(*reinterpret_cast<const uint32_t*>(d + HALF + i), b + i);
+                    }
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    a[ps][i] = inv > 0.f ? a[ps][i] * inv : 0.f;
-                    b[ps][i] = inv > 0.f ? b[ps][i] * inv : 0.f;
+                    for (int i = 0; i < VEC; ++i) { a[i] *= ratio; b[i] *= ratio; }
+                } else {
+                    continue;
                 }
-            } else if (row < lead && grown) {
+                uint32_t lo[VEC / 4], hi[VEC / 4];
 #pragma unroll
                 for (int i = 0; i < VEC; i += 4) {
-                    decode4f<E4M3>(*reinterpret_cast<const uint32_t*>(d + i), a[ps] + i);
-                    decode4f<E4M3>(*reinterpret_cast<const uint32_t*>(d + HALF + i), b[ps] + i);
+                    lo[i / 4] = encode4<E4M3>(a[i], a[i + 1], a[i + 2], a[i + 3]);
+                    hi[i / 4] = encode4<E4M3>(b[i], b[i + 1], b[i + 2], b[i + 3]);
                 }
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) { a[ps][i] *= ratio; b[ps][i] *= ratio; }
-            } else {
-                continue;
+                if constexpr (VEC == 8) {
+                    *reinterpret_cast<uint2*>(d) = make_uint2(lo[0], lo[1]);
+                    *reinterpret_cast<uint2*>(d + HALF) = make_uint2(hi[0], hi[1]);
+                } else {
+                    *reinterpret_cast<uint32_t*>(d) = lo[0];
+                    *reinterpret_cast<uint32_t*>(d + HALF) = hi[0];
+                }
             }
-            uint32_t lo[VEC / 4], hi[VEC / 4];
-#pragma unroll
-            for (int i = 0; i < VEC; i += 4) {
-                lo[i / 4] = encode4<E4M3>(a[ps][i], a[ps][i + 1], a[ps][i + 2], a[ps][i + 3]);
-                hi[i / 4] = encode4<E4M3>(b[ps][i], b[ps][i + 1], b[ps][i + 2], b[ps][i + 3]);
-            }
-            if constexpr (VEC == 8) {
-                *reinterpret_cast<uint2*>(d) = make_uint2(lo[0], lo[1]);
-                *reinterpret_cast<uint2*>(d + HALF) = make_uint2(hi[0], hi[1]);
-            } else {
-                *reinterpret_cast<uint32_t*>(d) = lo[0];
-                *reinterpret_cast<uint32_t*>(d + HALF) = hi[0];
-            }
+            if (row0 == 0 && lane == 0) (side ? c.scales[1] : c.scales[0])[kv8_scale_at(c, at)] = scale;
         }
-        if (row0 == 0 && lane == 0) *scale_at = scale;
+        if (!kAhead && it + static_cast<int>(gridDim.y) < its) load(it + gridDim.y, va, vb);
     }
 }
 
@@ -344,7 +435,8 @@ int32_t launch_norm_rope(NormRope& p, cudaStream_t s) {
     const int rows = p.tokens_per_cta * (p.heads[0] + p.heads[1]);
     const int split = p.num_tokens <= 37 ? (rows + rows_per_pass - 1) / rows_per_pass : 1;
     const dim3 grid((p.num_tokens + p.tokens_per_cta - 1) / p.tokens_per_cta, split);
-    qk_norm_rope_kernel<T><<<grid, kThreads, static_cast<size_t>(p.tokens_per_cta) * p.rotated * sizeof(float2), s>>>(p);
+    const size_t smem = 2 * p.head_dim * sizeof(float) + table_bytes(p.tokens_per_cta, p.rotated);
+    qk_norm_rope_kernel<T><<<grid, kThreads, smem, s>>>(p);
     return kv8_launched(cudaGetLastError(), "qk_norm_rope_kernel");
 }
 
@@ -354,9 +446,9 @@ int32_t launch_append(const Kv8Append& p, cudaStream_t s) {
     const unsigned blocks = p.starts == nullptr ? p.cache.num_seqs : p.num_tokens / sb + 2u * p.cache.num_seqs;
     const int groups = (kThreads / 32) / (sb / 16), steps = (2 * p.cache.num_kv_heads + groups - 1) / groups;
     const dim3 grid(blocks, blocks >= 592 ? 1 : steps);   // 592: four CTAs' worth of blocks for each SM
-    const size_t smem = static_cast<size_t>(sb) * p.rotated * sizeof(float2);   // up to 64 KB
+    const size_t smem = table_bytes(sb, p.rotated);   // up to 64.5 KB
     if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kv8_append_kernel<T, D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024);
+        const cudaError_t e = cudaFuncSetAttribute(kv8_append_kernel<T, D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, table_bytes(128, D / 2));
         if (e != cudaSuccess) return kv8_launched(e, "kv8_append_kernel");
     }
     kv8_append_kernel<T, D, E4M3><<<grid, kThreads, smem, s>>>(p);
