@@ -1,9 +1,11 @@
 // er_qk_norm_rope and er_kv8_append: head norms, rotation and block quantisation of a ragged batch of rows.
 //
-// Both are one pass over the rows and bound by memory.  A row (one head of one token) is held by kLanes neighbouring lanes of a warp, each
-// with one 16-byte vector of the first half of the row and the vector head_dim / 2 further, so that both members of a rotated pair are in
-// one thread, and the sum of squares takes log2(kLanes) shuffles.  The (cos, sin) table of a CTA's tokens is built once in shared memory
-// and used by all of their heads: a sincos of a 64-bit angle costs about 60 instructions, and there are 8 to 40 heads to a token.
+// Both are one pass over the rows and bound by memory, if the instructions an element stay under about ten.  A row (one head of one token) is held by
+// kLanes neighbouring lanes of a warp, each with one 16-byte vector of the first half of the row and the vector head_dim / 2 further, so that
+// both members of a rotated pair are in one thread, and the sum of squares takes log2(kLanes) shuffles.  Angles: the frequencies (a 64-bit exp2 each,
+// some 150 instructions of a slow pipe) once a CTA, the (cos, sin) of a token once for all of its heads, in shared memory in the order in which the
+// lanes read them: 16 bytes (two pairs) a lane, lane beside lane.
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 
@@ -75,132 +77,112 @@ struct NormRope {
     const int32_t* positions;
     int heads[2];
     int num_tokens, head_dim, rotated;   // rotated: pairs
-    int tokens_per_cta, lanes;           // lanes per row: a power of two >= head_dim / 2 / vector
+    int lanes, warps_per_token;          // lanes per row: a power of two >= head_dim / 2 / vector
     float eps;
     double log2_theta, inv_scaling;
 };
 
-// The turns of the pairs `first` .. of a row; pairs from `rotated` on stay.
+// Place of pair `pair` in a table of `vectors` lanes of VEC pairs: the i-th two pairs of all lanes lie side by side.
+template <int VEC> __host__ __device__ __forceinline__ int turn_place(int pair, int vectors) {
+    return (((pair % VEC) >> 1) * vectors + pair / VEC) * 2 + (pair & 1);
+}
+// A lane's pairs of a row, turned; `turns`: the token's table at the lane's vector, pairs from `rotated` on stay.
 template <int VEC>
-__device__ __forceinline__ void rotate(float (&a)[VEC], float (&b)[VEC], int first, int rotated, const float2* turns) {
-    if (first + VEC <= rotated) {
+__device__ __forceinline__ void rotate(float (&a)[VEC], float (&b)[VEC], int first, int rotated, int vectors, const float2* turns) {
+    if (first >= rotated) return;
 #pragma unroll
-        for (int i = 0; i < VEC; i += 2) {
-            const float4 cs = *reinterpret_cast<const float4*>(turns + first + i);
-            const float x0 = a[i], y0 = b[i], x1 = a[i + 1], y1 = b[i + 1];
-            a[i] = x0 * cs.x - y0 * cs.y;
-            b[i] = x0 * cs.y + y0 * cs.x;
-            a[i + 1] = x1 * cs.z - y1 * cs.w;
-            b[i + 1] = x1 * cs.w + y1 * cs.z;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            if (first + i < rotated) {
-                const float2 cs = turns[first + i];
-                const float x = a[i], y = b[i];
-                a[i] = x * cs.x - y * cs.y;
-                b[i] = x * cs.y + y * cs.x;
-            }
-        }
+    for (int i = 0; i < VEC; i += 2) {
+        const float4 cs = *reinterpret_cast<const float4*>(turns + i * vectors);
+        const float x0 = a[i], y0 = b[i], x1 = a[i + 1], y1 = b[i + 1];
+        a[i] = x0 * cs.x - y0 * cs.y;
+        b[i] = x0 * cs.y + y0 * cs.x;
+        a[i + 1] = x1 * cs.z - y1 * cs.w;
+        b[i + 1] = x1 * cs.w + y1 * cs.z;
     }
 }
-__device__ __forceinline__ void load_weights(float* f, const float* w, int n) {
-    for (int i = 0; i < n; i += 4) *reinterpret_cast<float4*>(f + i) = *reinterpret_cast<const float4*>(w + i);
-}
-// Rows of a table start on 16 bytes.  A frequency takes a 64-bit exp2, some 150 instructions of the slow pipe: once a pair, not once a turn.
-__host__ __device__ __forceinline__ int turn_stride(int rotated) { return (rotated + 1) & ~1; }
-__host__ __device__ __forceinline__ int table_bytes(int tokens, int rotated) { return (tokens + 1) * turn_stride(rotated) * 8; }
-// (cos, sin) of `tokens` tokens at turns[t * turn_stride + pair], by the whole CTA; the caller synchronises behind it.
-template <typename Position>
-__device__ __forceinline__ void build_turns(float2* turns, double* frequencies, int tokens, int rotated, int half, double log2_theta, double inv_scaling, Position position) {
-    if (rotated == 0) return;
-    for (int i = threadIdx.x; i < rotated; i += kThreads) frequencies[i] = rope_frequency(i, half, log2_theta, inv_scaling);
-    __syncthreads();
-    const int stride = turn_stride(rotated);
-    for (int e = threadIdx.x; e < tokens * rotated; e += kThreads) {
-        const int t = e / rotated, pair = e - t * rotated;
-        turns[t * stride + pair] = rope_turn(position(t), frequencies[pair]);
-    }
+__device__ __forceinline__ void make_frequencies(double* frequencies, int rotated, int half, double log2_theta, double inv_scaling) {
+    for (int i = threadIdx.x; i < rotated; i += blockDim.x) frequencies[i] = rope_frequency(i, half, log2_theta, inv_scaling);
 }
 
-// A warp works on kBatch sets of rows at a time, so that the loads of all are in flight together.
+// A warp takes the heads of a token (or every warps_per_token-th set of them when there are few tokens), with its lane's turns and weights in
+// registers, and kBatch sets of rows at a time, so that the loads of all are in flight together.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const __grid_constant__ NormRope p) {
-    extern __shared__ float4 shared4[];                            // weights [2][head_dim], turns [tokens_per_cta][turn_stride], frequencies
+    extern __shared__ double shared8[];                            // frequencies [rotated], turns of each warp's token [vectors * VEC]
     constexpr int VEC = Act<T>::kVec, kBatch = 2;
-    float* weights = reinterpret_cast<float*>(shared4);
-    float2* turns = reinterpret_cast<float2*>(weights + 2 * p.head_dim);
-    double* frequencies = reinterpret_cast<double*>(turns + p.tokens_per_cta * turn_stride(p.rotated));
-    const int half = p.head_dim >> 1, stride = turn_stride(p.rotated);
-    const int t0 = static_cast<int>(blockIdx.x) * p.tokens_per_cta;
-    const int nt = min(p.tokens_per_cta, p.num_tokens - t0);
-    const int rows_per_warp = 32 / p.lanes;
+    const int half = p.head_dim >> 1, vectors = half / VEC, table = half;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int sub = lane / p.lanes, first = (lane & (p.lanes - 1)) * VEC;
-    const int heads = p.heads[0] + p.heads[1], rows = nt * heads;
-    const int step = (kThreads / 32) * rows_per_warp * gridDim.y;
-    const bool any_norm = p.weight[0] != nullptr || p.weight[1] != nullptr;
-    if (any_norm) {
-        for (int e = threadIdx.x; e < 2 * p.head_dim; e += kThreads) {
-            const float* w = p.weight[e >= p.head_dim ? 1 : 0];
-            weights[e] = w != nullptr ? __ldg(w + (e >= p.head_dim ? e - p.head_dim : e)) : 1.f;
+    float2* turns = reinterpret_cast<float2*>(shared8 + ((p.rotated + 1) & ~1)) + warp * table;
+    const int rows_per_warp = 32 / p.lanes, sub = lane / p.lanes, vector = lane & (p.lanes - 1), first = vector * VEC;
+    const bool own = first < half;
+    make_frequencies(shared8, p.rotated, half, p.log2_theta, p.inv_scaling);
+    __syncthreads();
+    const int slots = gridDim.x * (kThreads / 32) / p.warps_per_token, share = warp % p.warps_per_token;
+    for (int t = (static_cast<int>(blockIdx.x) * (kThreads / 32) + warp) / p.warps_per_token; t < p.num_tokens; t += slots) {
+        if (p.rotated > 0) {
+            const int position = __ldg(p.positions + t);
+            __syncwarp();                                          // the last token's table has been read
+            for (int i = lane; i < half; i += 32) turns[turn_place<VEC>(i, vectors)] = i < p.rotated ? rope_turn(position, shared8[i]) : make_float2(1.f, 0.f);
+            __syncwarp();
         }
-    }
-    build_turns(turns, frequencies, nt, p.rotated, half, p.log2_theta, p.inv_scaling, [&](int t) { return __ldg(p.positions + t0 + t); });
-    bool ready = false;
-    for (int r0 = (static_cast<int>(blockIdx.y) * (kThreads / 32) + warp) * rows_per_warp; r0 < rows || !ready; r0 += kBatch * step) {
-        uint4 va[kBatch], vb[kBatch];
-        int t[kBatch], h[kBatch], side[kBatch];
-        bool on[kBatch];
+        float cs[2 * VEC];
+        if (own && first < p.rotated) {
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-            const int r = r0 + k * step + sub;
-            on[k] = r < rows && first < half;
-            t[k] = on[k] ? r / heads : 0;
-            h[k] = on[k] ? r - t[k] * heads : 0;
-            side[k] = h[k] >= p.heads[0] ? 1 : 0;
-            h[k] -= side[k] ? p.heads[0] : 0;
-            va[k] = vb[k] = make_uint4(0, 0, 0, 0);
-            if (on[k]) {
-                const T* src = static_cast<const T*>(side[k] ? p.in[1] : p.in[0]) + (t0 + t[k]) * (side[k] ? p.in_token[1] : p.in_token[0]) +
-                               h[k] * (side[k] ? p.in_head[1] : p.in_head[0]) + first;
-                va[k] = *reinterpret_cast<const uint4*>(src);
-                vb[k] = *reinterpret_cast<const uint4*>(src + half);
+            for (int i = 0; i < VEC; i += 2) *reinterpret_cast<float4*>(cs + 2 * i) = *reinterpret_cast<const float4*>(turns + vector * 2 + i * vectors);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) { cs[2 * i] = 1.f; cs[2 * i + 1] = 0.f; }
+        }
+#pragma unroll 1
+        for (int side = 0; side < 2; ++side) {
+            const int heads = side ? p.heads[1] : p.heads[0];
+            const float* w = side ? p.weight[1] : p.weight[0];
+            float wa[VEC], wb[VEC];
+            if (own && w != nullptr) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) { wa[i] = __ldg(w + first + i); wb[i] = __ldg(w + half + first + i); }
             }
-        }
-        if (!ready) {                                              // the tables are built while the first rows are on their way
-            __syncthreads();
-            ready = true;
-        }
+            const int64_t in_head = side ? p.in_head[1] : p.in_head[0], out_head = side ? p.out_head[1] : p.out_head[0];
+            const T* src = static_cast<const T*>(side ? p.in[1] : p.in[0]) + t * (side ? p.in_token[1] : p.in_token[0]) + first;
+            T* dst = static_cast<T*>(side ? p.out[1] : p.out[0]) + t * (side ? p.out_token[1] : p.out_token[0]) + first;
+            const int step = rows_per_warp * p.warps_per_token;
+            for (int h0 = share * rows_per_warp + sub; h0 - sub < heads; h0 += kBatch * step) {
+                uint4 va[kBatch], vb[kBatch];
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-            float a[VEC], b[VEC];
-            Act<T>::unpack(va[k], a);
-            Act<T>::unpack(vb[k], b);
-            if (any_norm) {
-                float ss = 0.f;
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
-                for (int off = p.lanes >> 1; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-                if (on[k] && (side[k] ? p.weight[1] : p.weight[0]) != nullptr) {
-                    const float f = rsqrtf(ss / static_cast<float>(p.head_dim) + p.eps);
-                    float wa[VEC], wb[VEC];
-                    load_weights(wa, weights + side[k] * p.head_dim + first, VEC);
-                    load_weights(wb, weights + side[k] * p.head_dim + half + first, VEC);
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) {
-                        a[i] *= f * wa[i];
-                        b[i] *= f * wb[i];
+                for (int k = 0; k < kBatch; ++k) {
+                    const int h = h0 + k * step;
+                    va[k] = vb[k] = make_uint4(0, 0, 0, 0);
+                    if (own && h < heads) {
+                        va[k] = *reinterpret_cast<const uint4*>(src + h * in_head);
+                        vb[k] = *reinterpret_cast<const uint4*>(src + h * in_head + half);
                     }
                 }
-            }
-            if (on[k]) {
-                rotate<VEC>(a, b, first, p.rotated, turns + t[k] * stride);
-                T* dst = static_cast<T*>(side[k] ? p.out[1] : p.out[0]) + (t0 + t[k]) * (side[k] ? p.out_token[1] : p.out_token[0]) +
-                         h[k] * (side[k] ? p.out_head[1] : p.out_head[0]) + first;
-                *reinterpret_cast<uint4*>(dst) = Act<T>::pack(a);
-                *reinterpret_cast<uint4*>(dst + half) = Act<T>::pack(b);
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) {
+                    const int h = h0 + k * step;
+                    float a[VEC], b[VEC];
+                    Act<T>::unpack(va[k], a);
+                    Act<T>::unpack(vb[k], b);
+                    if (w != nullptr) {
+                        float ss = 0.f;
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
+                        for (int off = p.lanes >> 1; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+                        const float f = rsqrtf(ss / static_cast<float>(p.head_dim) + p.eps);
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) { a[i] *= f * wa[i]; b[i] *= f * wb[i]; }
+                    }
+                    if (own && h < heads) {
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) {
+                            const float x = a[i], y = b[i];
+                            a[i] = x * cs[2 * i] - y * cs[2 * i + 1];
+                            b[i] = x * cs[2 * i + 1] + y * cs[2 * i];
+                        }
+                        *reinterpret_cast<uint4*>(dst + h * out_head) = Act<T>::pack(a);
+                        *reinterpret_cast<uint4*>(dst + h * out_head + half) = Act<T>::pack(b);
+                    }
+                }
             }
         }
     }
@@ -223,22 +205,22 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {   // a Na
     return r;
 }
 
-// CTA = one block of scale_block tokens of one sequence; its warps walk the (kv head, side) pairs, scale_block / 16 warps to a pair, a warp
-// holding up to 16 rows of it in registers between the maximum and the encoding, so that a row is read once; 16-bit rows stay packed there and the
-// loads of the warp's next pair are in flight meanwhile (float32: no room for both).  The norm factor of a row is positive, so it
-// multiplies the row's maximum and the reciprocal of the scale, not the elements.  blockIdx.x numbers the blocks a sequence can touch (kv8_find_slot):
-// sequence s owns the numbers from starts[s] / scale_block + 2 s on, always enough for a run of tokens that begins and ends inside a block; the rest
-// return at once.  blockIdx.y spreads the pairs over more CTAs when there are few blocks.
+// CTA = one block of scale_block tokens of one sequence; its warps walk the (kv head, side) pairs, scale_block / 8 warps to a pair (512
+// threads for blocks of 128), a warp holding up to 8 rows of it in registers between the maximum and the encoding, so that a row is read once, while the
+// loads of its next pair are in flight.  The norm factor of a row is positive, so it multiplies the row's maximum and the reciprocal of the
+// scale, not the elements.  blockIdx.x numbers the blocks a sequence can touch (kv8_find_slot): sequence s owns the numbers from
+// starts[s] / scale_block + 2 s on, always enough for a run of tokens that begins and ends inside a block; the rest return at once.  blockIdx.y spreads
+// the pairs over more CTAs when there are few blocks.
+constexpr int kWarpRows = 8;
 template <typename T, int D, bool E4M3>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) kv8_append_kernel(const __grid_constant__ Kv8Append p) {
-    extern __shared__ float4 shared4[];        // [scale_block][turn_stride], frequencies
-    float2* turns = reinterpret_cast<float2*>(shared4);
-    __shared__ float warp_max[2][kThreads / 32];
+__global__ void __launch_bounds__(512) kv8_append_kernel(const __grid_constant__ Kv8Append p) {
+    extern __shared__ double shared8[];        // frequencies [rotated], turns [scale_block][D / 2]
+    __shared__ float warp_max[2][16];
     constexpr int VEC = Act<T>::kVec, HALF = D / 2;
-    constexpr int kLanes = HALF / VEC, kRowsPerPass = 32 / kLanes, kPasses = 16 / kRowsPerPass;
-    constexpr bool kAhead = sizeof(T) == 2;
+    constexpr int kLanes = HALF / VEC, kRowsPerPass = 32 / kLanes, kPasses = kWarpRows / kRowsPerPass;
+    float2* turns = reinterpret_cast<float2*>(shared8 + HALF);
     const Kv8Cache& c = p.cache;
-    const int sb = c.scale_block, stride = turn_stride(p.rotated);
+    const int sb = c.scale_block;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // ---- which sequence, which block ----
     int seq, begin, count, j;
@@ -269,33 +251,40 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) kv8_append_k
     const int end = min(sb, len - block_pos);              // rows lead .. end are new
     const int token0 = begin + block_pos - first_pos;      // the call's token at row 0 of the block (negative below `lead`)
     const int64_t block_row = kv8_row(c, page, 0, kv8_in_page(c, block_pos));
-    const int wpp = sb / 16, groups = (kThreads / 32) / wpp, group = warp / wpp;     // warps per pair, pairs at a time
+    const int wpp = sb / kWarpRows, groups = static_cast<int>(blockDim.x >> 5) / wpp, group = warp / wpp;    // warps per pair, pairs at a time
     const int pairs = 2 * c.num_kv_heads;
-    const int row0 = (warp % wpp) * 16, sub = lane / kLanes, first = (lane % kLanes) * VEC;
+    const int row0 = (warp % wpp) * kWarpRows, sub = lane / kLanes, vector = lane % kLanes, first = vector * VEC;
     uint4 va[kPasses], vb[kPasses];
     float old = 0.f;
     // keys and values take turns in a warp, keys cost more: pairs 2 m, 2 m + 1 are the sides of a head, swapped every other time round
     auto side_of = [&](int it, int pr) { return groups > 1 ? (pr ^ it) & 1 : pr & 1; };
-    auto load = [&](int it, uint4 (&a)[kPasses], uint4 (&b)[kPasses]) {
+    auto load = [&](int it) {
         const int pr = it * groups + group, side = side_of(it, pr), head = pr >> 1;
         const T* base = static_cast<const T*>(side ? p.in[1] : p.in[0]) + head * (side ? p.in_head[1] : p.in_head[0]) + first;
         const int64_t token = side ? p.in_token[1] : p.in_token[0];
 #pragma unroll
         for (int ps = 0; ps < kPasses; ++ps) {
             const int row = row0 + ps * kRowsPerPass + sub;
-            a[ps] = b[ps] = make_uint4(0, 0, 0, 0);
+            va[ps] = vb[ps] = make_uint4(0, 0, 0, 0);
             if (pr < pairs && row >= lead && row < end) {
                 const T* src = base + (token0 + row) * token;
-                a[ps] = __ldg(reinterpret_cast<const uint4*>(src));
-                b[ps] = __ldg(reinterpret_cast<const uint4*>(src + HALF));
+                va[ps] = __ldg(reinterpret_cast<const uint4*>(src));
+                vb[ps] = __ldg(reinterpret_cast<const uint4*>(src + HALF));
             }
         }
         if (pr < pairs && lead > 0) old = (side ? c.scales[1] : c.scales[0])[kv8_scale_at(c, block_row + static_cast<int64_t>(head) * c.page_size)];
     };
     const int its = (pairs + groups - 1) / groups;
     int it = blockIdx.y;
-    load(it, va, vb);
-    build_turns(turns, reinterpret_cast<double*>(turns + sb * stride), end - lead, p.rotated, HALF, p.log2_theta, p.inv_scaling, [&](int t) { return block_pos + lead + t; });
+    load(it);
+    if (p.rotated > 0) {
+        make_frequencies(shared8, p.rotated, HALF, p.log2_theta, p.inv_scaling);
+        __syncthreads();
+        for (int e = threadIdx.x; e < (end - lead) * HALF; e += blockDim.x) {
+            const int t = e / HALF, pair = e % HALF;
+            turns[t * HALF + turn_place<VEC>(pair, kLanes)] = pair < p.rotated ? rope_turn(block_pos + lead + t, shared8[pair]) : make_float2(1.f, 0.f);
+        }
+    }
     float wa[VEC], wb[VEC];
     if (p.weight != nullptr) {
 #pragma unroll
@@ -305,54 +294,46 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) kv8_append_k
         }
     }
     __syncthreads();
+#pragma unroll 1
     for (int turn = 0; it < its; it += gridDim.y, turn ^= 1) {         // uniform over the CTA
         const int pr = it * groups + group, side = side_of(it, pr), head = pr >> 1;
-        uint4 ca[kPasses], cb[kPasses];
-#pragma unroll
-        for (int ps = 0; ps < kPasses; ++ps) { ca[ps] = va[ps]; cb[ps] = vb[ps]; }
-        const float before = lead > 0 ? old : 0.f;
-        if (kAhead && it + static_cast<int>(gridDim.y) < its) load(it + gridDim.y, va, vb);
-        // ---- the largest magnitude ----
-        float factor[kPasses], mx = 0.f;
-        auto element = [&](int ps, float (&a)[VEC], float (&b)[VEC]) {      // a row without its norm factor
-            Act<T>::unpack(ca[ps], a);
-            Act<T>::unpack(cb[ps], b);
-            if (side == 0) {
-                if (p.weight != nullptr) {
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) { a[i] *= wa[i]; b[i] *= wb[i]; }
-                }
-                // rows of zeros turn by some token's angle
-                rotate<VEC>(a, b, first, p.rotated, turns + min(max(row0 + ps * kRowsPerPass + sub - lead, 0), end - lead - 1) * stride);
-            }
-        };
+        float a[kPasses][VEC], b[kPasses][VEC];
 #pragma unroll
         for (int ps = 0; ps < kPasses; ++ps) {
-            float a[VEC], b[VEC];
+            Act<T>::unpack(va[ps], a[ps]);
+            Act<T>::unpack(vb[ps], b[ps]);
+        }
+        const float before = lead > 0 ? old : 0.f;
+        if (it + static_cast<int>(gridDim.y) < its) load(it + gridDim.y);
+        // ---- norm, rotation, the largest magnitude ----
+        float factor[kPasses], mx = 0.f;
+#pragma unroll
+        for (int ps = 0; ps < kPasses; ++ps) {
             factor[ps] = 1.f;
-            if (side == 0 && p.weight != nullptr) {                         // uniform over a warp
-                Act<T>::unpack(ca[ps], a);
-                Act<T>::unpack(cb[ps], b);
-                float ss = 0.f;
+            if (side == 0) {                                               // uniform over a warp
+                if (p.weight != nullptr) {
+                    float ss = 0.f;
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
+                    for (int i = 0; i < VEC; ++i) ss = fmaf(a[ps][i], a[ps][i], fmaf(b[ps][i], b[ps][i], ss));
 #pragma unroll
-                for (int off = kLanes / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-                factor[ps] = rsqrtf(ss / static_cast<float>(D) + p.eps);
+                    for (int off = kLanes / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+                    factor[ps] = rsqrtf(ss / static_cast<float>(D) + p.eps);
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) { a[ps][i] *= wa[i]; b[ps][i] *= wb[i]; }
+                }
+                const int t = min(max(row0 + ps * kRowsPerPass + sub - lead, 0), end - lead - 1);    // rows of zeros turn by some token's angle
+                rotate<VEC>(a[ps], b[ps], first, p.rotated, kLanes, turns + t * HALF + vector * 2);
             }
-            element(ps, a, b);
             float m = 0.f;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) m = max3_nan(m, fabsf(a[i]), fabsf(b[i]));
+            for (int i = 0; i < VEC; ++i) m = max3_nan(m, fabsf(a[ps][i]), fabsf(b[ps][i]));
             mx = max3_nan(mx, m * factor[ps], 0.f);
         }
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) mx = max3_nan(mx, __shfl_xor_sync(0xffffffffu, mx, off), 0.f);
-        if (wpp > 1) {
-            if (lane == 0) warp_max[turn][warp] = mx;
-            asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(wpp * 32) : "memory");      // the warps of the pair; the other half of the array is for the next pair
-            for (int w = 0; w < wpp; ++w) mx = max3_nan(mx, warp_max[turn][group * wpp + w], 0.f);
-        }
+        if (lane == 0) warp_max[turn][warp] = mx;
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(wpp * 32) : "memory");      // the warps of the pair; the other half of the array is for the next pair
+        for (int w = 0; w < wpp; ++w) mx = max3_nan(mx, warp_max[turn][group * wpp + w], 0.f);
         if (pr < pairs) {
             const float need = needed_scale<E4M3>(mx);
             const float scale = (before >= need) ? before : (isnan(before) ? before : need);  // a NaN on either side stays
@@ -365,32 +346,30 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) kv8_append_k
             for (int ps = 0; ps < kPasses; ++ps) {
                 const int row = row0 + ps * kRowsPerPass + sub;
                 uint8_t* d = dst + row * D;
-                float a[VEC], b[VEC];
                 if (row >= lead && row < end) {
-                    element(ps, a, b);
                     const float f = factor[ps] * inv;
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) { a[i] *= f; b[i] *= f; }
+                    for (int i = 0; i < VEC; ++i) { a[ps][i] *= f; b[ps][i] *= f; }
                     if (!(inv > 0.f)) {                                     // zeros, or a NaN scale: codes of zeros
 #pragma unroll
-                        for (int i = 0; i < VEC; ++i) a[i] = b[i] = 0.f;
+                        for (int i = 0; i < VEC; ++i) a[ps][i] = b[ps][i] = 0.f;
                     }
                 } else if (row < lead && grown) {
 #pragma unroll
                     for (int i = 0; i < VEC; i += 4) {
-                        decode4f<E4M3>(*reinterpret_cast<const uint32_t*>(d + i), a + i);
-                        decode4f<E4M3>(*reinterpret_cast<const uint32_t*>(d + HALF + i), b + i);
+                        decode4f<E4M3>(*reinterpret_cast<const uint32_t*>(d + i), a[ps] + i);
+                        decode4f<E4M3>(*reinterpret_cast<const uint32_t*>(d + HALF + i), b[ps] + i);
                     }
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) { a[i] *= ratio; b[i] *= ratio; }
+                    for (int i = 0; i < VEC; ++i) { a[ps][i] *= ratio; b[ps][i] *= ratio; }
                 } else {
                     continue;
                 }
                 uint32_t lo[VEC / 4], hi[VEC / 4];
 #pragma unroll
                 for (int i = 0; i < VEC; i += 4) {
-                    lo[i / 4] = encode4<E4M3>(a[i], a[i + 1], a[i + 2], a[i + 3]);
-                    hi[i / 4] = encode4<E4M3>(b[i], b[i + 1], b[i + 2], b[i + 3]);
+                    lo[i / 4] = encode4<E4M3>(a[ps][i], a[ps][i + 1], a[ps][i + 2], a[ps][i + 3]);
+                    hi[i / 4] = encode4<E4M3>(b[ps][i], b[ps][i + 1], b[ps][i + 2], b[ps][i + 3]);
                 }
                 if constexpr (VEC == 8) {
                     *reinterpret_cast<uint2*>(d) = make_uint2(lo[0], lo[1]);
@@ -402,7 +381,6 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) kv8_append_k
             }
             if (row0 == 0 && lane == 0) (side ? c.scales[1] : c.scales[0])[kv8_scale_at(c, at)] = scale;
         }
-        if (!kAhead && it + static_cast<int>(gridDim.y) < its) load(it + gridDim.y, va, vb);
     }
 }
 
@@ -428,14 +406,12 @@ int32_t launch_norm_rope(NormRope& p, cudaStream_t s) {
     const int vecs = p.head_dim / 2 / Act<T>::kVec;
     p.lanes = 1;
     while (p.lanes < vecs) p.lanes *= 2;
-    // One token to a CTA while that leaves SMs idle, then up to four: the table of four tokens is one sincos a thread.  With fewer tokens
-    // than a quarter of the SMs the rows of a token are spread over several CTAs, each with the table of its own.
-    p.tokens_per_cta = p.num_tokens <= 2048 ? 1 : 4;
-    const int rows_per_pass = kThreads / p.lanes;
-    const int rows = p.tokens_per_cta * (p.heads[0] + p.heads[1]);
-    const int split = p.num_tokens <= 37 ? (rows + rows_per_pass - 1) / rows_per_pass : 1;
-    const dim3 grid((p.num_tokens + p.tokens_per_cta - 1) / p.tokens_per_cta, split);
-    const size_t smem = 2 * p.head_dim * sizeof(float) + table_bytes(p.tokens_per_cta, p.rotated);
+    // A warp a token when that gives each SM 16 warps of work, else the heads of a token over two, four, eight warps; up to four CTAs an SM walk the tokens.
+    p.warps_per_token = 1;
+    while (p.warps_per_token < 8 && static_cast<int64_t>(p.num_tokens) * p.warps_per_token < 148 * 16) p.warps_per_token *= 2;
+    const int tokens_per_cta = (kThreads / 32) / p.warps_per_token;
+    const int grid = std::min((p.num_tokens + tokens_per_cta - 1) / tokens_per_cta, 148 * 4);
+    const size_t smem = ((p.rotated + 1) & ~1) * sizeof(double) + (kThreads / 32) * (p.head_dim / 2) * sizeof(float2);
     qk_norm_rope_kernel<T><<<grid, kThreads, smem, s>>>(p);
     return kv8_launched(cudaGetLastError(), "qk_norm_rope_kernel");
 }
@@ -444,14 +420,15 @@ template <typename T, int D, bool E4M3>
 int32_t launch_append(const Kv8Append& p, cudaStream_t s) {
     const int sb = p.cache.scale_block;
     const unsigned blocks = p.starts == nullptr ? p.cache.num_seqs : p.num_tokens / sb + 2u * p.cache.num_seqs;
-    const int groups = (kThreads / 32) / (sb / 16), steps = (2 * p.cache.num_kv_heads + groups - 1) / groups;
+    const int threads = sb == 128 ? 512 : 256;
+    const int groups = threads / 32 / (sb / kWarpRows), steps = (2 * p.cache.num_kv_heads + groups - 1) / groups;
     const dim3 grid(blocks, blocks >= 592 ? 1 : steps);   // 592: four CTAs' worth of blocks for each SM
-    const size_t smem = table_bytes(sb, p.rotated);   // up to 64.5 KB
+    const size_t smem = D / 2 * sizeof(double) + static_cast<size_t>(sb) * (D / 2) * sizeof(float2);   // up to 64.5 KB
     if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kv8_append_kernel<T, D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, table_bytes(128, D / 2));
+        const cudaError_t e = cudaFuncSetAttribute(kv8_append_kernel<T, D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
         if (e != cudaSuccess) return kv8_launched(e, "kv8_append_kernel");
     }
-    kv8_append_kernel<T, D, E4M3><<<grid, kThreads, smem, s>>>(p);
+    kv8_append_kernel<T, D, E4M3><<<grid, threads, smem, s>>>(p);
     return kv8_launched(cudaGetLastError(), "kv8_append_kernel");
 }
 
