@@ -113,6 +113,17 @@ __device__ __forceinline__ float needed_scale(float amax) {
     }
 }
 
+// 1 / scale, 0 for a scale of zero or NaN.  A power of two at or above 2^-126: by its exponent.
+template <bool E4M3>
+__device__ __forceinline__ float reciprocal_scale(float scale) {
+    if (!(scale > 0.f)) return 0.f;
+    if constexpr (E4M3) {
+        const uint32_t b = __float_as_uint(scale);
+        if ((b & 0x7FFFFFu) == 0u && b < 0x7E800000u) return __uint_as_float(0x7F000000u - b);
+    }
+    return __frcp_rn(scale);
+}
+
 // ---- pages ----
 struct Kv8Cache {
     uint8_t* codes[2];      // keys, values

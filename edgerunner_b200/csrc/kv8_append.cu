@@ -109,7 +109,8 @@ __device__ __forceinline__ void make_frequencies(double* frequencies, int rotate
 template <typename T>
 __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const __grid_constant__ NormRope p) {
     extern __shared__ double shared8[];                            // frequencies [rotated], turns of each warp's token [vectors * VEC]
-    constexpr int VEC = Act<T>::kVec, kBatch = 2;
+    constexpr int VEC = Act<T>::kVec, kBatch = 4;
+    const float inv_dim = 1.f / static_cast<float>(p.head_dim);
     const int half = p.head_dim >> 1, vectors = half / VEC, table = half;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     float2* turns = reinterpret_cast<float2*>(shared8 + ((p.rotated + 1) & ~1)) + warp * table;
@@ -125,7 +126,7 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const __grid_con
             for (int i = lane; i < half; i += 32) turns[turn_place<VEC>(i, vectors)] = i < p.rotated ? rope_turn(position, shared8[i]) : make_float2(1.f, 0.f);
             __syncwarp();
         }
-        float cs[2 * VEC];
+        float cs[2 * VEC];                                          // cos, sin of the lane's pairs
         if (own && first < p.rotated) {
 #pragma unroll
             for (int i = 0; i < VEC; i += 2) *reinterpret_cast<float4*>(cs + 2 * i) = *reinterpret_cast<const float4*>(turns + vector * 2 + i * vectors);
@@ -137,10 +138,14 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const __grid_con
         for (int side = 0; side < 2; ++side) {
             const int heads = side ? p.heads[1] : p.heads[0];
             const float* w = side ? p.weight[1] : p.weight[0];
-            float wa[VEC], wb[VEC];
-            if (own && w != nullptr) {
+            float ca[VEC], sa[VEC], cb[VEC], sb[VEC];              // ... times the weights of the two members
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) { wa[i] = __ldg(w + first + i); wb[i] = __ldg(w + half + first + i); }
+            for (int i = 0; i < VEC; ++i) {
+                const float wa = own && w != nullptr ? __ldg(w + first + i) : 1.f, wb = own && w != nullptr ? __ldg(w + half + first + i) : 1.f;
+                ca[i] = cs[2 * i] * wa;
+                sa[i] = cs[2 * i + 1] * wa;
+                cb[i] = cs[2 * i] * wb;
+                sb[i] = cs[2 * i + 1] * wb;
             }
             const int64_t in_head = side ? p.in_head[1] : p.in_head[0], out_head = side ? p.out_head[1] : p.out_head[0];
             const T* src = static_cast<const T*>(side ? p.in[1] : p.in[0]) + t * (side ? p.in_token[1] : p.in_token[0]) + first;
@@ -168,16 +173,16 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const __grid_con
 #pragma unroll
                         for (int i = 0; i < VEC; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
                         for (int off = p.lanes >> 1; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-                        const float f = rsqrtf(ss / static_cast<float>(p.head_dim) + p.eps);
+                        const float f = rsqrtf(ss * inv_dim + p.eps);
 #pragma unroll
-                        for (int i = 0; i < VEC; ++i) { a[i] *= f * wa[i]; b[i] *= f * wb[i]; }
+                        for (int i = 0; i < VEC; ++i) { a[i] *= f; b[i] *= f; }
                     }
                     if (own && h < heads) {
 #pragma unroll
                         for (int i = 0; i < VEC; ++i) {
                             const float x = a[i], y = b[i];
-                            a[i] = x * cs[2 * i] - y * cs[2 * i + 1];
-                            b[i] = x * cs[2 * i + 1] + y * cs[2 * i];
+                            a[i] = x * ca[i] - y * sb[i];
+                            b[i] = x * sa[i] + y * cb[i];
                         }
                         *reinterpret_cast<uint4*>(dst + h * out_head) = Act<T>::pack(a);
                         *reinterpret_cast<uint4*>(dst + h * out_head + half) = Act<T>::pack(b);
@@ -212,6 +217,11 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {   // a Na
 // starts[s] / scale_block + 2 s on, always enough for a run of tokens that begins and ends inside a block; the rest return at once.  blockIdx.y spreads
 // the pairs over more CTAs when there are few blocks.
 constexpr int kWarpRows = 8;
+__device__ __forceinline__ float min3_nan(float a, float b, float c) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 template <typename T, int D, bool E4M3>
 __global__ void __launch_bounds__(512) kv8_append_kernel(const __grid_constant__ Kv8Append p) {
     extern __shared__ double shared8[];        // frequencies [rotated], turns [scale_block][D / 2]
@@ -317,27 +327,29 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const __grid_constant__
                     for (int i = 0; i < VEC; ++i) ss = fmaf(a[ps][i], a[ps][i], fmaf(b[ps][i], b[ps][i], ss));
 #pragma unroll
                     for (int off = kLanes / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-                    factor[ps] = rsqrtf(ss / static_cast<float>(D) + p.eps);
+                    factor[ps] = rsqrtf(ss * (1.f / D) + p.eps);
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) { a[ps][i] *= wa[i]; b[ps][i] *= wb[i]; }
                 }
                 const int t = min(max(row0 + ps * kRowsPerPass + sub - lead, 0), end - lead - 1);    // rows of zeros turn by some token's angle
                 rotate<VEC>(a[ps], b[ps], first, p.rotated, kLanes, turns + t * HALF + vector * 2);
             }
-            float m = 0.f;
+            float up = 0.f, down = 0.f;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) m = max3_nan(m, fabsf(a[ps][i]), fabsf(b[ps][i]));
-            mx = max3_nan(mx, m * factor[ps], 0.f);
+            for (int i = 0; i < VEC; ++i) {
+                up = max3_nan(up, a[ps][i], b[ps][i]);
+                down = min3_nan(down, a[ps][i], b[ps][i]);
+            }
+            mx = max3_nan(mx, up * factor[ps], -down * factor[ps]);
         }
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) mx = max3_nan(mx, __shfl_xor_sync(0xffffffffu, mx, off), 0.f);
+        mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx) & 0x7FFFFFFFu));   // magnitudes compare like integers, NaN above all
         if (lane == 0) warp_max[turn][warp] = mx;
         asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(wpp * 32) : "memory");      // the warps of the pair; the other half of the array is for the next pair
         for (int w = 0; w < wpp; ++w) mx = max3_nan(mx, warp_max[turn][group * wpp + w], 0.f);
         if (pr < pairs) {
             const float need = needed_scale<E4M3>(mx);
             const float scale = (before >= need) ? before : (isnan(before) ? before : need);  // a NaN on either side stays
-            const float inv = scale > 0.f ? __frcp_rn(scale) : 0.f;
+            const float inv = reciprocal_scale<E4M3>(scale);
             const bool grown = lead > 0 && scale > before;
             const float ratio = grown ? __fdiv_rn(before, scale) : 1.f;
             const int64_t at = block_row + static_cast<int64_t>(head) * c.page_size;
