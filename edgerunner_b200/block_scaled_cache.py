@@ -202,7 +202,7 @@ class BlockScaledKVCache:
         if tokens == 0:
             return out
         # a fresh block of the caching allocator for each call: calls on different streams never share one, and a captured call keeps its own
-        key = (n, tokens, heads, query_len, max_query_len, kind)
+        key = (n, block_tables.shape[1], tokens, heads, query_len, max_query_len, kind)
         size = self._workspace_bytes.get(key)
         if size is None:
             if len(self._workspace_bytes) > 256:

@@ -594,24 +594,28 @@ __global__ void __launch_bounds__(256) kv8_prefill_join_kernel(const __grid_cons
 struct Plan {
     int slots, split_from, parts, grid;
 };
-// One CTA fits an SM, so a grid of equal CTAs takes ceil(CTAs / SMs) rounds.  The tile pairs of the last, partly filled round are cut along the
-// keys into the number of parts (up to 8, and no more CTAs than four rounds) that fills whole rounds best; a second launch joins them.
-Plan make_plan(uint32_t num_tokens, int group, int num_seqs, int kv_heads, int sms) {
+// One CTA fits an SM.  With fewer than four rounds of tile pairs the last round counts: its pairs are cut along the keys into the number of parts
+// (up to 8, no more CTAs than four rounds, at least four tiles of the longest sequence to a part) that fills whole rounds best; a second launch
+// joins them.  With more rounds the pairs that see most run first and the short ones of the prompts' beginnings fill the gaps.
+Plan make_plan(const er_kv8_cache* c, const er_kv8_attention_params* u, int sms) {
     Plan pl;
-    pl.slots = static_cast<int>(static_cast<int64_t>(num_tokens) * group / 256) + num_seqs;
-    const int units = pl.slots * kv_heads, rest = units % sms;
-    pl.split_from = units;
+    const int group = static_cast<int>(u->num_heads / c->num_kv_heads), kv_heads = static_cast<int>(c->num_kv_heads);
+    pl.slots = static_cast<int>(static_cast<int64_t>(u->num_tokens) * group / 256) + static_cast<int>(c->num_seqs);
+    const int64_t units = static_cast<int64_t>(pl.slots) * kv_heads;
+    const int64_t most_tiles = (static_cast<int64_t>(c->block_table_width) * c->page_size + kTok - 1) / kTok;
+    const int rest = static_cast<int>(units % sms);
+    pl.split_from = static_cast<int>(units);
     pl.parts = 1;
     double best = 1.0;
-    for (int k = 2; k <= 8 && rest > 0 && rest * k <= 4 * sms; ++k) {
+    for (int k = 2; k <= 8 && units < 4 * sms && rest > 0 && rest * k <= 4 * sms && 4 * k <= most_tiles; ++k) {
         const double rounds = static_cast<double>((rest * k + sms - 1) / sms) / k;
         if (rounds < best - 0.02) {
             best = rounds;
             pl.parts = k;
-            pl.split_from = units - rest;
+            pl.split_from = static_cast<int>(units) - rest;
         }
     }
-    pl.grid = pl.split_from + (units - pl.split_from) * pl.parts;
+    pl.grid = pl.split_from + (static_cast<int>(units) - pl.split_from) * pl.parts;
     return pl;
 }
 
@@ -659,7 +663,7 @@ extern "C" int64_t er_kv8_prefill_workspace_bytes(const er_kv8_cache* cache, con
     const Split sp = split_of(cache, u);
     int64_t bytes = sp.few ? kv8_decode_workspace(cache, u, true) : 0;      // the two kernels run one after the other
     if (sp.many) {
-        const Plan pl = make_plan(u->num_tokens, static_cast<int>(u->num_heads / cache->num_kv_heads), static_cast<int>(cache->num_seqs), static_cast<int>(cache->num_kv_heads), sms);
+        const Plan pl = make_plan(cache, u, sms);
         if (pl.parts > 1) bytes = std::max(bytes, static_cast<int64_t>(pl.grid - pl.split_from) * 256 * (cache->head_dim + 4) * 4);
     }
     return bytes;
@@ -691,7 +695,7 @@ extern "C" int32_t er_kv8_attention_prefill(const er_kv8_cache* cache, const er_
         p.window = static_cast<int>(u->sliding_window);
         p.min_rows = kFewRows + 1;
         p.scale_log2 = kv8_scale_log2(u->softmax_scale, cache->head_dim);
-        const Plan pl = make_plan(u->num_tokens, p.group, c.num_seqs, c.num_kv_heads, kv8_sm_count());
+        const Plan pl = make_plan(cache, u, kv8_sm_count());
         p.slots = pl.slots; p.split_from = pl.split_from; p.parts = pl.parts;
         rc = u->type == ER_TYPE_FLOAT16 ? launch_shape<__half>(p, pl, cache->head_dim, e4m3, s) : launch_shape<__nv_bfloat16>(p, pl, cache->head_dim, e4m3, s);
         if (rc != ER_OK) return rc;
