@@ -18,6 +18,7 @@
 // Tensor memory: S_0, S_1 at columns 0, 128; O_0, O_1 at 256, 384.  Shared memory: Q (2 x 128 rows), a ring of K / V tiles of 128 tokens, scales.
 // Every wait is bounded (2 s): then the status word is set, the rest of the waits are skipped, tensor memory is freed, the kernel returns.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv8.cuh"
 #include "prefill_umma.cuh"
@@ -45,6 +46,7 @@ struct Kv8Prefill {
     int num_tokens, group, window, min_rows;    // sequences with fewer query rows are somebody else's
     int slots, split_from, parts;               // CTAs [0, split_from) own a tile pair, the others a part of its keys
     float scale_log2;
+    uint64_t group_magic;                       // ceil(2^64 / group)
 };
 
 // The sequence and the 256 query rows of slot `slot`: sequence s owns the slots from starts[s] * group / 256 + s on.
@@ -72,6 +74,11 @@ __device__ __forceinline__ Tile find_tile(const Kv8Prefill& p, int slot) {
     t.wrong = t.len > most ? ER_ERR_OUT_OF_PAGES : t.len < 0 ? ER_ERR_SHAPE : 0;
     t.len = max(0, min(t.len, most));
     return t;
+}
+
+// r / group by a multiplication (exact below 2^30)
+__device__ __forceinline__ int row_query(const Kv8Prefill& p, int r) {
+    return p.group == 1 ? r : static_cast<int>(__umul64hi(static_cast<uint64_t>(static_cast<uint32_t>(r)), p.group_magic));
 }
 
 struct Waiter {
@@ -183,7 +190,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             uint32_t n = 1;
             if (i < kBarEmpty) n = kTok / 16;
             else if (i == kBarP || i == kBarP + 1) n = 4;
-            else if (i == kBarQ) n = two ? 256 : 128;
+            else if (i == kBarQ) n = two ? 8 : 4;
             else if (i >= kBarScale) n = kTok / 16;
             mbar_init(bars + i, n);
         }
@@ -348,40 +355,55 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
         if (warp < 4 || two) {
         const int i = warp >> 2, m_row = tid & 127, row = tile.row0 + i * 128 + m_row;
-        const bool row_ok = row < tile.rows;
-        const int r_use = min(row, tile.rows - 1), qi = r_use / p.group, qh = head * p.group + r_use % p.group;
+        const int qi = row_query(p, min(row, tile.rows - 1));
         const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t tm_s = tmem + 128u * i + lane_base, tm_o = tmem + 256u + 128u * i + lane_base;
-        float factor;                          // log2(e) * scale * the power of two that the row was divided by
+        // Queries: each warp copies its 32 rows into the operand layout, whole rows at a time (D / 8 lanes a row) and past the L1, most of whose memory
+        // is shared memory here: as loads they waited for room there, 5 us a CTA.  float16 rows are operands as they are; a bfloat16 row is divided by
+        // a power of two in place, since its range is not fp16's.
+        float factor = p.scale_log2;           // log2(e) * scale * that power of two
         {
-            const T* src = static_cast<const T*>(p.q) + static_cast<int64_t>(tile.begin + qi) * p.q_token + qh * p.q_head;
-            uint32_t mx = 0;
-            uint4 v[D / 8];
-#pragma unroll
-            for (int k = 0; k < D / 8; ++k) {
-                v[k] = row_ok ? __ldg(reinterpret_cast<const uint4*>(src) + k) : make_uint4(0, 0, 0, 0);
-                float f[8];
-                Act<T>::unpack(v[k], f);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) mx = max(mx, __float_as_uint(f[e]) & 0x7FFFFFFFu);
+            constexpr int kLanes = D / 8, kRows = 32 / kLanes;
+            const int chunk = lane % kLanes;
+            uint8_t* tile_gen = q_gen + i * kTile;
+            const uint32_t to = smem_u32(tile_gen) + (chunk >> 3) * kRegion;
+#pragma unroll 4
+            for (int r0 = (warp & 3) * 32 + lane / kLanes; r0 < (warp & 3) * 32 + 32; r0 += kRows) {
+                const int r = min(tile.row0 + i * 128 + r0, tile.rows - 1), query = row_query(p, r);
+                const T* src = static_cast<const T*>(p.q) + static_cast<int64_t>(tile.begin + query) * p.q_token + (head * p.group + r - query * p.group) * p.q_head + chunk * 8;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + um_swz(r0, chunk & 7)), "l"(src), "r"(tile.row0 + i * 128 + r0 < tile.rows ? 16 : 0) : "memory");
             }
-            const uint32_t ex = min(max(mx >> 23, 1u), 252u);
-            const float down = __uint_as_float((253u - ex) << 23);
-            factor = __uint_as_float((ex + 1u) << 23) * p.scale_log2;
-            uint8_t* dst = q_gen + i * kTile;
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            __syncwarp();
+            if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value) {
+                uint32_t mx = 0;
+#pragma unroll 4
+                for (int k = 0; k < D / 8; ++k) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(tile_gen + (k >> 3) * kRegion + um_swz(m_row, k & 7));
+                    const uint32_t w[4] = {v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu, v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu};
 #pragma unroll
-            for (int k = 0; k < D / 8; ++k) {
-                float f[8];
-                Act<T>::unpack(v[k], f);
-                uint4 o;
-                o.x = half2_word(f[0] * down, f[1] * down);
-                o.y = half2_word(f[2] * down, f[3] * down);
-                o.z = half2_word(f[4] * down, f[5] * down);
-                o.w = half2_word(f[6] * down, f[7] * down);
-                *reinterpret_cast<uint4*>(dst + (k >> 3) * kRegion + um_swz(m_row, k & 7)) = o;
+                    for (int e = 0; e < 4; ++e) mx = __vmaxu2(mx, w[e]);                  // magnitudes compare like integers
+                }
+                mx = max(mx >> 16, mx & 0xFFFFu);
+                const uint32_t ex = min(max(mx >> 7, 1u), 252u);
+                const float down = __uint_as_float((253u - ex) << 23);
+                factor *= __uint_as_float((ex + 1u) << 23);
+#pragma unroll 4
+                for (int k = 0; k < D / 8; ++k) {
+                    uint4* at = reinterpret_cast<uint4*>(tile_gen + (k >> 3) * kRegion + um_swz(m_row, k & 7));
+                    float f[8];
+                    Act<T>::unpack(*at, f);
+                    uint4 o;
+                    o.x = half2_word(f[0] * down, f[1] * down);
+                    o.y = half2_word(f[2] * down, f[3] * down);
+                    o.z = half2_word(f[4] * down, f[5] * down);
+                    o.w = half2_word(f[6] * down, f[7] * down);
+                    *at = o;
+                }
             }
             fence_async_smem();
-            mbar_arrive(bars + kBarQ);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bars + kBarQ);
         }
         const int limit = min(tile.len - 1, past + qi);
         const int lower = p.window > 0 ? past + qi - p.window + 1 : 0;
@@ -537,8 +559,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         const float up = fast_exp2(LR - kCarry), f = parts > 1 ? up : (l == 0.f ? 0.f : up / l);
         float* part_row = parts > 1 ? p.partial + (static_cast<int64_t>(static_cast<int>(blockIdx.x) - p.split_from) * 256 + i * 128 + m_row) * (D + 4) : nullptr;
         if (parts > 1) { part_row[0] = m; part_row[1] = l; }
-        T* dst = static_cast<T*>(p.out) + static_cast<int64_t>(tile.begin + qi) * p.out_token + qh * p.out_head;
-#pragma unroll
+        // Finished rows leave through shared memory, a bulk copy a row: over the ring of K / V tiles, which every product has read.
+        constexpr int kOutRow = D * 2 + 16;
+        uint8_t* out_row = gen + (i * 128 + m_row) * kOutRow;
+        static_assert(256 * kOutRow <= kStages * kTile, "");
+#pragma unroll 1
         for (int c0 = 0; c0 < D; c0 += 32) {
             uint32_t o[32];
             if (tiles > 0) {
@@ -551,10 +576,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             if (parts > 1) {
 #pragma unroll
                 for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(part_row + 4 + c0 + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
-            } else if (row_ok) {
+            } else {
 #pragma unroll
-                for (int k = 0; k < 32; k += 8) *reinterpret_cast<uint4*>(dst + c0 + k) = Act<T>::pack(x + k);
+                for (int k = 0; k < 32; k += 8) *reinterpret_cast<uint4*>(out_row + (c0 + k) * 2) = Act<T>::pack(x + k);
             }
+        }
+        if (parts == 1 && row < tile.rows) {
+            fence_async_smem();
+            T* dst = static_cast<T*>(p.out) + static_cast<int64_t>(tile.begin + qi) * p.out_token + (head * p.group + row - qi * p.group) * p.out_head;
+            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(out_row)), "r"(D * 2) : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         }
         }
     }
@@ -694,6 +726,7 @@ extern "C" int32_t er_kv8_attention_prefill(const er_kv8_cache* cache, const er_
         p.group = static_cast<int>(u->num_heads) / c.num_kv_heads;
         p.window = static_cast<int>(u->sliding_window);
         p.min_rows = kFewRows + 1;
+        p.group_magic = p.group == 1 ? 0 : ~0ull / static_cast<uint64_t>(p.group) + 1;
         p.scale_log2 = kv8_scale_log2(u->softmax_scale, cache->head_dim);
         const Plan pl = make_plan(cache, u, kv8_sm_count());
         p.slots = pl.slots; p.split_from = pl.split_from; p.parts = pl.parts;
