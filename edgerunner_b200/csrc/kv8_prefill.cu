@@ -367,11 +367,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             const int chunk = lane % kLanes;
             uint8_t* tile_gen = q_gen + i * kTile;
             const uint32_t to = smem_u32(tile_gen) + (chunk >> 3) * kRegion;
+            // row r0 of the tile is head `at_head` of query `query`; kRows further is dq queries and dh heads further
+            int r0 = (warp & 3) * 32 + lane / kLanes;
+            const int r = tile.row0 + i * 128 + r0, query = row_query(p, r), dq = row_query(p, kRows), dh = kRows - dq * p.group;
+            int at_head = r - query * p.group;
+            const T* src = static_cast<const T*>(p.q) + static_cast<int64_t>(tile.begin + query) * p.q_token + (head * p.group + at_head) * p.q_head + chunk * 8;
+            const int64_t on = dq * p.q_token + dh * p.q_head, wrap = p.q_token - p.group * p.q_head;
 #pragma unroll 4
-            for (int r0 = (warp & 3) * 32 + lane / kLanes; r0 < (warp & 3) * 32 + 32; r0 += kRows) {
-                const int r = min(tile.row0 + i * 128 + r0, tile.rows - 1), query = row_query(p, r);
-                const T* src = static_cast<const T*>(p.q) + static_cast<int64_t>(tile.begin + query) * p.q_token + (head * p.group + r - query * p.group) * p.q_head + chunk * 8;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + um_swz(r0, chunk & 7)), "l"(src), "r"(tile.row0 + i * 128 + r0 < tile.rows ? 16 : 0) : "memory");
+            for (int k = 0; k < 32 / kRows; ++k) {
+                if (r + k * kRows < tile.rows)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + um_swz(r0, chunk & 7)), "l"(src) : "memory");
+                else
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to + um_swz(r0, chunk & 7)), "r"(0) : "memory");
+                r0 += kRows;
+                src += on;
+                at_head += dh;
+                if (at_head >= p.group) { at_head -= p.group; src += wrap; }
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
             __syncwarp();
@@ -586,7 +597,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             T* dst = static_cast<T*>(p.out) + static_cast<int64_t>(tile.begin + qi) * p.out_token + (head * p.group + row - qi * p.group) * p.out_head;
             asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(out_row)), "r"(D * 2) : "memory");
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         }
         }
     }
