@@ -93,55 +93,76 @@ struct Place {        // a position in the list
     }
     __device__ __forceinline__ int token(int u) const { return (r.first_unit + unit + u) * kUnit; }   // of the u-th unit from here
 };
-// Total units, by every thread of the CTA (scratch: a value a warp).
-__device__ int64_t total_units(const Kv8Decode& p, int64_t* scratch) {
-    int64_t sum = 0;
-    for (int s = threadIdx.x; s < p.cache.num_seqs; s += blockDim.x) {
-        const SeqRange r = seq_range(p, s);
-        sum += static_cast<int64_t>(r.units) * r.row_tiles;
+// The list, by every thread of the CTA.  `pick(total)` names the unit that the CTA looks for, negative: none.  With a thread a sequence the lengths are
+// read once for both; longer batches are summed first and then walked 32 sequences at a time.
+struct Found {
+    int64_t total;
+    Place place;
+};
+struct ListScratch {
+    int64_t sums[16];
+    Place place;
+};
+template <typename Pick>
+__device__ Found find_in_list(const Kv8Decode& p, ListScratch* scratch, Pick pick) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, seqs = p.cache.num_seqs, heads = p.cache.num_kv_heads;
+    auto units_of = [&](const SeqRange& r) { return static_cast<int64_t>(r.units) * r.row_tiles * heads; };
+    auto take = [&](int s, const SeqRange& r, int64_t offset) {
+        Place pl;
+        pl.seq = s;
+        pl.r = r;
+        pl.item = static_cast<int>(offset / r.units);
+        pl.unit = static_cast<int>(offset % r.units);
+        scratch->place = pl;
+    };
+    const bool once = seqs <= static_cast<int>(blockDim.x);
+    SeqRange mine{};
+    int64_t sum = 0, incl = 0;
+    for (int s = threadIdx.x; s < seqs; s += blockDim.x) {
+        mine = seq_range(p, s);
+        sum += units_of(mine);
     }
+    incl = sum;
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = sum;
+    for (int off = 1; off < 32; off <<= 1) {
+        const int64_t o = __shfl_up_sync(0xffffffffu, incl, off);
+        if (lane >= off) incl += o;
+    }
+    if (lane == 31) scratch->sums[warp] = incl;
     __syncthreads();
-    sum = 0;
-    for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) sum += scratch[w];
-    __syncthreads();
-    return sum * p.cache.num_kv_heads;
-}
-// The place of unit `at` (0 <= at < total), by every thread of the CTA: warp 0 walks the sequences 32 at a time.
-__device__ Place find_place(const Kv8Decode& p, int64_t at, Place* shared_place) {
-    if (threadIdx.x < 32) {
-        int64_t before = 0;
-        for (int s0 = 0; s0 < p.cache.num_seqs; s0 += 32) {
-            const int s = s0 + static_cast<int>(threadIdx.x);
+    Found f{};
+    int64_t before = 0;
+    for (int w = 0; w < warps; ++w) {
+        if (w < warp) before += scratch->sums[w];
+        f.total += scratch->sums[w];
+    }
+    const int64_t at = pick(f.total);
+    if (once) {
+        const int64_t start = before + incl - sum;
+        if (at >= start && at < start + sum) take(threadIdx.x, mine, at - start);
+    } else if (warp == 0 && at >= 0) {
+        before = 0;
+        for (int s0 = 0; s0 < seqs; s0 += 32) {
+            const int s = s0 + lane;
             SeqRange r{};
-            if (s < p.cache.num_seqs) r = seq_range(p, s);
-            const int64_t mine = static_cast<int64_t>(r.units) * r.row_tiles * p.cache.num_kv_heads;
-            int64_t incl = mine;
+            if (s < seqs) r = seq_range(p, s);
+            const int64_t n = units_of(r);
+            incl = n;
 #pragma unroll
             for (int off = 1; off < 32; off <<= 1) {
                 const int64_t o = __shfl_up_sync(0xffffffffu, incl, off);
-                if (static_cast<int>(threadIdx.x) >= off) incl += o;
+                if (lane >= off) incl += o;
             }
-            const int64_t start = before + incl - mine;
-            const bool here = mine > 0 && at >= start && at < start + mine;
-            if (here) {
-                Place pl;
-                pl.seq = s;
-                pl.r = r;
-                pl.item = static_cast<int>((at - start) / pl.r.units);
-                pl.unit = static_cast<int>((at - start) % pl.r.units);
-                *shared_place = pl;
-            }
+            const int64_t start = before + incl - n;
+            const bool here = at >= start && at < start + n;
+            if (here) take(s, r, at - start);
             before += __shfl_sync(0xffffffffu, incl, 31);
             if (__any_sync(0xffffffffu, here)) break;
         }
     }
     __syncthreads();
-    const Place pl = *shared_place;
-    __syncthreads();
-    return pl;
+    f.place = scratch->place;
+    return f;
 }
 // CTA c of n takes the units [total c / n, total (c + 1) / n).
 __device__ __forceinline__ int used_ctas(int64_t total, int ctas) { return static_cast<int>(min(static_cast<int64_t>(ctas), (total + kMinUnits - 1) / kMinUnits)); }
@@ -200,7 +221,7 @@ template <typename T, int D, int NT> __host__ __device__ constexpr int decode_st
 }
 template <typename T, int D, int NT> __host__ __device__ constexpr int join_floats() { return join_warps<T, NT>() * 8 * NT * (D + 4); }
 template <typename T, int D, int NT> __host__ __device__ constexpr int decode_smem() {
-    return decode_warps<T, NT>() * decode_stages<T, D, NT>() * (Stage<D>::kBytes + 16 + 8) + (join_floats<T, D, NT>() + join_warps<T, NT>() * 8 * NT * 2) * 4 + 128 + 1024;
+    return decode_warps<T, NT>() * decode_stages<T, D, NT>() * (Stage<D>::kBytes + 16 + 8) + (join_floats<T, D, NT>() + join_warps<T, NT>() * 8 * NT * 2) * 4 + static_cast<int>(sizeof(ListScratch)) + 16 + 1024;
 }
 // One partial: max, sum, -, - and the unnormalised row.
 template <int D> __host__ __device__ constexpr int partial_stride() { return D + 4; }
@@ -236,8 +257,8 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
     float* join = stage_scales + kWarps * kStages * 4;
     float* join_ml = join + join_floats<T, D, NT>();
     uint64_t* bars = reinterpret_cast<uint64_t*>(join_ml + kJoin * kRows * 2);
-    int64_t* scratch = reinterpret_cast<int64_t*>(bars + kWarps * kStages);   // 96 bytes
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(scratch + 14);
+    ListScratch* scratch = reinterpret_cast<ListScratch*>(bars + kWarps * kStages);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(scratch + 1);
     const Kv8Cache& c = p.cache;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, half = lane >> 4;
     const int odd = D == 64 ? t & 1 : 0;
@@ -247,8 +268,13 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
     if (threadIdx.x == 0) *abort_flag = 0;
     mbar_init_fence();
 
-    const int64_t total = total_units(p, scratch);
-    const int n = used_ctas(total, gridDim.x), cta = blockIdx.x;
+    const int cta = blockIdx.x;
+    const Found list = find_in_list(p, scratch, [&](int64_t total) {
+        const int n = used_ctas(total, gridDim.x);
+        return cta < n ? cta_begin(total, n, cta) : -1;
+    });
+    const int64_t total = list.total;
+    const int n = used_ctas(total, gridDim.x);
     if (cta == 0) {                 // what the host cannot see
         for (int s = threadIdx.x; s < c.num_seqs; s += kThreads) {
             if (__ldg(c.lens + s) > c.table_width * c.page_size) kv8_report(c, ER_ERR_OUT_OF_PAGES);
@@ -258,7 +284,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
     }
     if (cta >= n) return;
     int64_t left = cta_begin(total, n, cta + 1) - cta_begin(total, n, cta);       // units of this CTA not yet walked over
-    Place at = find_place(p, cta_begin(total, n, cta), reinterpret_cast<Place*>(scratch));
+    Place at = list.place;
 
     // ---- producer: this warp's units, kStages - 1 ahead ----
     uint8_t* my_stages = stages + warp * kStages * Stage<D>::kBytes;
@@ -314,6 +340,21 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) produce();
 
+    // the rows of this lane's columns g, dims [D/4 t, D/4 (t+1)): of the next item while the warps of this one are joined
+    constexpr int kVecs = D / 4 / Act<T>::kVec;
+    uint4 ahead[NT][kVecs];
+    auto load_queries = [&]() {
+        const int head = at.item / at.r.row_tiles, first_row = at.item % at.r.row_tiles * kRows;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = first_row + nt * 8 + g, qi = r / p.group;
+            const T* src = static_cast<const T*>(p.q) + static_cast<int64_t>(at.r.begin + qi) * p.q_token + (head * p.group + r - qi * p.group) * p.q_head + (D / 4) * t;
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) ahead[nt][i] = r < at.r.n * p.group ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    load_queries();
+
     int cstage = 0, cphase = 0;
     bool first_segment = true;
     while (left > 0) {
@@ -329,16 +370,9 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
         int limit[NT][2];           // last row that they see
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const int r = rt * kRows + nt * 8 + g;
             float x[D / 4];
 #pragma unroll
-            for (int i = 0; i < D / 4; ++i) x[i] = 0.f;
-            if (r < rows) {
-                const int qi = r / p.group, qh_ = head * p.group + r % p.group;
-                const T* src = static_cast<const T*>(p.q) + static_cast<int64_t>(at.r.begin + qi) * p.q_token + qh_ * p.q_head + (D / 4) * t;
-#pragma unroll
-                for (int i = 0; i < D / 4; i += Act<T>::kVec) Act<T>::unpack(__ldg(reinterpret_cast<const uint4*>(src + i)), x + i);
-            }
+            for (int i = 0; i < kVecs; ++i) Act<T>::unpack(ahead[nt][i], x + i * Act<T>::kVec);
             uint32_t mx = 0;
 #pragma unroll
             for (int i = 0; i < D / 4; ++i) mx = max(mx, __float_as_uint(x[i]) & 0x7FFFFFFFu);
@@ -547,6 +581,12 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
             cphase ^= cstage == 0 ? 1 : 0;
         }
 
+        const Place done = at;
+        left -= seg;
+        if (left > 0) {
+            at.next_item(p);
+            load_queries();
+        }
         // ---- join the warps of the CTA ----
         const float out_scale = R * (1.f / kWeightScale);
 #pragma unroll
@@ -605,7 +645,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
             leave(warp);
         }
         __syncthreads();
-        const bool whole = at.unit == 0 && seg == at.r.units;
+        const bool whole = done.unit == 0 && seg == done.r.units;
         const int cols = min(kRows, rows - rt * kRows);
         for (int e = threadIdx.x; e < cols * (D / 2); e += kThreads) {
             const int col = e / (D / 2), d = (e % (D / 2)) * 2;
@@ -626,7 +666,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
             if (whole) {
                 const int r = rt * kRows + col;
                 const float inv = L == 0.f ? 0.f : 1.f / L;
-                T* dst = static_cast<T*>(p.out) + static_cast<int64_t>(at.r.begin + r / p.group) * p.out_token + (head * p.group + r % p.group) * p.out_head + d;
+                T* dst = static_cast<T*>(p.out) + static_cast<int64_t>(done.r.begin + r / p.group) * p.out_token + (head * p.group + r % p.group) * p.out_head + d;
                 store_pair(dst, x * inv, y * inv);
             } else {
                 float* dst = p.partial + ((static_cast<int64_t>(cta) * 2 + (first_segment ? 0 : 1)) * kRows + col) * partial_stride<D>();
@@ -636,10 +676,6 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
         }
         __syncthreads();
         first_segment = false;
-        left -= seg;
-        if (left > 0) {
-            at.next_item(p);
-        }
     }
     cp_async_wait<0>();
 }
@@ -650,16 +686,21 @@ constexpr int kJoinThreads = 256;
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kJoinThreads) kv8_decode_join_kernel(const __grid_constant__ Kv8Decode p) {
     constexpr int kWarps = kJoinThreads / 32, kRows = decode_rows<NT>(), V = D / 32;
-    __shared__ int64_t scratch[16];
+    __shared__ ListScratch scratch;
     __shared__ float ml[kWarps][2], rows[kWarps][D];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.y;
     // every block waits, also one with nothing to do: this grid must not end before the one whose partials it stands for
     auto wait = [] { asm volatile("griddepcontrol.wait;" ::: "memory"); };
-    const int64_t total = total_units(p, scratch);
-    const int n = used_ctas(total, gridDim.x), cta = blockIdx.x;
+    const int cta = blockIdx.x;
+    const Found list = find_in_list(p, &scratch, [&](int64_t total) {
+        const int n = used_ctas(total, gridDim.x);
+        return cta < n - 1 ? cta_begin(total, n, cta + 1) - 1 : -1;
+    });
+    const int64_t total = list.total;
+    const int n = used_ctas(total, gridDim.x);
     if (cta >= n - 1) { wait(); return; }
     const int64_t begin = cta_begin(total, n, cta), end = cta_begin(total, n, cta + 1);
-    const Place last = find_place(p, end - 1, reinterpret_cast<Place*>(scratch));
+    const Place last = list.place;
     const int64_t item_begin = end - 1 - last.unit, item_end = item_begin + last.r.units;
     const int head = last.item / last.r.row_tiles, r = (last.item % last.r.row_tiles) * kRows + row;
     const int last_cta = cta_of(total, n, item_end - 1);
