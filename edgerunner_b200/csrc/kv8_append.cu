@@ -264,25 +264,42 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const __grid_constant__
     const int wpp = sb / kWarpRows, groups = static_cast<int>(blockDim.x >> 5) / wpp, group = warp / wpp;    // warps per pair, pairs at a time
     const int pairs = 2 * c.num_kv_heads;
     const int row0 = (warp % wpp) * kWarpRows, sub = lane / kLanes, vector = lane % kLanes, first = vector * VEC;
+    // Where a warp's side lives.  With several pairs at a time the even groups take keys, the odd ones values, and this is worked out once.
+    int side;
+    const T* in_rows;              // of head 0: this lane's vector of its first row
+    int64_t in_head, in_pass;
+    uint8_t* code_rows;
+    float* scale_row;
+    auto take_side = [&](int s) {
+        side = s;
+        const int64_t token = s ? p.in_token[1] : p.in_token[0];
+        in_head = s ? p.in_head[1] : p.in_head[0];
+        in_rows = static_cast<const T*>(s ? p.in[1] : p.in[0]) + (token0 + row0 + sub) * token + first;
+        in_pass = kRowsPerPass * token;
+        code_rows = (s ? c.codes[1] : c.codes[0]) + (block_row + row0 + sub) * D + first;
+        scale_row = (s ? c.scales[1] : c.scales[0]) + kv8_scale_at(c, block_row);
+    };
+    take_side(group & 1);
+    const int scale_head = c.page_size >> c.scale_shift;                 // scales of a head in a page
+    const int64_t code_head = static_cast<int64_t>(c.page_size) * D;
+    bool is_new[kPasses];
+#pragma unroll
+    for (int ps = 0; ps < kPasses; ++ps) is_new[ps] = row0 + ps * kRowsPerPass + sub >= lead && row0 + ps * kRowsPerPass + sub < end;
     uint4 va[kPasses], vb[kPasses];
     float old = 0.f;
-    // keys and values take turns in a warp, keys cost more: pairs 2 m, 2 m + 1 are the sides of a head, swapped every other time round
-    auto side_of = [&](int it, int pr) { return groups > 1 ? (pr ^ it) & 1 : pr & 1; };
     auto load = [&](int it) {
-        const int pr = it * groups + group, side = side_of(it, pr), head = pr >> 1;
-        const T* base = static_cast<const T*>(side ? p.in[1] : p.in[0]) + head * (side ? p.in_head[1] : p.in_head[0]) + first;
-        const int64_t token = side ? p.in_token[1] : p.in_token[0];
+        const int pr = it * groups + group, head = pr >> 1;
+        if (groups == 1) take_side(pr & 1);
+        const T* src = in_rows + head * in_head;
 #pragma unroll
         for (int ps = 0; ps < kPasses; ++ps) {
-            const int row = row0 + ps * kRowsPerPass + sub;
             va[ps] = vb[ps] = make_uint4(0, 0, 0, 0);
-            if (pr < pairs && row >= lead && row < end) {
-                const T* src = base + (token0 + row) * token;
-                va[ps] = __ldg(reinterpret_cast<const uint4*>(src));
-                vb[ps] = __ldg(reinterpret_cast<const uint4*>(src + HALF));
+            if (pr < pairs && is_new[ps]) {
+                va[ps] = __ldg(reinterpret_cast<const uint4*>(src + ps * in_pass));
+                vb[ps] = __ldg(reinterpret_cast<const uint4*>(src + ps * in_pass + HALF));
             }
         }
-        if (pr < pairs && lead > 0) old = (side ? c.scales[1] : c.scales[0])[kv8_scale_at(c, block_row + static_cast<int64_t>(head) * c.page_size)];
+        if (pr < pairs && lead > 0) old = scale_row[head * scale_head];
     };
     const int its = (pairs + groups - 1) / groups;
     int it = blockIdx.y;
@@ -306,7 +323,9 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const __grid_constant__
     __syncthreads();
 #pragma unroll 1
     for (int turn = 0; it < its; it += gridDim.y, turn ^= 1) {         // uniform over the CTA
-        const int pr = it * groups + group, side = side_of(it, pr), head = pr >> 1;
+        const int pr = it * groups + group, head = pr >> 1, now = side;
+        uint8_t* const dst = code_rows + head * code_head;
+        float* const scale_at = scale_row + head * scale_head;
         float a[kPasses][VEC], b[kPasses][VEC];
 #pragma unroll
         for (int ps = 0; ps < kPasses; ++ps) {
@@ -320,7 +339,7 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const __grid_constant__
 #pragma unroll
         for (int ps = 0; ps < kPasses; ++ps) {
             factor[ps] = 1.f;
-            if (side == 0) {                                               // uniform over a warp
+            if (now == 0) {                                                // uniform over a warp
                 if (p.weight != nullptr) {
                     float ss = 0.f;
 #pragma unroll
@@ -352,13 +371,10 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const __grid_constant__
             const float inv = reciprocal_scale<E4M3>(scale);
             const bool grown = lead > 0 && scale > before;
             const float ratio = grown ? __fdiv_rn(before, scale) : 1.f;
-            const int64_t at = block_row + static_cast<int64_t>(head) * c.page_size;
-            uint8_t* dst = (side ? c.codes[1] : c.codes[0]) + at * D + first;
 #pragma unroll
             for (int ps = 0; ps < kPasses; ++ps) {
-                const int row = row0 + ps * kRowsPerPass + sub;
-                uint8_t* d = dst + row * D;
-                if (row >= lead && row < end) {
+                uint8_t* d = dst + ps * kRowsPerPass * D;
+                if (is_new[ps]) {
                     const float f = factor[ps] * inv;
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) { a[ps][i] *= f; b[ps][i] *= f; }
@@ -366,7 +382,7 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const __grid_constant__
 #pragma unroll
                         for (int i = 0; i < VEC; ++i) a[ps][i] = b[ps][i] = 0.f;
                     }
-                } else if (row < lead && grown) {
+                } else if (grown && row0 + ps * kRowsPerPass + sub < lead) {
 #pragma unroll
                     for (int i = 0; i < VEC; i += 4) {
                         decode4f<E4M3>(*reinterpret_cast<const uint32_t*>(d + i), a[ps] + i);
@@ -391,7 +407,7 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const __grid_constant__
                     *reinterpret_cast<uint32_t*>(d + HALF) = hi[0];
                 }
             }
-            if (row0 == 0 && lane == 0) (side ? c.scales[1] : c.scales[0])[kv8_scale_at(c, at)] = scale;
+            if (row0 == 0 && lane == 0) *scale_at = scale;
         }
     }
 }
