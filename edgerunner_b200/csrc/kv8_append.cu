@@ -370,34 +370,12 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const __grid_constant__
             const float scale = (before >= need) ? before : (isnan(before) ? before : need);  // a NaN on either side stays
             const float inv = reciprocal_scale<E4M3>(scale);
             const bool grown = lead > 0 && scale > before;
-            const float ratio = grown ? __fdiv_rn(before, scale) : 1.f;
-#pragma unroll
-            for (int ps = 0; ps < kPasses; ++ps) {
-                uint8_t* d = dst + ps * kRowsPerPass * D;
-                if (is_new[ps]) {
-                    const float f = factor[ps] * inv;
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) { a[ps][i] *= f; b[ps][i] *= f; }
-                    if (!(inv > 0.f)) {                                     // zeros, or a NaN scale: codes of zeros
-#pragma unroll
-                        for (int i = 0; i < VEC; ++i) a[ps][i] = b[ps][i] = 0.f;
-                    }
-                } else if (grown && row0 + ps * kRowsPerPass + sub < lead) {
-#pragma unroll
-                    for (int i = 0; i < VEC; i += 4) {
-                        decode4f<E4M3>(*reinterpret_cast<const uint32_t*>(d + i), a[ps] + i);
-                        decode4f<E4M3>(*reinterpret_cast<const uint32_t*>(d + HALF + i), b[ps] + i);
-                    }
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) { a[ps][i] *= ratio; b[ps][i] *= ratio; }
-                } else {
-                    continue;
-                }
+            auto store = [&](uint8_t* d, const float* x, const float* y) {
                 uint32_t lo[VEC / 4], hi[VEC / 4];
 #pragma unroll
                 for (int i = 0; i < VEC; i += 4) {
-                    lo[i / 4] = encode4<E4M3>(a[ps][i], a[ps][i + 1], a[ps][i + 2], a[ps][i + 3]);
-                    hi[i / 4] = encode4<E4M3>(b[ps][i], b[ps][i + 1], b[ps][i + 2], b[ps][i + 3]);
+                    lo[i / 4] = encode4<E4M3>(x[i], x[i + 1], x[i + 2], x[i + 3]);
+                    hi[i / 4] = encode4<E4M3>(y[i], y[i + 1], y[i + 2], y[i + 3]);
                 }
                 if constexpr (VEC == 8) {
                     *reinterpret_cast<uint2*>(d) = make_uint2(lo[0], lo[1]);
@@ -405,6 +383,37 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const __grid_constant__
                 } else {
                     *reinterpret_cast<uint32_t*>(d) = lo[0];
                     *reinterpret_cast<uint32_t*>(d + HALF) = hi[0];
+                }
+            };
+            if (grown && row0 < lead) {                                     // the earlier rows' codes; a loop of its own, since few blocks come here
+                const float ratio = __fdiv_rn(before, scale);
+#pragma unroll 1
+                for (int r = sub; r < min(kWarpRows, lead - row0); r += kRowsPerPass) {
+                    uint8_t* d = dst + (r - sub) * D;
+                    float x[VEC], y[VEC];
+#pragma unroll
+                    for (int i = 0; i < VEC; i += 4) {
+                        decode4f<E4M3>(*reinterpret_cast<const uint32_t*>(d + i), x + i);
+                        decode4f<E4M3>(*reinterpret_cast<const uint32_t*>(d + HALF + i), y + i);
+                    }
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) { x[i] *= ratio; y[i] *= ratio; }
+                    store(d, x, y);
+                }
+            }
+            if (!(inv > 0.f)) {                                             // zeros, or a NaN scale: codes of zeros
+#pragma unroll
+                for (int ps = 0; ps < kPasses; ++ps)
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) a[ps][i] = b[ps][i] = 0.f;
+            }
+#pragma unroll
+            for (int ps = 0; ps < kPasses; ++ps) {
+                if (is_new[ps]) {
+                    const float f = inv > 0.f ? factor[ps] * inv : 0.f;
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) { a[ps][i] *= f; b[ps][i] *= f; }
+                    store(dst + ps * kRowsPerPass * D, a[ps], b[ps]);
                 }
             }
             if (row0 == 0 && lane == 0) *scale_at = scale;
