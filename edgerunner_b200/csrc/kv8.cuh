@@ -61,6 +61,60 @@ __device__ __forceinline__ void store_pair(float* p, float a, float b) { *reinte
 __device__ __forceinline__ void store_pair(__half* p, float a, float b) { *reinterpret_cast<__half2*>(p) = __floats2half2_rn(a, b); }
 __device__ __forceinline__ void store_pair(__nv_bfloat16* p, float a, float b) { *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b); }
 
+// Two float32 lanes in one instruction.
+struct F2 {
+    uint64_t v;
+};
+__device__ __forceinline__ F2 pack2(float a, float b) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(F2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+// A lane's pairs (a[i], b[i]) turned by the angles with cosines c[i] and sines s[i].
+template <int VEC>
+__device__ __forceinline__ void turn2(F2 (&a)[VEC / 2], F2 (&b)[VEC / 2], int i, F2 c, F2 s) {
+    const F2 x = a[i], y = b[i], minus = pack2(-1.f, -1.f);
+    a[i] = fma2(mul2(y, minus), s, mul2(x, c));
+    b[i] = fma2(x, s, mul2(y, c));
+}
+template <int VEC>
+__device__ __forceinline__ float square_sum(const F2 (&a)[VEC / 2], const F2 (&b)[VEC / 2]) {
+    F2 x = pack2(0.f, 0.f), y = x;
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) { x = fma2(a[i], a[i], x); y = fma2(b[i], b[i], y); }
+    float u, v;
+    unpack2(add2(x, y), u, v);
+    return u + v;
+}
+template <typename T>
+__device__ __forceinline__ void unpack_pairs(const uint4& v, F2 (&x)[Act<T>::kVec / 2]) {
+    float f[Act<T>::kVec];
+    Act<T>::unpack(v, f);
+#pragma unroll
+    for (int i = 0; i < Act<T>::kVec / 2; ++i) x[i] = pack2(f[2 * i], f[2 * i + 1]);
+}
+template <int N>
+__device__ __forceinline__ void floats_of(const F2 (&x)[N], float* f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) unpack2(x[i], f[2 * i], f[2 * i + 1]);
+}
+
 // ---- codes ----
 // Four values (already divided by the scale) -> four codes, the first in the low byte.  Rounded to nearest even, saturating.
 template <bool E4M3>

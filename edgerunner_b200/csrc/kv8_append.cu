@@ -82,22 +82,20 @@ struct NormRope {
     double log2_theta, inv_scaling;
 };
 
-// Place of pair `pair` in a table of `vectors` lanes of VEC pairs: the i-th two pairs of all lanes lie side by side.
-template <int VEC> __host__ __device__ __forceinline__ int turn_place(int pair, int vectors) {
-    return (((pair % VEC) >> 1) * vectors + pair / VEC) * 2 + (pair & 1);
-}
-// A lane's pairs of a row, turned; `turns`: the token's table at the lane's vector, pairs from `rotated` on stay.
+// A table of turns: the i-th two pairs of all `vectors` lanes of VEC pairs lie side by side, (cos, cos, sin, sin) in 16 bytes.
 template <int VEC>
-__device__ __forceinline__ void rotate(float (&a)[VEC], float (&b)[VEC], int first, int rotated, int vectors, const float2* turns) {
-    if (first >= rotated) return;
+__device__ __forceinline__ void put_turn(float* table, int pair, int vectors, float2 turn) {
+    float* at = table + (((pair % VEC) >> 1) * vectors + pair / VEC) * 4 + (pair & 1);
+    at[0] = turn.x;
+    at[2] = turn.y;
+}
+// A lane's pairs of a row, turned; `turns`: the token's table at the lane's vector.
+template <int VEC>
+__device__ __forceinline__ void rotate(F2 (&a)[VEC / 2], F2 (&b)[VEC / 2], int vectors, const float* turns) {
 #pragma unroll
-    for (int i = 0; i < VEC; i += 2) {
-        const float4 cs = *reinterpret_cast<const float4*>(turns + i * vectors);
-        const float x0 = a[i], y0 = b[i], x1 = a[i + 1], y1 = b[i + 1];
-        a[i] = x0 * cs.x - y0 * cs.y;
-        b[i] = x0 * cs.y + y0 * cs.x;
-        a[i + 1] = x1 * cs.z - y1 * cs.w;
-        b[i + 1] = x1 * cs.w + y1 * cs.z;
+    for (int i = 0; i < VEC / 2; ++i) {
+        const float4 cs = *reinterpret_cast<const float4*>(turns + i * vectors * 4);
+        turn2<VEC>(a, b, i, pack2(cs.x, cs.y), pack2(cs.z, cs.w));
     }
 }
 __device__ __forceinline__ void make_frequencies(double* frequencies, int rotated, int half, double log2_theta, double inv_scaling) {
@@ -113,7 +111,7 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const __grid_con
     const float inv_dim = 1.f / static_cast<float>(p.head_dim);
     const int half = p.head_dim >> 1, vectors = half / VEC, table = half;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    float2* turns = reinterpret_cast<float2*>(shared8 + ((p.rotated + 1) & ~1)) + warp * table;
+    float* turns = reinterpret_cast<float*>(shared8 + ((p.rotated + 1) & ~1)) + warp * 2 * table;
     const int rows_per_warp = 32 / p.lanes, sub = lane / p.lanes, vector = lane & (p.lanes - 1), first = vector * VEC;
     const bool own = first < half;
     make_frequencies(shared8, p.rotated, half, p.log2_theta, p.inv_scaling);
@@ -123,29 +121,34 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const __grid_con
         if (p.rotated > 0) {
             const int position = __ldg(p.positions + t);
             __syncwarp();                                          // the last token's table has been read
-            for (int i = lane; i < half; i += 32) turns[turn_place<VEC>(i, vectors)] = i < p.rotated ? rope_turn(position, shared8[i]) : make_float2(1.f, 0.f);
+            for (int i = lane; i < half; i += 32) put_turn<VEC>(turns, i, vectors, i < p.rotated ? rope_turn(position, shared8[i]) : make_float2(1.f, 0.f));
             __syncwarp();
         }
-        float cs[2 * VEC];                                          // cos, sin of the lane's pairs
-        if (own && first < p.rotated) {
+        F2 c2[VEC / 2], s2[VEC / 2];                               // cos, sin of the lane's pairs
 #pragma unroll
-            for (int i = 0; i < VEC; i += 2) *reinterpret_cast<float4*>(cs + 2 * i) = *reinterpret_cast<const float4*>(turns + vector * 2 + i * vectors);
-        } else {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) { cs[2 * i] = 1.f; cs[2 * i + 1] = 0.f; }
+        for (int i = 0; i < VEC / 2; ++i) {
+            float4 cs = make_float4(1.f, 1.f, 0.f, 0.f);
+            if (own && p.rotated > 0) cs = *reinterpret_cast<const float4*>(turns + (i * vectors + vector) * 4);
+            c2[i] = pack2(cs.x, cs.y);
+            s2[i] = pack2(cs.z, cs.w);
         }
 #pragma unroll 1
         for (int side = 0; side < 2; ++side) {
             const int heads = side ? p.heads[1] : p.heads[0];
             const float* w = side ? p.weight[1] : p.weight[0];
-            float ca[VEC], sa[VEC], cb[VEC], sb[VEC];              // ... times the weights of the two members
+            F2 ca[VEC / 2], sa[VEC / 2], cb[VEC / 2], sb[VEC / 2];  // ... times the weights of the two members, sb negated
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const float wa = own && w != nullptr ? __ldg(w + first + i) : 1.f, wb = own && w != nullptr ? __ldg(w + half + first + i) : 1.f;
-                ca[i] = cs[2 * i] * wa;
-                sa[i] = cs[2 * i + 1] * wa;
-                cb[i] = cs[2 * i] * wb;
-                sb[i] = cs[2 * i + 1] * wb;
+            for (int i = 0; i < VEC / 2; ++i) {
+                F2 wa = pack2(1.f, 1.f), wb = wa;
+                if (own && w != nullptr) {
+                    const float2 x = __ldg(reinterpret_cast<const float2*>(w + first) + i), y = __ldg(reinterpret_cast<const float2*>(w + half + first) + i);
+                    wa = pack2(x.x, x.y);
+                    wb = pack2(y.x, y.y);
+                }
+                ca[i] = mul2(c2[i], wa);
+                sa[i] = mul2(s2[i], wa);
+                cb[i] = mul2(c2[i], wb);
+                sb[i] = mul2(mul2(s2[i], wb), pack2(-1.f, -1.f));
             }
             const int64_t in_head = side ? p.in_head[1] : p.in_head[0], out_head = side ? p.out_head[1] : p.out_head[0];
             const T* src = static_cast<const T*>(side ? p.in[1] : p.in[0]) + t * (side ? p.in_token[1] : p.in_token[0]) + first;
@@ -165,27 +168,29 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const __grid_con
 #pragma unroll
                 for (int k = 0; k < kBatch; ++k) {
                     const int h = h0 + k * step;
-                    float a[VEC], b[VEC];
-                    Act<T>::unpack(va[k], a);
-                    Act<T>::unpack(vb[k], b);
+                    F2 a[VEC / 2], b[VEC / 2];
+                    unpack_pairs<T>(va[k], a);
+                    unpack_pairs<T>(vb[k], b);
                     if (w != nullptr) {
-                        float ss = 0.f;
-#pragma unroll
-                        for (int i = 0; i < VEC; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
+                        float ss = square_sum<VEC>(a, b);
                         for (int off = p.lanes >> 1; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
                         const float f = rsqrtf(ss * inv_dim + p.eps);
+                        const F2 f2 = pack2(f, f);
 #pragma unroll
-                        for (int i = 0; i < VEC; ++i) { a[i] *= f; b[i] *= f; }
+                        for (int i = 0; i < VEC / 2; ++i) { a[i] = mul2(a[i], f2); b[i] = mul2(b[i], f2); }
                     }
                     if (own && h < heads) {
+                        float x[VEC], y[VEC];
 #pragma unroll
-                        for (int i = 0; i < VEC; ++i) {
-                            const float x = a[i], y = b[i];
-                            a[i] = x * ca[i] - y * sb[i];
-                            b[i] = x * sa[i] + y * cb[i];
+                        for (int i = 0; i < VEC / 2; ++i) {
+                            const F2 u = a[i];
+                            a[i] = fma2(u, ca[i], mul2(b[i], sb[i]));
+                            b[i] = fma2(u, sa[i], mul2(b[i], cb[i]));
                         }
-                        *reinterpret_cast<uint4*>(dst + h * out_head) = Act<T>::pack(a);
-                        *reinterpret_cast<uint4*>(dst + h * out_head + half) = Act<T>::pack(b);
+                        floats_of(a, x);
+                        floats_of(b, y);
+                        *reinterpret_cast<uint4*>(dst + h * out_head) = Act<T>::pack(x);
+                        *reinterpret_cast<uint4*>(dst + h * out_head + half) = Act<T>::pack(y);
                     }
                 }
             }
@@ -216,7 +221,7 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {   // a Na
 // scale, not the elements.  blockIdx.x numbers the blocks a sequence can touch (kv8_find_slot): sequence s owns the numbers from
 // starts[s] / scale_block + 2 s on, always enough for a run of tokens that begins and ends inside a block; the rest return at once.  blockIdx.y spreads
 // the pairs over more CTAs when there are few blocks.
-constexpr int kWarpRows = 8;
+constexpr int kWarpRows = 8, kAppendSlots = 2;
 __device__ __forceinline__ float min3_nan(float a, float b, float c) {
     float r;
     asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -224,11 +229,11 @@ __device__ __forceinline__ float min3_nan(float a, float b, float c) {
 }
 template <typename T, int D, bool E4M3>
 __global__ void __launch_bounds__(512) kv8_append_kernel(const __grid_constant__ Kv8Append p) {
-    extern __shared__ double shared8[];        // frequencies [rotated], turns [scale_block][D / 2]
+    extern __shared__ double shared8[];        // frequencies [rotated], turns [scale_block][D / 2], rings of the warps
     __shared__ float warp_max[2][16];
     constexpr int VEC = Act<T>::kVec, HALF = D / 2;
     constexpr int kLanes = HALF / VEC, kRowsPerPass = 32 / kLanes, kPasses = kWarpRows / kRowsPerPass;
-    float2* turns = reinterpret_cast<float2*>(shared8 + HALF);
+    float* turns = reinterpret_cast<float*>(shared8 + HALF);
     const Kv8Cache& c = p.cache;
     const int sb = c.scale_block;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -285,55 +290,66 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const __grid_constant__
     bool is_new[kPasses];
 #pragma unroll
     for (int ps = 0; ps < kPasses; ++ps) is_new[ps] = row0 + ps * kRowsPerPass + sub >= lead && row0 + ps * kRowsPerPass + sub < end;
-    uint4 va[kPasses], vb[kPasses];
-    float old = 0.f;
-    auto load = [&](int it) {
-        const int pr = it * groups + group, head = pr >> 1;
-        if (groups == 1) take_side(pr & 1);
-        const T* src = in_rows + head * in_head;
+    // A warp's rows come through its own ring in shared memory, the next pair's while this one is worked on (deeper rings measured the same,
+    // registers are short); a lane reads what it copied, so no barrier is needed.
+    uint4* ring = reinterpret_cast<uint4*>(turns + sb * D) + warp * (kAppendSlots * kPasses * 2 * 32) + lane;
+    auto fetch = [&](int it, int slot) {           // one group, empty behind the last pair
+        const int pr = it * groups + group;
+        if (pr < pairs) {
+            if (groups == 1) take_side(pr & 1);
+            const T* src = in_rows + (pr >> 1) * in_head;
+            const uint32_t to = smem_u32(ring + slot * (kPasses * 2 * 32));
 #pragma unroll
-        for (int ps = 0; ps < kPasses; ++ps) {
-            va[ps] = vb[ps] = make_uint4(0, 0, 0, 0);
-            if (pr < pairs && is_new[ps]) {
-                va[ps] = __ldg(reinterpret_cast<const uint4*>(src + ps * in_pass));
-                vb[ps] = __ldg(reinterpret_cast<const uint4*>(src + ps * in_pass + HALF));
+            for (int ps = 0; ps < kPasses; ++ps) {
+                if (is_new[ps]) {
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + ps * 1024), "l"(src + ps * in_pass) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + ps * 1024 + 512), "l"(src + ps * in_pass + HALF) : "memory");
+                }
             }
         }
-        if (pr < pairs && lead > 0) old = scale_row[head * scale_head];
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
     const int its = (pairs + groups - 1) / groups;
     int it = blockIdx.y;
-    load(it);
+#pragma unroll
+    for (int k = 0; k < kAppendSlots - 1; ++k) fetch(it + k * gridDim.y, k);
     if (p.rotated > 0) {
         make_frequencies(shared8, p.rotated, HALF, p.log2_theta, p.inv_scaling);
         __syncthreads();
         for (int e = threadIdx.x; e < (end - lead) * HALF; e += blockDim.x) {
             const int t = e / HALF, pair = e % HALF;
-            turns[t * HALF + turn_place<VEC>(pair, kLanes)] = pair < p.rotated ? rope_turn(block_pos + lead + t, shared8[pair]) : make_float2(1.f, 0.f);
+            put_turn<VEC>(turns + t * D, pair, kLanes, pair < p.rotated ? rope_turn(block_pos + lead + t, shared8[pair]) : make_float2(1.f, 0.f));
         }
     }
-    float wa[VEC], wb[VEC];
+    F2 wa[VEC / 2], wb[VEC / 2];
     if (p.weight != nullptr) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            wa[i] = __ldg(p.weight + first + i);
-            wb[i] = __ldg(p.weight + HALF + first + i);
+        for (int i = 0; i < VEC / 2; ++i) {
+            const float2 x = __ldg(reinterpret_cast<const float2*>(p.weight + first) + i), y = __ldg(reinterpret_cast<const float2*>(p.weight + HALF + first) + i);
+            wa[i] = pack2(x.x, x.y);
+            wb[i] = pack2(y.x, y.y);
         }
     }
     __syncthreads();
 #pragma unroll 1
-    for (int turn = 0; it < its; it += gridDim.y, turn ^= 1) {         // uniform over the CTA
-        const int pr = it * groups + group, head = pr >> 1, now = side;
+    for (int turn = 0, slot = 0; it < its; it += gridDim.y, turn ^= 1) {         // uniform over the CTA
+        const int pr = it * groups + group, head = pr >> 1;
+        if (groups == 1) take_side(pr & 1);
+        const int now = side;
         uint8_t* const dst = code_rows + head * code_head;
         float* const scale_at = scale_row + head * scale_head;
-        float a[kPasses][VEC], b[kPasses][VEC];
+        const float before = lead > 0 && pr < pairs ? *scale_at : 0.f;
+        F2 a[kPasses][VEC / 2], b[kPasses][VEC / 2];
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAppendSlots - 2) : "memory");
 #pragma unroll
         for (int ps = 0; ps < kPasses; ++ps) {
-            Act<T>::unpack(va[ps], a[ps]);
-            Act<T>::unpack(vb[ps], b[ps]);
+            const bool on = is_new[ps] && pr < pairs;
+            const uint4 zero = make_uint4(0, 0, 0, 0);
+            unpack_pairs<T>(on ? ring[(slot * kPasses + ps) * 64] : zero, a[ps]);
+            unpack_pairs<T>(on ? ring[(slot * kPasses + ps) * 64 + 32] : zero, b[ps]);
         }
-        const float before = lead > 0 ? old : 0.f;
-        if (it + static_cast<int>(gridDim.y) < its) load(it + gridDim.y);
+        fetch(it + (kAppendSlots - 1) * gridDim.y, slot == 0 ? kAppendSlots - 1 : slot - 1);
+        slot = slot + 1 == kAppendSlots ? 0 : slot + 1;
         // ---- norm, rotation, the largest magnitude ----
         float factor[kPasses], mx = 0.f;
 #pragma unroll
@@ -341,23 +357,26 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const __grid_constant__
             factor[ps] = 1.f;
             if (now == 0) {                                                // uniform over a warp
                 if (p.weight != nullptr) {
-                    float ss = 0.f;
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) ss = fmaf(a[ps][i], a[ps][i], fmaf(b[ps][i], b[ps][i], ss));
+                    float ss = square_sum<VEC>(a[ps], b[ps]);
 #pragma unroll
                     for (int off = kLanes / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
                     factor[ps] = rsqrtf(ss * (1.f / D) + p.eps);
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) { a[ps][i] *= wa[i]; b[ps][i] *= wb[i]; }
+                    for (int i = 0; i < VEC / 2; ++i) { a[ps][i] = mul2(a[ps][i], wa[i]); b[ps][i] = mul2(b[ps][i], wb[i]); }
                 }
                 const int t = min(max(row0 + ps * kRowsPerPass + sub - lead, 0), end - lead - 1);    // rows of zeros turn by some token's angle
-                rotate<VEC>(a[ps], b[ps], first, p.rotated, kLanes, turns + t * HALF + vector * 2);
+                if (p.rotated > 0) rotate<VEC>(a[ps], b[ps], kLanes, turns + t * D + vector * 4);
             }
             float up = 0.f, down = 0.f;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                up = max3_nan(up, a[ps][i], b[ps][i]);
-                down = min3_nan(down, a[ps][i], b[ps][i]);
+            for (int i = 0; i < VEC / 2; ++i) {
+                float x, y;
+                unpack2(a[ps][i], x, y);
+                up = max3_nan(up, x, y);
+                down = min3_nan(down, x, y);
+                unpack2(b[ps][i], x, y);
+                up = max3_nan(up, x, y);
+                down = min3_nan(down, x, y);
             }
             mx = max3_nan(mx, up * factor[ps], -down * factor[ps]);
         }
@@ -401,19 +420,21 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const __grid_constant__
                     store(d, x, y);
                 }
             }
-            if (!(inv > 0.f)) {                                             // zeros, or a NaN scale: codes of zeros
-#pragma unroll
-                for (int ps = 0; ps < kPasses; ++ps)
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) a[ps][i] = b[ps][i] = 0.f;
-            }
 #pragma unroll
             for (int ps = 0; ps < kPasses; ++ps) {
                 if (is_new[ps]) {
-                    const float f = inv > 0.f ? factor[ps] * inv : 0.f;
+                    const float f = factor[ps] * inv;
+                    const F2 f2 = pack2(f, f);
+                    float x[VEC], y[VEC];
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) { a[ps][i] *= f; b[ps][i] *= f; }
-                    store(dst + ps * kRowsPerPass * D, a[ps], b[ps]);
+                    for (int i = 0; i < VEC / 2; ++i) { a[ps][i] = mul2(a[ps][i], f2); b[ps][i] = mul2(b[ps][i], f2); }
+                    floats_of(a[ps], x);
+                    floats_of(b[ps], y);
+                    if (!(inv > 0.f)) {                                     // zeros, or a NaN scale: codes of zeros
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) x[i] = y[i] = 0.f;
+                    }
+                    store(dst + ps * kRowsPerPass * D, x, y);
                 }
             }
             if (row0 == 0 && lane == 0) *scale_at = scale;
@@ -460,7 +481,7 @@ int32_t launch_append(const Kv8Append& p, cudaStream_t s) {
     const int threads = sb == 128 ? 512 : 256;
     const int groups = threads / 32 / (sb / kWarpRows), steps = (2 * p.cache.num_kv_heads + groups - 1) / groups;
     const dim3 grid(blocks, blocks >= 592 ? 1 : steps);   // 592: four CTAs' worth of blocks for each SM
-    const size_t smem = D / 2 * sizeof(double) + static_cast<size_t>(sb) * (D / 2) * sizeof(float2);   // up to 64.5 KB
+    const size_t smem = D / 2 * sizeof(double) + static_cast<size_t>(sb) * (D / 2) * sizeof(float2) + threads / 32 * kAppendSlots * kWarpRows * D * sizeof(T);
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kv8_append_kernel<T, D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
         if (e != cudaSuccess) return kv8_launched(e, "kv8_append_kernel");
