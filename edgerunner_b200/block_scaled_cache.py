@@ -35,7 +35,10 @@ def _types():
 
 
 def _stream(stream, index):
-    return _torch.cuda.current_stream(index).cuda_stream if stream is None else stream_ptr(stream)
+    if stream is not None:
+        return stream_ptr(stream)
+    raw = getattr(_torch._C, "_cuda_getCurrentRawStream", None)      # the same without a Stream object
+    return raw(index) if raw is not None else _torch.cuda.current_stream(index).cuda_stream
 
 
 def _call(fn, index, *args):

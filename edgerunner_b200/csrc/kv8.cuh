@@ -7,6 +7,7 @@
 
 #include <cuda_bf16.h>
 
+#include <atomic>
 #include <cmath>
 
 #include "../../include/er_kv.h"
@@ -251,6 +252,16 @@ int32_t kv8_check_attention(const er_kv8_cache* c, const er_kv8_attention_params
 int32_t kv8_check_workspace(const er_kv8_attention_params* u, int64_t need);
 int64_t kv8_decode_workspace(const er_kv8_cache* c, const er_kv8_attention_params* u, bool ragged);
 int32_t kv8_launch_decode(const Kv8Cache& cache, const er_kv8_cache* c, const er_kv8_attention_params* u, bool ragged, int few_rows, cudaStream_t s);
+// Dynamic shared memory beyond 48 KB has to be allowed once for each kernel and device.  `most`: the largest size that any call of the kernel asks for.
+template <typename Kernel>
+inline cudaError_t kv8_allow_smem(Kernel kernel, int most, std::atomic<uint64_t>& devices) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess || (device < 64 && (devices.load(std::memory_order_acquire) >> device & 1u) != 0)) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (e == cudaSuccess && device < 64) devices.fetch_or(1ull << device, std::memory_order_release);
+    return e;
+}
 inline float kv8_scale_log2(float softmax_scale, uint32_t head_dim) {       // scores in units of log2
     return (softmax_scale > 0.f ? softmax_scale : 1.f / std::sqrt(static_cast<float>(head_dim))) * 1.4426950408889634f;
 }

@@ -483,7 +483,10 @@ int32_t launch_append(const Kv8Append& p, cudaStream_t s) {
     const dim3 grid(blocks, blocks >= 592 ? 1 : steps);   // 592: four CTAs' worth of blocks for each SM
     const size_t smem = D / 2 * sizeof(double) + static_cast<size_t>(sb) * (D / 2) * sizeof(float2) + threads / 32 * kAppendSlots * kWarpRows * D * sizeof(T);
     if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kv8_append_kernel<T, D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        constexpr int kMost = D / 2 * 8 + 128 * (D / 2) * 8 + 16 * kAppendSlots * kWarpRows * D * static_cast<int>(sizeof(T));
+        static_assert(kMost <= 232448, "append kernel exceeds the shared memory of an sm_100 CTA");
+        static std::atomic<uint64_t> devices{0};
+        const cudaError_t e = kv8_allow_smem(kv8_append_kernel<T, D, E4M3>, kMost, devices);
         if (e != cudaSuccess) return kv8_launched(e, "kv8_append_kernel");
     }
     kv8_append_kernel<T, D, E4M3><<<grid, threads, smem, s>>>(p);

@@ -769,7 +769,8 @@ int32_t launch(Kv8Decode& p, int most_rows, int sms, cudaStream_t s) {
     constexpr int kSmem = decode_smem<T, D, NT>();
     static_assert(kSmem <= 232448, "decode kernel exceeds the shared memory of an sm_100 CTA");
     p.tile_rows = 8 * NT;
-    cudaError_t e = cudaFuncSetAttribute(kv8_decode_kernel<T, D, E4M3, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    static std::atomic<uint64_t> devices{0};
+    cudaError_t e = kv8_allow_smem(kv8_decode_kernel<T, D, E4M3, NT>, kSmem, devices);
     if (e != cudaSuccess) return kv8_launched(e, "kv8_decode_kernel");
     kv8_decode_kernel<T, D, E4M3, NT><<<sms, decode_warps<T, NT>() * 32, kSmem, s>>>(p);
     const int32_t rc = kv8_launched(cudaGetLastError(), "kv8_decode_kernel");

@@ -646,7 +646,8 @@ template <typename T, int D, bool E4M3>
 int32_t launch(const Kv8Prefill& p, const Plan& pl, cudaStream_t s) {
     constexpr int kSmem = prefill_smem<D>();
     static_assert(kSmem <= 232448, "prefill kernel exceeds the shared memory of an sm_100 CTA");
-    const cudaError_t e = cudaFuncSetAttribute(kv8_prefill_kernel<T, D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    static std::atomic<uint64_t> devices{0};
+    const cudaError_t e = kv8_allow_smem(kv8_prefill_kernel<T, D, E4M3>, kSmem, devices);
     if (e != cudaSuccess) return kv8_launched(e, "kv8_prefill_kernel");
     kv8_prefill_kernel<T, D, E4M3><<<pl.grid, kThreads, kSmem, s>>>(p);
     const int32_t rc = kv8_launched(cudaGetLastError(), "kv8_prefill_kernel");
