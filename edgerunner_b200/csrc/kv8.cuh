@@ -245,7 +245,7 @@ __device__ __forceinline__ float2 rope_turn(int position, double frequency) {
 int32_t report_error(int32_t code, const char* message);   // er_kv.cu: records the thread's last-error text
 void count_kernel_launch();                                 // er_kv.cu: bumps er_kernel_launch_count()
 int32_t kv8_check(const er_kv8_cache* cache, Kv8Cache* out);                // kv8_append.cu: the fields; fills the kernels' form
-int32_t kv8_check_device(const er_kv8_cache* cache);                         // the buffers are the current device's
+int32_t kv8_check_device(const void* buffer);                                // it is the current device's
 int32_t kv8_launched(cudaError_t e, const char* kernel);                     // status of the launch just made
 int kv8_sm_count();                                                          // kv8_decode.cu: SMs of the current device, 0 without one
 int32_t kv8_check_attention(const er_kv8_cache* c, const er_kv8_attention_params* u);
@@ -264,6 +264,14 @@ inline cudaError_t kv8_allow_smem(Kernel kernel, int most, std::atomic<uint64_t>
 }
 inline float kv8_scale_log2(float softmax_scale, uint32_t head_dim) {       // scores in units of log2
     return (softmax_scale > 0.f ? softmax_scale : 1.f / std::sqrt(static_cast<float>(head_dim))) * 1.4426950408889634f;
+}
+// Rows of an output do not overlap (heads beside each other inside a token, or tokens inside a head).
+inline bool kv8_rows_apart(int64_t token_stride, int64_t head_stride, int64_t tokens, int64_t heads, int64_t head_dim) {
+    if (tokens <= 1 && heads <= 1) return true;
+    if (heads <= 1) return token_stride >= head_dim;
+    if (tokens <= 1) return head_stride >= head_dim;
+    const bool heads_inside = head_stride >= head_dim && token_stride >= head_stride * (heads - 1) + head_dim;
+    return heads_inside || (token_stride >= head_dim && head_stride >= token_stride * (tokens - 1) + head_dim);
 }
 inline bool kv8_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

@@ -21,17 +21,17 @@ int32_t kv8_launched(cudaError_t e, const char* kernel) {
     return report_error(ER_ERR_CUDA, msg);
 }
 
-int32_t kv8_check_device(const er_kv8_cache* c) {
+int32_t kv8_check_device(const void* buffer) {
     int device = 0;
     cudaPointerAttributes at{};
     cudaError_t e = cudaGetDevice(&device);
-    if (e == cudaSuccess) e = cudaPointerGetAttributes(&at, c->keys);
+    if (e == cudaSuccess) e = cudaPointerGetAttributes(&at, buffer);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return report_error(ER_ERR_CUDA, cudaGetErrorString(e));
     }
-    if (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged) return report_error(ER_ERR_INVALID_ARGUMENT, "keys is not device memory");
-    if (at.device != device) return report_error(ER_ERR_INVALID_ARGUMENT, "the cache lives on another device than the current one");
+    if (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged) return report_error(ER_ERR_INVALID_ARGUMENT, "a buffer is not device memory");
+    if (at.device != device) return report_error(ER_ERR_INVALID_ARGUMENT, "the buffers live on another device than the current one");
     return ER_OK;
 }
 
@@ -44,8 +44,8 @@ int32_t kv8_check(const er_kv8_cache* c, Kv8Cache* out) {
         return report_error(ER_ERR_UNSUPPORTED, "scale_block must be 16, 32, 64 or 128");
     if (c->page_size == 0 || c->page_size % c->scale_block != 0 || c->page_size > (1u << 20))
         return report_error(ER_ERR_SHAPE, "page_size must be a multiple of scale_block (up to 2^20)");
-    if (c->num_pages == 0 || c->num_pages > 0x7FFFFFFFu || c->num_kv_heads == 0 || c->num_kv_heads > 65535u)
-        return report_error(ER_ERR_SHAPE, "num_pages and num_kv_heads must be positive (kv heads up to 65535)");
+    if (c->num_pages == 0 || c->num_pages > 0x7FFFFFFFu || c->num_kv_heads == 0 || c->num_kv_heads > 4096u)
+        return report_error(ER_ERR_SHAPE, "num_pages and num_kv_heads must be positive (kv heads up to 4096)");
     if (c->num_seqs > 65536u) return report_error(ER_ERR_UNSUPPORTED, "num_seqs beyond 65536");
     if (c->block_table_width > c->block_table_stride) return report_error(ER_ERR_SHAPE, "block_table_width exceeds block_table_stride");
     if (static_cast<uint64_t>(c->block_table_width) * c->page_size > 0x7FFFFF00ull)
@@ -518,6 +518,9 @@ extern "C" int32_t er_qk_norm_rope(const er_qk_norm_rope_params* u, void* stream
     const int64_t strides[8] = {u->q_token_stride, u->q_head_stride, u->q_out_token_stride, u->q_out_head_stride,
                                 u->k_token_stride, u->k_head_stride, u->k_out_token_stride, u->k_out_head_stride};
     if (!strides_ok(u->type, strides, u->k ? 8 : 4)) return report_error(ER_ERR_INVALID_ARGUMENT, "strides must be multiples of 16 bytes");
+    if (!kv8_rows_apart(u->q_out_token_stride, u->q_out_head_stride, u->num_tokens, u->num_heads, u->head_dim) ||
+        (u->k && !kv8_rows_apart(u->k_out_token_stride, u->k_out_head_stride, u->num_tokens, u->num_kv_heads, u->head_dim)))
+        return report_error(ER_ERR_SHAPE, "rows of an output overlap");
     NormRope p{};
     p.in[0] = u->q; p.in[1] = u->k; p.out[0] = u->q_out; p.out[1] = u->k_out;
     p.in_token[0] = u->q_token_stride; p.in_head[0] = u->q_head_stride; p.out_token[0] = u->q_out_token_stride; p.out_head[0] = u->q_out_head_stride;
@@ -532,6 +535,8 @@ extern "C" int32_t er_qk_norm_rope(const er_qk_norm_rope_params* u, void* stream
     p.log2_theta = p.rotated > 0 ? std::log2(static_cast<double>(u->rope_theta)) : 0.0;
     p.inv_scaling = p.rotated > 0 ? 1.0 / static_cast<double>(u->rope_scaling) : 0.0;
     if (u->num_tokens == 0) return ER_OK;
+    rc = kv8_check_device(u->q);
+    if (rc != ER_OK) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (u->type) {
         case ER_TYPE_FLOAT32: return launch_norm_rope<float>(p, s);
@@ -554,7 +559,7 @@ extern "C" int32_t er_kv8_append(const er_kv8_cache* cache, const er_kv8_append_
     if (!strides_ok(u->type, strides, 4)) return report_error(ER_ERR_INVALID_ARGUMENT, "strides must be multiples of 16 bytes");
     if (u->num_tokens > 0x7FFFFF00u) return report_error(ER_ERR_UNSUPPORTED, "num_tokens beyond 2^31");
     if (!u->query_starts && u->num_tokens != cache->num_seqs) return report_error(ER_ERR_SHAPE, "without query_starts num_tokens must be num_seqs");
-    rc = kv8_check_device(cache);
+    rc = kv8_check_device(cache->keys);
     if (rc != ER_OK) return rc;
     if (u->num_tokens == 0 || cache->num_seqs == 0) return ER_OK;
     p.in[0] = u->k; p.in[1] = u->v;

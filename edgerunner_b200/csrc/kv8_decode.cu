@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
     };
     int pstage = 0;
     auto produce = [&]() {          // the next unit, if there is one: lanes 0-15 see to half 0, 16-31 to half 1
-        if (pmore) {
+        if (pmore && !*abort_flag) {
             const int tok = pp.token(pu) + half * kKv8Unit;
             float* sc = my_scales + pstage * 4 + half * 2;
             const int64_t row = kv8_row(c, max(ppage, 0), pp.item / pp.r.row_tiles, kv8_in_page(c, tok));
@@ -813,6 +813,7 @@ int32_t kv8_check_attention(const er_kv8_cache* c, const er_kv8_attention_params
     const int64_t vec = u->type == ER_TYPE_FLOAT32 ? 4 : 8;
     for (const int64_t st : {u->q_token_stride, u->q_head_stride, u->out_token_stride, u->out_head_stride})
         if (st < 0 || st % vec != 0) return report_error(ER_ERR_INVALID_ARGUMENT, "strides must be multiples of 16 bytes");
+    if (!kv8_rows_apart(u->out_token_stride, u->out_head_stride, u->num_tokens, u->num_heads, c->head_dim)) return report_error(ER_ERR_SHAPE, "rows of out overlap");
     if (!(u->softmax_scale >= 0.f && std::isfinite(u->softmax_scale))) return report_error(ER_ERR_INVALID_ARGUMENT, "softmax_scale must be finite and not negative");
     if (u->num_tokens > 0x7FFFFF00u || u->sliding_window > 0x7FFFFFFFu) return report_error(ER_ERR_UNSUPPORTED, "num_tokens or sliding_window beyond 2^31");
     return ER_OK;
@@ -881,7 +882,7 @@ extern "C" int32_t er_kv8_attention_decode(const er_kv8_cache* cache, const er_k
     if (rc != ER_OK) return rc;
     if (u->query_len == 0 || u->query_len > 16) return report_error(ER_ERR_UNSUPPORTED, "query_len must be between 1 and 16 (longer runs: er_kv8_attention_prefill)");
     if (u->num_tokens != static_cast<uint64_t>(cache->num_seqs) * u->query_len) return report_error(ER_ERR_SHAPE, "num_tokens must be num_seqs * query_len");
-    rc = kv8_check_device(cache);
+    rc = kv8_check_device(cache->keys);
     if (rc == ER_OK) rc = kv8_check_workspace(u, kv8_decode_workspace(cache, u, false));
     if (rc != ER_OK || cache->num_seqs == 0) return rc;
     return kv8_launch_decode(c, cache, u, false, 0, static_cast<cudaStream_t>(stream));

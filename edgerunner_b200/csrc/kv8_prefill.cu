@@ -14,8 +14,9 @@
 //   warps 8-11, 13-15  fetch codes and write them as fp16 into the operand layout: a conversion in the loader reads 1 byte an element from L2
 //                    and serves 256 rows.
 //   warp 12          one lane issues the products: S_i = Q_i K^T (M128 N128 K16 steps, operands in shared memory), O_i += W_i V (A from tensor memory).
-//                    Products of one thread execute in the order of issue, so that S_i of the next tokens may overwrite W_i.
-// Tensor memory: S_0, S_1 at columns 0, 128; O_0, O_1 at 256, 384.  Shared memory: Q (2 x 128 rows), a ring of K / V tiles of 128 tokens, scales.
+//                    Only products of one shape into one accumulator are ordered by their issue, so S_i of the next tokens, which goes over W_i, waits
+//                    until O_i += W_i V has been executed (head size 128; with 64 there is room for W beside S).
+// Tensor memory: S_0, S_1 at columns 0, 128; O_0, O_1 from 256 on, D columns each; W_i over S_i, or (head size 64) W_0, W_1 at 384, 448.  Shared memory: Q (2 x 128 rows), a ring of K / V tiles of 128 tokens, scales.
 // Every wait is bounded (2 s): then the status word is set, the rest of the waits are skipped, tensor memory is freed, the kernel returns.
 #include <algorithm>
 #include <type_traits>
@@ -130,7 +131,8 @@ template <typename T, int D, bool E4M3>
 __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_constant__ Kv8Prefill p) {
     constexpr int kStages = stage_count<D>(), kTile = tile_bytes<D>(), kRegion = kTok * 128;   // a region: 128 rows x 64 halves
     constexpr int kBarFull = 0, kBarEmpty = kStages, kBarS = 2 * kStages, kBarP = kBarS + 2, kBarQ = kBarP + 2, kBarO = kBarQ + 1, kBarScale = kBarO + 1,
-                  kNumBars = kBarScale + kScaleRing;
+                  kBarRead = kBarScale + kScaleRing, kNumBars = kBarRead + 2;
+    constexpr uint32_t kColO = 256, kColW = D == 128 ? 0 : 384, kStrideW = D == 128 ? 128 : 64;   // tensor-memory columns
     static_assert(kNumBars * 8 + 8 <= 256, "");
     extern __shared__ uint8_t raw[];
     const Kv8Cache& c = p.cache;
@@ -171,7 +173,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             if (i < kBarEmpty) n = kTok / 16;
             else if (i == kBarP || i == kBarP + 1) n = 4;
             else if (i == kBarQ) n = two ? 8 : 4;
-            else if (i >= kBarScale) n = kTok / 16;
+            else if (i >= kBarScale && i < kBarRead) n = kTok / 16;
             mbar_init(bars + i, n);
         }
         *abort_flag = 0;
@@ -284,17 +286,25 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                 __syncwarp();
             };
             auto outputs = [&](int i, int idx, bool first) {     // O_i += W_i V
-                uint32_t vd = v_lo + static_cast<uint32_t>(idx % kStages) * (kTile >> 4), a = tmem + 128u * i;
+                uint32_t vd = v_lo + static_cast<uint32_t>(idx % kStages) * (kTile >> 4), a = tmem + kColW + kStrideW * i;
                 if (leader) {
 #pragma unroll
                     for (int kt = 0; kt < kTok / 16; ++kt)
-                        umma_f16_ts(tmem + 256u + 128u * i, a + 8u * kt, umma_desc_pack(vd + ((kt * 2048) >> 4), kHi), idesc_pv, !first || kt > 0);
+                        umma_f16_ts(tmem + kColO + static_cast<uint32_t>(D) * i, a + 8u * kt, umma_desc_pack(vd + ((kt * 2048) >> 4), kHi), idesc_pv, !first || kt > 0);
                 }
                 __syncwarp();
             };
             auto full = [&](int idx) {
                 wait(bars + kBarFull + idx % kStages, (idx / kStages) & 1);
                 tc_fence_after();
+            };
+            auto read = [&](int i, int j) {                       // W_i of tile j has been read
+                if constexpr (D == 128) {
+                    if (leader) umma_commit(smem_u32(bars + kBarRead + i));
+                    __syncwarp();
+                    wait(bars + kBarRead + i, j & 1);
+                    tc_fence_after();
+                }
             };
             auto release = [&](int idx) {
                 if (leader) umma_commit(smem_u32(bars + kBarEmpty + idx % kStages));
@@ -314,6 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                 outputs(0, vi, j == 0);
                 if (more) {
                     full(ki);
+                    read(0, j);
                     scores(0, ki);
                 }
                 if (two) {
@@ -323,7 +334,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                 }
                 release(vi);
                 if (more) {
-                    if (two) scores(1, ki);
+                    if (two) {
+                        read(1, j);
+                        scores(1, ki);
+                    }
                     release(ki);
                 }
             }
@@ -337,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         const int i = warp >> 2, m_row = tid & 127, row = tile.row0 + i * 128 + m_row;
         const int qi = row_query(p, min(row, tile.rows - 1));
         const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t tm_s = tmem + 128u * i + lane_base, tm_o = tmem + 256u + 128u * i + lane_base;
+        const uint32_t tm_s = tmem + 128u * i + lane_base, tm_o = tmem + kColO + static_cast<uint32_t>(D) * i + lane_base, tm_w = tmem + kColW + kStrideW * i + lane_base;
         // Queries: each warp copies its 32 rows into the operand layout, whole rows at a time (D / 8 lanes a row) and past the L1, most of whose memory
         // is shared memory here: as loads they waited for room there, 5 us a CTA.  float16 rows are operands as they are; a bfloat16 row is divided by
         // a power of two in place, since its range is not fp16's.
@@ -535,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                 if (c0 == 0) tmem_ld32_nowait(tm_s + 64, a);
                 weigh(b, 2);
                 if (c0 == 0) tmem_ld32_nowait(tm_s + 96, b);
-                tmem_st32_words(tm_s + static_cast<uint32_t>(c0 / 2), out);
+                tmem_st32_words(tm_w + static_cast<uint32_t>(c0 / 2), out);
             }
             tmem_st_wait();
             tc_fence_before();
@@ -673,7 +687,8 @@ Split split_of(const er_kv8_cache* c, const er_kv8_attention_params* u) {
     const uint64_t most = u->max_query_len > 0 ? std::min(u->max_query_len, u->num_tokens) : u->num_tokens;
     const int64_t least = static_cast<int64_t>(u->num_tokens) - static_cast<int64_t>(most) * (static_cast<int64_t>(c->num_seqs) - 1);   // tokens of the shortest
     if (u->type == ER_TYPE_FLOAT32) return {true, false};
-    return {least < 0 || static_cast<uint64_t>(least) * group <= kFewRows, most * group > kFewRows};
+    const bool many = most * group > kFewRows;
+    return {!many || least < 0 || static_cast<uint64_t>(least) * group <= kFewRows, many};
 }
 
 }  // namespace
@@ -701,7 +716,9 @@ extern "C" int32_t er_kv8_attention_prefill(const er_kv8_cache* cache, const er_
     if (rc == ER_OK) rc = kv8_check_attention(cache, u);
     if (rc != ER_OK) return rc;
     if (!u->query_starts) return report_error(ER_ERR_INVALID_ARGUMENT, "query_starts is needed for a ragged batch");
-    rc = kv8_check_device(cache);
+    if ((static_cast<uint64_t>(u->num_tokens) * (u->num_heads / cache->num_kv_heads) / 256 + cache->num_seqs) * cache->num_kv_heads > (1u << 28))
+        return report_error(ER_ERR_UNSUPPORTED, "more than 2^28 tiles of query rows");
+    rc = kv8_check_device(cache->keys);
     if (rc == ER_OK) rc = kv8_check_workspace(u, er_kv8_prefill_workspace_bytes(cache, u));
     if (rc != ER_OK || cache->num_seqs == 0 || u->num_tokens == 0) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -717,7 +734,7 @@ extern "C" int32_t er_kv8_attention_prefill(const er_kv8_cache* cache, const er_
         p.num_tokens = static_cast<int>(u->num_tokens);
         p.group = static_cast<int>(u->num_heads) / c.num_kv_heads;
         p.window = static_cast<int>(u->sliding_window);
-        p.min_rows = kFewRows + 1;
+        p.min_rows = sp.few ? kFewRows + 1 : 0;      // a hint that is wrong costs time, not rows
         p.group_magic = p.group == 1 ? 0 : ~0ull / static_cast<uint64_t>(p.group) + 1;
         p.scale_log2 = kv8_scale_log2(u->softmax_scale, cache->head_dim);
         const Plan pl = make_plan(cache, u, kv8_sm_count());
@@ -725,5 +742,5 @@ extern "C" int32_t er_kv8_attention_prefill(const er_kv8_cache* cache, const er_
         rc = u->type == ER_TYPE_FLOAT16 ? launch_shape<__half>(p, pl, cache->head_dim, e4m3, s) : launch_shape<__nv_bfloat16>(p, pl, cache->head_dim, e4m3, s);
         if (rc != ER_OK) return rc;
     }
-    return sp.few ? kv8_launch_decode(c, cache, u, true, u->type == ER_TYPE_FLOAT32 ? 0 : kFewRows, s) : ER_OK;
+    return sp.few ? kv8_launch_decode(c, cache, u, true, sp.many ? kFewRows : 0, s) : ER_OK;
 }

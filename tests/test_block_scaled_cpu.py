@@ -96,6 +96,26 @@ def test_norm_refusals(er, change, code):
     assert er.lib().er_qk_norm_rope(C.byref(norm(**change)), None) == code
 
 
+@pytest.mark.parametrize("change, code", [
+    (dict(q=0), INVALID), (dict(out=0), INVALID), (dict(type=3), INVALID), (dict(num_heads=3), SHAPE), (dict(num_heads=0), SHAPE), (dict(q=BASE + 8), INVALID),
+    (dict(q_head_stride=4), INVALID), (dict(softmax_scale=-1.0), INVALID), (dict(softmax_scale=float("inf")), INVALID), (dict(sliding_window=0xFFFFFFFF), UNSUPPORTED),
+    (dict(out_head_stride=64), SHAPE), (dict(out_token_stride=128), SHAPE), (dict(num_tokens=1 << 30), UNSUPPORTED)])
+def test_attention_refusals(er, change, code):
+    L = er.lib()
+    assert L.er_kv8_attention_decode(C.byref(cache()), C.byref(attention(**change)), None) == code
+    assert L.er_kv8_attention_prefill(C.byref(cache()), C.byref(attention(**change)), None) == code
+
+
+def test_decode_and_prefill_refusals(er):
+    L = er.lib()
+    for change, code in ((dict(query_len=0), UNSUPPORTED), (dict(query_len=17, num_tokens=34), UNSUPPORTED), (dict(num_tokens=3), SHAPE)):
+        assert L.er_kv8_attention_decode(C.byref(cache()), C.byref(attention(**change)), None) == code
+    assert L.er_kv8_attention_prefill(C.byref(cache()), C.byref(attention(query_starts=0)), None) == INVALID
+    assert L.er_qk_norm_rope(C.byref(norm(q_out_head_stride=0)), None) == SHAPE
+    assert L.er_kv8_attention_decode(None, C.byref(attention()), None) == INVALID
+    assert L.er_kv8_append(C.byref(cache()), None, None) == INVALID
+
+
 def test_attention_needs_a_device(er):
     """What passes every check of arguments reaches the device check and, without one, fails loudly."""
     import torch

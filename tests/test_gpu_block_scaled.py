@@ -418,6 +418,80 @@ def test_scales_of_very_different_blocks(er, torch, t):
             check_attention(torch, got[s:s + 1], want, big, t)
 
 
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_prefill_with_wrong_hints_and_short_caches(er, torch, t):
+    """max_query_len is a hint: too small a one loses no rows.  Queries in front of row 0 (more queries than rows) see nothing."""
+    lens, new = [300, 40, 9], [120, 40, 1]
+    cache, table, rows = fill(er, torch, "e4m3", lens, 16, 2, 64, 16)
+    starts = ints(torch, [0, 120, 160, 161])
+    q = torch.randn(161, 8, 64, generator=gen(torch, 3), device="cuda").to(dtype(torch, t))
+    for hint in (0, 1, 120, 10000):
+        got = cache.attention_prefill(q, starts, table, ints(torch, lens), max_query_len=hint)
+        for s, at in enumerate((0, 120, 160)):
+            want, big = ref_attention(torch, q[at:at + new[s]], *rows[s], lens[s], 64 ** -0.5)
+            check_attention(torch, got[at:at + new[s]], want, big, t)
+    got = cache.attention_prefill(q, starts, table, ints(torch, [50, 40, 0]))
+    assert bool((got[:70] == 0).all()) and bool((got[160:] == 0).all())
+    want, big = ref_attention(torch, q[70:120], rows[0][0][:50], rows[0][1][:50], 50, 64 ** -0.5)
+    check_attention(torch, got[70:120], want, big, t)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+def test_a_cache_beyond_four_gigabytes(er, torch, t):
+    """Pages whose bytes lie behind the first 2^32 of a side."""
+    pages, page, heads, dim = 34000, 128, 8, 128                     # 4.46 GB of codes a side
+    codes = [torch.empty(pages, heads, page, dim, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    scales = [torch.empty(pages, heads, 1, device="cuda") for _ in range(2)]
+    cache = er.BlockScaledKVCache.from_tensors(*codes, *scales)
+    ids, n = [pages - 1, 0, pages - 2], 300
+    g = gen(torch, 6)
+    k, v = (torch.randn(n, heads, dim, generator=g, device="cuda").to(dtype(torch, t)) for _ in range(2))
+    table = ints(torch, [ids])
+    cache.append(k, v, table, ints(torch, [n]), ints(torch, [0, n]), partial_rotary_factor=0.0)
+    dk, dv = (x.double() for x in cache.decoded_rows(ids, n))
+    assert bool(((dv - v.double()).abs() <= v.double().abs() * 2.0 ** -4 + 2.0 ** -14).all())
+    q = torch.randn(n, 16, dim, generator=g, device="cuda").to(dtype(torch, t))
+    want, big = ref_attention(torch, q, dk, dv, n, dim ** -0.5)
+    check_attention(torch, cache.attention_prefill(q, ints(torch, [0, n]), table, ints(torch, [n])), want, big, t)
+    check_attention(torch, cache.attention_decode(q[-1:], table, ints(torch, [n])), want[-1:], big[-1:], t)
+    assert cache.device_status() == 0
+
+
+def test_outputs_that_overlap_are_refused(er, torch):
+    cache, table, rows = fill(er, torch, "e4m3", [40], 16, 2, 128, 16)
+    q = torch.randn(1, 4, 128, device="cuda")
+    with pytest.raises(er.EdgeRunnerCUDAError) as e:
+        cache.attention_decode(q, table, ints(torch, [40]), out=torch.empty(1, 1, 128, device="cuda").expand(1, 4, 128))
+    assert e.value.name == "shape"
+    with pytest.raises(er.EdgeRunnerCUDAError) as e:
+        er.QKNormRopeKernel().encode(q, torch.empty(1, 1, 128, device="cuda").expand(1, 4, 128), ints(torch, [3]))
+    assert e.value.name == "shape"
+    out = torch.empty(4, 1, 128, device="cuda").transpose(0, 1)       # heads far apart, tokens inside
+    assert torch.equal(cache.attention_decode(q, table, ints(torch, [40]), out=out), cache.attention_decode(q, table, ints(torch, [40])))
+
+
+def test_many_sequences(er, torch):
+    """More sequences than a CTA has threads, empty ones and ones without queries among them."""
+    n = 700
+    lens = [(7 * s) % 50 for s in range(n)]
+    new = [min(lens[s], s % 4) for s in range(n)]
+    cache, table, rows = fill(er, torch, "int8", lens, 16, 1, 64, 16)
+    starts = [sum(new[:s]) for s in range(n + 1)]
+    q = torch.randn(starts[-1], 4, 64, generator=gen(torch, 2), device="cuda").bfloat16()
+    got = cache.attention_prefill(q, ints(torch, starts), table, ints(torch, lens), max_query_len=3)
+    dec = cache.attention_decode(q[:n], table, ints(torch, lens))
+    for s in range(n):
+        if new[s]:
+            want, big = ref_attention(torch, q[starts[s]:starts[s + 1]], *rows[s], lens[s], 64 ** -0.5)
+            check_attention(torch, got[starts[s]:starts[s + 1]], want, big, "bf16")
+        if lens[s]:
+            want, big = ref_attention(torch, q[s:s + 1], *rows[s], lens[s], 64 ** -0.5)
+            check_attention(torch, dec[s:s + 1], want, big, "bf16")
+        else:
+            assert bool((dec[s] == 0).all())
+    assert cache.device_status() == 0
+
+
 def test_two_streams_and_a_graph(er, torch):
     """Calls on two streams do not share a workspace; captured calls follow the lengths and queries of their buffers at replay."""
     lens = [3000, 2500]
