@@ -6,9 +6,8 @@
 // costs an operation a score: a multiplies the factor inside exp2's argument, log2(b / R) is part of its offset, and the sum of 16 weights is
 // divided by b / R once.
 //
-// One CTA owns two tiles of 128 query rows of a (sequence, kv head): row r is query r / group, head r % group, any group.  Bound by the tensor
-// pipe and, as closely, by exp2 (16 a clock and SM against 128 x 128 x D products in 512 clocks), so the two tiles take turns: while one is in its softmax
-// the products of the other run.
+// One CTA owns two tiles of 128 query rows of a (sequence, kv head): row r is query r / group, head r % group, any group.  The tensor pipe takes 1024
+// clocks for 128 tokens of a tile, exp2 (16 a clock and SM) as long, so the two tiles take turns: while one is in its softmax the products of the other run.
 //   warps 0-3, 4-7   softmax of tile 0, 1: a thread is a row.  Reads S from tensor memory twice (maximum, then weights), writes w as fp16 over S.  The
 //                    running maximum may lag by 2^8 before the row of O is rescaled in tensor memory, so that this is rare.
 //   warps 8-11, 13-15  fetch codes and write them as fp16 into the operand layout: a conversion in the loader reads 1 byte an element from L2
@@ -16,8 +15,16 @@
 //   warp 12          one lane issues the products: S_i = Q_i K^T (M128 N128 K16 steps, operands in shared memory), O_i += W_i V (A from tensor memory).
 //                    Only products of one shape into one accumulator are ordered by their issue, so S_i of the next tokens, which goes over W_i, waits
 //                    until O_i += W_i V has been executed (head size 128; with 64 there is room for W beside S).
-// Tensor memory: S_0, S_1 at columns 0, 128; O_0, O_1 from 256 on, D columns each; W_i over S_i, or (head size 64) W_0, W_1 at 384, 448.  Shared memory: Q (2 x 128 rows), a ring of K / V tiles of 128 tokens, scales.
+// Tensor memory: S_0, S_1 at columns 0, 128; O_0, O_1 from 256 on, D columns each; W_i over S_i, or (head size 64) W_0, W_1 at 384, 448.  Shared
+// memory: Q (2 x 128 rows), a ring of K / V tiles of 128 tokens, scales.
 // Every wait is bounded (2 s): then the status word is set, the rest of the waits are skipped, tensor memory is freed, the kernel returns.
+//
+// Measured (B200, 32 query / 8 kv heads of 128): a chunk of 2048 tokens at 32768, int8, float16: 1.28 ms = 835 TFLOP/s = 0.50 of the library's bf16
+// product; the same without the softmax arithmetic 0.80 ms, without the conversion besides 0.63 ms.  A tile's softmax takes 3400 clocks of a period
+// of 4500: 2400 for the weights (1890 alone; 1024 of them exp2), 550 for the maximum.  What changed it on the way: loops over 64 columns instead of
+// straight-line code, which had the warps wait for instructions (2.20 -> 1.39 ms); seven loader warps, packed arithmetic, no divisions (1.29); scores of half
+// a tile kept in registers between the passes (1.21, before products were ordered by commits: +1 %).  Tried and dropped: part of the exponentials as
+// polynomials on the FMA pipe (the same or slower), weights in one pass against the old maximum (registers spill).
 #include <algorithm>
 #include <type_traits>
 
