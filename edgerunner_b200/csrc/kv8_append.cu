@@ -304,11 +304,11 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const __grid_constant__
             const T* src = in_rows + (pr >> 1) * in_head;
             const uint32_t to = smem_u32(ring + slot * (kPasses * 2 * 32));
 #pragma unroll
-            for (int ps = 0; ps < kPasses; ++ps) {
-                if (is_new[ps]) {
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + ps * 1024), "l"(src + ps * in_pass) : "memory");
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + ps * 1024 + 512), "l"(src + ps * in_pass + HALF) : "memory");
-                }
+            for (int ps = 0; ps < kPasses; ++ps) {                          // rows that are not new: zeros
+                const T* from = is_new[ps] ? src + ps * in_pass : static_cast<const T*>(p.in[0]);
+                const int bytes = is_new[ps] ? 16 : 0;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + ps * 1024), "l"(from), "r"(bytes) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + ps * 1024 + 512), "l"(from + HALF), "r"(bytes) : "memory");
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -347,10 +347,8 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const __grid_constant__
         asm volatile("cp.async.wait_group %0;" ::"n"(kAppendSlots - 2) : "memory");
 #pragma unroll
         for (int ps = 0; ps < kPasses; ++ps) {
-            const bool on = is_new[ps] && pr < pairs;
-            const uint4 zero = make_uint4(0, 0, 0, 0);
-            unpack_pairs<T>(on ? ring[(slot * kPasses + ps) * 64] : zero, a[ps]);
-            unpack_pairs<T>(on ? ring[(slot * kPasses + ps) * 64 + 32] : zero, b[ps]);
+            unpack_pairs<T>(ring[(slot * kPasses + ps) * 64], a[ps]);
+            unpack_pairs<T>(ring[(slot * kPasses + ps) * 64 + 32], b[ps]);
         }
         fetch(it + (kAppendSlots - 1) * gridDim.y, slot == 0 ? kAppendSlots - 1 : slot - 1);
         slot = slot + 1 == kAppendSlots ? 0 : slot + 1;
@@ -424,9 +422,9 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const __grid_constant__
                     store(d, x, y);
                 }
             }
+            if (inv > 0.f) {
 #pragma unroll
-            for (int ps = 0; ps < kPasses; ++ps) {
-                if (is_new[ps]) {
+                for (int ps = 0; ps < kPasses; ++ps) {
                     const float f = factor[ps] * inv;
                     const F2 f2 = pack2(f, f);
                     float x[VEC], y[VEC];
@@ -434,11 +432,14 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const __grid_constant__
                     for (int i = 0; i < VEC / 2; ++i) { a[ps][i] = mul2(a[ps][i], f2); b[ps][i] = mul2(b[ps][i], f2); }
                     floats_of(a[ps], x);
                     floats_of(b[ps], y);
-                    if (!(inv > 0.f)) {                                     // zeros, or a NaN scale: codes of zeros
-#pragma unroll
-                        for (int i = 0; i < VEC; ++i) x[i] = y[i] = 0.f;
-                    }
-                    store(dst + ps * kRowsPerPass * D, x, y);
+                    if (is_new[ps]) store(dst + ps * kRowsPerPass * D, x, y);
+                }
+            } else {                                                        // zeros, or a NaN scale: codes of zeros
+                const float zeros[VEC] = {};
+#pragma unroll 1
+                for (int ps = 0; ps < kPasses; ++ps) {
+                    const int row = row0 + ps * kRowsPerPass + sub;
+                    if (row >= lead && row < end) store(dst + ps * kRowsPerPass * D, zeros, zeros);
                 }
             }
             if (row0 == 0 && lane == 0) *scale_at = scale;

@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
         const int tok = pp.token(pu) + half * kKv8Unit;
         ppage = tok < pp.r.len ? kv8_page(c, pp.seq, tok) : -1;
     };
-    int pstage = 0;
+    int pstage = 0, produced = 0;
     auto produce = [&]() {          // the next unit, if there is one: lanes 0-15 see to half 0, 16-31 to half 1
         if (pmore && !*abort_flag) {
             const int tok = pp.token(pu) + half * kKv8Unit;
@@ -337,6 +337,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
                 else sc[lane & 15] = -1.f;      // nothing to see: no row yet, or no page
             }
             pu += kWarps;
+            ++produced;
             settle();
         }
         cp_async_commit();
@@ -684,6 +685,11 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
         first_segment = false;
     }
     cp_async_wait<0>();
+    if (*abort_flag) {                  // a wait gave up: the copies that are still on their way write into this CTA's memory
+        const uint64_t start = global_timer_ns();
+        for (int k = max(0, produced - kStages); k < produced; ++k)
+            while (!mbar_try_wait(my_bars + k % kStages, (k / kStages) & 1) && global_timer_ns() - start < 1000000000ull) {}
+    }
 }
 
 // Joins the partials of the items that more than one CTA worked on.  At most one item begins in a CTA's range and goes on behind it: block
