@@ -37,12 +37,17 @@ namespace {
 constexpr int kTok = 128;                  // tokens of a K / V tile
 constexpr int kSoftWarps = 8, kLoadWarps = 7, kIssueWarp = 12;   // loaders: warps 8-11 and 13-15
 constexpr int kThreads = 512;
-constexpr int kScaleRing = 4;
 constexpr float kLag = 8.f;                // how far (log2) a row's maximum may rise above the one in use
 constexpr float kCarry = 5.f;              // weights are carried 2^5 times: w <= 2^(8 + 2 + 5) < 65504
 template <int D> __host__ __device__ constexpr int stage_count() { return D == 128 ? 5 : 8; }
+// Slots for the scales of a tile's blocks.  The loader of key tile j waits for the ring entry that it fills, not for the scale slot.  With an even number of
+// entries that one held the keys of tile j - entries / 2, and those are released by their score product, before the softmax of the same tile reads its scales;
+// what is sure to have ended is the softmax of the tile before it.  So a slot may come round after entries / 2 + 1 tiles, no earlier.  (With an odd number the
+// entry held values of tile j - entries / 2 - 1, whose product follows that tile's softmax: the same distance.)
+template <int D> __host__ __device__ constexpr int scale_slots() { return stage_count<D>() / 2 + 1; }
+constexpr int kMostScaleSlots = 5;
 template <int D> __host__ __device__ constexpr int tile_bytes() { return kTok * D * 2; }   // also a tile of 128 query rows
-template <int D> __host__ __device__ constexpr int prefill_smem() { return (stage_count<D>() + 2) * tile_bytes<D>() + 256 + kScaleRing * 32 * 4 + 1024; }
+template <int D> __host__ __device__ constexpr int prefill_smem() { return (stage_count<D>() + 2) * tile_bytes<D>() + 256 + kMostScaleSlots * 32 * 4 + 1024; }
 
 struct Kv8Prefill {
     Kv8Cache cache;
@@ -136,11 +141,12 @@ __device__ __forceinline__ uint32_t half2_word(float a, float b) {
 
 template <typename T, int D, bool E4M3>
 __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_constant__ Kv8Prefill p) {
-    constexpr int kStages = stage_count<D>(), kTile = tile_bytes<D>(), kRegion = kTok * 128;   // a region: 128 rows x 64 halves
+    constexpr int kStages = stage_count<D>(), kScaleRing = scale_slots<D>(), kTile = tile_bytes<D>(), kRegion = kTok * 128;   // a region: 128 rows x 64 halves
     constexpr int kBarFull = 0, kBarEmpty = kStages, kBarS = 2 * kStages, kBarP = kBarS + 2, kBarQ = kBarP + 2, kBarO = kBarQ + 1, kBarScale = kBarO + 1,
                   kBarRead = kBarScale + kScaleRing, kNumBars = kBarRead + 2;
     constexpr uint32_t kColO = 256, kColW = D == 128 ? 0 : 384, kStrideW = D == 128 ? 128 : 64;   // tensor-memory columns
     static_assert(kNumBars * 8 + 8 <= 256, "");
+    static_assert(kScaleRing > kStages / 2 && kScaleRing <= kMostScaleSlots, "scales would be overwritten while the softmax reads them");
     extern __shared__ uint8_t raw[];
     const Kv8Cache& c = p.cache;
     const uint32_t sbase = (smem_u32(raw) + 1023u) & ~1023u;
@@ -196,8 +202,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     const uint32_t tmem = *tmem_slot;
     const Waiter wait{abort_flag, &c};
     // Codes -> fp16 operand tiles.  The 16-token units of the half tiles (keys of tile 0, values of tile 0, keys of tile 1, ...; eight to a half
-    // tile) go round robin to the loader warps, each with three units in flight in registers.  Lane: 16 codes of the rows lane / 4 and 8 further, two
-    // rows of four chunks to eight lanes, which store without bank conflicts.
+    // tile) go round robin to the loader warps, each with the codes of its next unit on the way in registers and the page of the one behind it looked
+    // up.  Lane: 16 codes of the rows lane / 4 and 8 further, two rows of four chunks to eight lanes, which store without bank conflicts.
     auto load_tiles = [&](int w) {
         constexpr int kParts = D / 64, kLoads = 2 * kParts;          // 64 codes of 8 rows at a time
         struct Unit {

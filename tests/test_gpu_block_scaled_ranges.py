@@ -1,0 +1,53 @@
+"""The 8-bit block-scaled cache where its ranges end: long runs of keys, scales far apart, extreme windows, epsilons and magnitudes, streams.
+
+Tolerances are those of test_gpu_block_scaled.py (derived there), with one more term where keys run long: each product of 16 keys that the tensor cores add
+to a running sum truncates it, by less than one unit in the last place, 2^-23 relative; a run of n keys adds n / 16 of them at most.
+"""
+import math
+
+import pytest
+
+from test_gpu_block_scaled import check_attention, dtype, er, fill, gen, half_step, ints, make_cache, ref_attention, tables, torch  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def far_apart(torch, cache, seed, key_bits=4, value_bits=6):
+    """Block scales that differ by powers of two from block to block: keys down to 2^-key_bits, values 2^-value_bits .. 2^value_bits of what they were."""
+    g = gen(torch, seed)
+    cache.key_scales.mul_(torch.exp2(-torch.randint(0, key_bits + 1, cache.key_scales.shape, generator=g, device="cuda").float()))
+    cache.value_scales.mul_(torch.exp2(torch.randint(-value_bits, value_bits + 1, cache.value_scales.shape, generator=g, device="cuda").float()))
+
+
+def rows_of(cache, table, length):
+    return tuple(x.double() for x in cache.decoded_rows([p for p in table.tolist() if p >= 0], length))
+
+
+def check_long(torch, got, want, big, t, keys):
+    bound = (6e-5 + 2.0 ** -11 + keys / 16 * 2.0 ** -23) * big + half_step(torch, dtype(torch, t)) * want.abs() + 2.0 ** -25
+    err = (got.double() - want).abs()
+    assert bool((err <= bound).all()), float((err / bound).max())
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("dim, seqs, n, longest, block", [
+    (64, 32, 10, 8000, 16), (64, 23, 40, 4100, 16), (64, 23, 40, 2500, 128), (128, 32, 10, 4000, 16), (128, 23, 40, 2300, 32)])
+def test_prefill_over_many_key_tiles(er, torch, fmt, t, dim, seqs, n, longest, block):  # noqa: F811
+    """18 to 63 key tiles to a CTA: 4 kv heads times 37 slots of 256 query rows make 148 tile pairs, which are not cut along the keys.  One row tile a CTA
+    (10 queries of 4 heads) and two (40 of them).  The sequences read the same pages, at lengths of their own."""
+    heads, kv_heads = 16, 4
+    cache, table, _ = fill(er, torch, fmt, [longest], 128, kv_heads, dim, block, seed=dim + block)
+    far_apart(torch, cache, 5)
+    k, v = rows_of(cache, table[0], longest)
+    lens = [longest - 37 * s for s in range(seqs)]
+    starts = ints(torch, [n * s for s in range(seqs + 1)])
+    q = torch.randn(n * seqs, heads, dim, generator=gen(torch, 7), device="cuda").to(dtype(torch, t))
+    many = table.expand(seqs, -1).contiguous()
+    got = [cache.attention_prefill(q, starts, many, ints(torch, lens), max_query_len=n) for _ in range(3)]
+    assert cache.device_status() == 0
+    assert all(torch.equal(x, got[0]) for x in got[1:])
+    for s, length in enumerate(lens):
+        mine = slice(n * s, n * (s + 1))
+        want, big = ref_attention(torch, q[mine], k[:length], v[:length], length, dim ** -0.5)
+        check_long(torch, got[0][mine], want, big, t, length)
