@@ -83,7 +83,10 @@ def _weight(w, name, dim, index):
         return 0
     if w.dtype is not _torch.float32 or w.shape != (dim,) or not w.is_contiguous() or w.get_device() != index:
         raise ValueError("%s must be float32 [%d] on CUDA device %d" % (name, dim, index))
-    return w.data_ptr()
+    p = w.data_ptr()
+    if p & 7:
+        raise ValueError("%s must start on an 8-byte boundary (a view at an odd offset of a larger buffer does not)" % name)
+    return p
 
 
 class QKNormRopeKernel:

@@ -273,6 +273,6 @@ inline bool kv8_rows_apart(int64_t token_stride, int64_t head_stride, int64_t to
     const bool heads_inside = head_stride >= head_dim && token_stride >= head_stride * (heads - 1) + head_dim;
     return heads_inside || (token_stride >= head_dim && head_stride >= token_stride * (tokens - 1) + head_dim);
 }
-inline bool kv8_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool kv8_aligned(const void* p, uintptr_t bytes = 16) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 }  // namespace er

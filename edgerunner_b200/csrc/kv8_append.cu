@@ -57,6 +57,8 @@ int32_t kv8_check(const er_kv8_cache* c, Kv8Cache* out) {
     if (static_cast<uint64_t>(c->num_pages) * c->num_kv_heads * c->page_size > 0x7FFFFFFFull)
         return report_error(ER_ERR_UNSUPPORTED, "the cache has more than 2^31 rows (pages * kv heads * page_size)");
     if (!kv8_aligned(c->keys) || !kv8_aligned(c->values)) return report_error(ER_ERR_INVALID_ARGUMENT, "keys and values must be 16-byte aligned");
+    if (!kv8_aligned(c->key_scales, 4) || !kv8_aligned(c->value_scales, 4) || !kv8_aligned(c->block_tables, 4) || !kv8_aligned(c->kv_lens, 4) || !kv8_aligned(c->status, 4))
+        return report_error(ER_ERR_INVALID_ARGUMENT, "scales, block_tables, kv_lens and status must be 4-byte aligned");
     out->codes[0] = c->keys; out->codes[1] = c->values;
     out->scales[0] = c->key_scales; out->scales[1] = c->value_scales;
     out->tables = c->block_tables; out->lens = c->kv_lens; out->status = c->status;
@@ -520,6 +522,8 @@ extern "C" int32_t er_qk_norm_rope(const er_qk_norm_rope_params* u, void* stream
     if (rc != ER_OK) return rc;
     if (!kv8_aligned(u->q) || !kv8_aligned(u->q_out) || !kv8_aligned(u->k) || !kv8_aligned(u->k_out))
         return report_error(ER_ERR_INVALID_ARGUMENT, "q, k and the outputs must be 16-byte aligned");
+    if (!kv8_aligned(u->q_norm_weight, 8) || !kv8_aligned(u->k_norm_weight, 8) || !kv8_aligned(u->positions, 4))      // weights are read in pairs
+        return report_error(ER_ERR_INVALID_ARGUMENT, "norm weights must be 8-byte, positions 4-byte aligned");
     const int64_t strides[8] = {u->q_token_stride, u->q_head_stride, u->q_out_token_stride, u->q_out_head_stride,
                                 u->k_token_stride, u->k_head_stride, u->k_out_token_stride, u->k_out_head_stride};
     if (!strides_ok(u->type, strides, u->k ? 8 : 4)) return report_error(ER_ERR_INVALID_ARGUMENT, "strides must be multiples of 16 bytes");
@@ -560,6 +564,8 @@ extern "C" int32_t er_kv8_append(const er_kv8_cache* cache, const er_kv8_append_
     rc = check_rope(u->rope_theta, u->rope_scaling, u->partial_rotary_factor, u->rms_eps);
     if (rc != ER_OK) return rc;
     if (!kv8_aligned(u->k) || !kv8_aligned(u->v)) return report_error(ER_ERR_INVALID_ARGUMENT, "k and v must be 16-byte aligned");
+    if (!kv8_aligned(u->k_norm_weight, 8) || !kv8_aligned(u->query_starts, 4))
+        return report_error(ER_ERR_INVALID_ARGUMENT, "the norm weight must be 8-byte, query_starts 4-byte aligned");
     const int64_t strides[4] = {u->k_token_stride, u->k_head_stride, u->v_token_stride, u->v_head_stride};
     if (!strides_ok(u->type, strides, 4)) return report_error(ER_ERR_INVALID_ARGUMENT, "strides must be multiples of 16 bytes");
     if (u->num_tokens > 0x7FFFFF00u) return report_error(ER_ERR_UNSUPPORTED, "num_tokens beyond 2^31");

@@ -729,6 +729,7 @@ extern "C" int32_t er_kv8_attention_prefill(const er_kv8_cache* cache, const er_
     if (rc == ER_OK) rc = kv8_check_attention(cache, u);
     if (rc != ER_OK) return rc;
     if (!u->query_starts) return report_error(ER_ERR_INVALID_ARGUMENT, "query_starts is needed for a ragged batch");
+    if (!kv8_aligned(u->query_starts, 4)) return report_error(ER_ERR_INVALID_ARGUMENT, "query_starts must be 4-byte aligned");
     if ((static_cast<uint64_t>(u->num_tokens) * (u->num_heads / cache->num_kv_heads) / 256 + cache->num_seqs) * cache->num_kv_heads > (1u << 28))
         return report_error(ER_ERR_UNSUPPORTED, "more than 2^28 tiles of query rows");
     rc = kv8_check_device(cache->keys);

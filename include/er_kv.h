@@ -452,7 +452,7 @@ enum { ER_KV8_E4M3 = 0, ER_KV8_INT8 = 1 };
  * head_dim) / rope_scaling (angles in 64 bits), arithmetic in 32 bits, one rounding at the end.  A NULL weight: no norm for that
  * tensor; partial_rotary_factor 0: no rotation (positions may be NULL).  Strides are in elements; the elements of a head are
  * contiguous.  in and out are the same buffer with the same strides, or do not overlap.  k NULL: queries only.  head_dim: a multiple of 16 up to
- * 256.  Buffers and strides are 16-byte aligned; weights are float32. */
+ * 256.  Buffers and strides are 16-byte aligned; weights are float32, 8-byte aligned. */
 typedef struct {
     const void* q;
     void* q_out;
@@ -495,7 +495,7 @@ typedef struct {
     const void* v;
     int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;   /* elements, 16-byte multiples */
     const int32_t* query_starts; /* device [num_seqs + 1] or NULL */
-    const float* k_norm_weight;  /* device [head_dim] or NULL */
+    const float* k_norm_weight;  /* device [head_dim], 8-byte aligned, or NULL */
     uint32_t num_tokens;
     uint32_t type;               /* ER_TYPE_* of k and v */
     float rms_eps, rope_theta, rope_scaling, partial_rotary_factor;

@@ -1,0 +1,56 @@
+"""Refusals of the 8-bit block-scaled cache and of the head-norm operator that keep kernels inside their buffers; nothing here needs a device."""
+import ctypes as C
+
+import pytest
+
+from test_block_scaled_cpu import BASE, INVALID, append, attention, cache, er, norm  # noqa: F401
+
+
+@pytest.mark.parametrize("change", [dict(q_norm_weight=BASE + 4), dict(k=BASE, k_out=BASE, num_kv_heads=2, k_token_stride=256, k_head_stride=128, k_out_token_stride=256,
+                                                                       k_out_head_stride=128, k_norm_weight=BASE + 12), dict(positions=BASE + 2)])
+def test_norm_refuses_misaligned_buffers(er, change):  # noqa: F811
+    """Weights are read as pairs of floats: a view at an odd offset would be a misaligned load."""
+    assert er.lib().er_qk_norm_rope(C.byref(norm(**change)), None) == INVALID
+
+
+@pytest.mark.parametrize("change", [dict(k_norm_weight=BASE + 4), dict(query_starts=BASE + 1)])
+def test_append_refuses_misaligned_buffers(er, change):  # noqa: F811
+    assert er.lib().er_kv8_append(C.byref(cache()), C.byref(append(**change)), None) == INVALID
+
+
+@pytest.mark.parametrize("field", ["key_scales", "value_scales", "block_tables", "kv_lens", "status"])
+def test_cache_refuses_misaligned_words(er, field):  # noqa: F811
+    L, c = er.lib(), cache(**{field: BASE + 2})
+    assert L.er_kv8_append(C.byref(c), C.byref(append()), None) == INVALID
+    assert L.er_kv8_attention_decode(C.byref(c), C.byref(attention()), None) == INVALID
+    assert L.er_kv8_attention_prefill(C.byref(c), C.byref(attention()), None) == INVALID
+
+
+def test_prefill_refuses_misaligned_starts(er):  # noqa: F811
+    assert er.lib().er_kv8_attention_prefill(C.byref(cache()), C.byref(attention(query_starts=BASE + 2)), None) == INVALID
+
+
+def test_python_layer_refuses_misaligned_weights(er):  # noqa: F811
+    """The check itself, on a stand-in with the address of a view that starts one float into an aligned buffer."""
+    import torch
+    from edgerunner_b200 import block_scaled_cache as b
+
+    class View:
+        dtype, shape = torch.float32, (128,)
+
+        def __init__(self, at):
+            self.at = at
+
+        def is_contiguous(self):
+            return True
+
+        def get_device(self):
+            return 0
+
+        def data_ptr(self):
+            return self.at
+
+    b._types()
+    assert b._weight(View(BASE + 8), "w", 128, 0) == BASE + 8
+    with pytest.raises(ValueError, match="8-byte"):
+        b._weight(View(BASE + 4), "w", 128, 0)
