@@ -517,7 +517,7 @@ extern "C" int32_t er_qk_norm_rope(const er_qk_norm_rope_params* u, void* stream
     if (u->head_dim == 0 || u->head_dim % 16 != 0 || u->head_dim > 256) return report_error(ER_ERR_UNSUPPORTED, "head_dim must be a multiple of 16 up to 256");
     if (u->num_heads == 0 || u->num_heads > 65535u || (u->k && (u->num_kv_heads == 0 || u->num_kv_heads > 65535u)))
         return report_error(ER_ERR_SHAPE, "head counts must be between 1 and 65535");
-    if (u->num_tokens > 0x7FFFFF00u) return report_error(ER_ERR_UNSUPPORTED, "num_tokens beyond 2^31");
+    if (u->num_tokens > 0x7FFF0000u) return report_error(ER_ERR_UNSUPPORTED, "num_tokens beyond 2^31 - 2^16");   // a warp's next token number stays an int
     int32_t rc = check_rope(u->rope_theta, u->rope_scaling, u->partial_rotary_factor, u->rms_eps);
     if (rc != ER_OK) return rc;
     if (!kv8_aligned(u->q) || !kv8_aligned(u->q_out) || !kv8_aligned(u->k) || !kv8_aligned(u->k_out))

@@ -3,7 +3,7 @@ import ctypes as C
 
 import pytest
 
-from test_block_scaled_cpu import BASE, INVALID, append, attention, cache, er, norm  # noqa: F401
+from test_block_scaled_cpu import BASE, INVALID, UNSUPPORTED, append, attention, cache, er, norm  # noqa: F401
 
 
 @pytest.mark.parametrize("change", [dict(q_norm_weight=BASE + 4), dict(k=BASE, k_out=BASE, num_kv_heads=2, k_token_stride=256, k_head_stride=128, k_out_token_stride=256,
@@ -54,3 +54,12 @@ def test_python_layer_refuses_misaligned_weights(er):  # noqa: F811
     assert b._weight(View(BASE + 8), "w", 128, 0) == BASE + 8
     with pytest.raises(ValueError, match="8-byte"):
         b._weight(View(BASE + 4), "w", 128, 0)
+
+
+def test_norm_refuses_more_tokens_than_its_counter_holds(er):  # noqa: F811
+    """A warp steps by the slots of the whole grid (148 * 4 * 8 at most) from token to token: the number behind the last one has to stay an int."""
+    for tokens in (0x7FFFFF00, 0x7FFF0001):
+        assert er.lib().er_qk_norm_rope(C.byref(norm(num_tokens=tokens)), None) == UNSUPPORTED
+    import torch
+    if not torch.cuda.is_available():
+        assert er.lib().er_qk_norm_rope(C.byref(norm(num_tokens=0x7FFF0000)), None) == -8      # past the checks of arguments: no device
