@@ -382,7 +382,8 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const __grid_constant__
                 up = max3_nan(up, x, y);
                 down = min3_nan(down, x, y);
             }
-            mx = max3_nan(mx, up * factor[ps], -down * factor[ps]);
+            // rows that are not new have no part in it: without an epsilon the factor of their zeros is infinite
+            mx = max3_nan(mx, is_new[ps] ? up * factor[ps] : 0.f, is_new[ps] ? -down * factor[ps] : 0.f);
         }
         mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx) & 0x7FFFFFFFu));   // magnitudes compare like integers, NaN above all
         if (lane == 0) warp_max[turn][warp] = mx;

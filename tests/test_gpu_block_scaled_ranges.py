@@ -51,3 +51,28 @@ def test_prefill_over_many_key_tiles(er, torch, fmt, t, dim, seqs, n, longest, b
         mine = slice(n * s, n * (s + 1))
         want, big = ref_attention(torch, q[mine], k[:length], v[:length], length, dim ** -0.5)
         check_long(torch, got[0][mine], want, big, t, length)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_append_without_an_epsilon(er, torch, fmt, t):  # noqa: F811
+    """rms_eps 0: rows of the block that the call does not write have no norm, and must not decide its scale."""
+    g = gen(torch, 3)
+    cache = er.BlockScaledKVCache(4, 32, 2, 128, er.BlockScaledFormat[fmt])
+    table, kw = ints(torch, [[2, 0], [1, 3]]), 1 + 0.1 * torch.randn(128, generator=g, device="cuda")
+    lens, new = [0, 0], [[5, 1], [1, 1], [14, 1], [13, 33]]
+    kept = [[], []]
+    for step in new:
+        lens = [a + b for a, b in zip(lens, step)]
+        k, v = (torch.randn(sum(step), 2, 128, generator=g, device="cuda").to(dtype(torch, t)) for _ in range(2))
+        cache.append(k, v, table, ints(torch, lens), ints(torch, [0, step[0], sum(step)]), k_norm_weight=kw, rms_eps=0.0, partial_rotary_factor=0.0)
+        for s, part in enumerate(k.split(step)):
+            x = part.double()
+            kept[s].append(x / x.square().mean(-1, keepdim=True).sqrt() * kw.double())
+    assert bool(torch.isfinite(cache.key_scales).all()) and bool(torch.isfinite(cache.value_scales).all())
+    for s in range(2):
+        want, (k, _) = torch.cat(kept[s]), cache.decoded_rows(table[s], lens[s])
+        # a code is written once and rounded again when its block's scale grows, on each of 3 later calls at most: half a step each, of a block whose
+        # magnitudes stay below 8; E4M3's smallest codes 2^-10 of a scale of at most 2^-5
+        bound = 4 * 8 / 127 / 2 if fmt == "int8" else want.abs() * 2.0 ** -4 * (1 + 1e-4) + 4 * 2.0 ** -15
+        assert bool(((k.double() - want).abs() <= bound).all())
