@@ -428,7 +428,13 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const __grid_constant__
             if (inv > 0.f) {
 #pragma unroll
                 for (int ps = 0; ps < kPasses; ++ps) {
-                    const float f = factor[ps] * inv;
+                    float f = factor[ps] * inv;
+                    if (isinf(f)) {                                         // elements below 2^-119: first the norm, then the scale
+                        const F2 norm = pack2(factor[ps], factor[ps]);
+#pragma unroll
+                        for (int i = 0; i < VEC / 2; ++i) { a[ps][i] = mul2(a[ps][i], norm); b[ps][i] = mul2(b[ps][i], norm); }
+                        f = inv;
+                    }
                     const F2 f2 = pack2(f, f);
                     float x[VEC], y[VEC];
 #pragma unroll

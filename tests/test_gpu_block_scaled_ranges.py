@@ -76,3 +76,21 @@ def test_append_without_an_epsilon(er, torch, fmt, t):  # noqa: F811
         # magnitudes stay below 8; E4M3's smallest codes 2^-10 of a scale of at most 2^-5
         bound = 4 * 8 / 127 / 2 if fmt == "int8" else want.abs() * 2.0 ** -4 * (1 + 1e-4) + 4 * 2.0 ** -15
         assert bool(((k.double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_append_of_tiny_rows(er, torch, fmt, t):  # noqa: F811
+    """Keys of 1e-37 under an epsilon of 1e-6: what turns them into codes, the norm factor (1000) over the scale, is beyond float32's range."""
+    g = gen(torch, 4)
+    cache = er.BlockScaledKVCache(2, 32, 1, 64, er.BlockScaledFormat[fmt])
+    k = (torch.randn(20, 1, 64, generator=g, device="cuda") * 1e-37).to(dtype(torch, t))
+    k[3] = 0
+    k[:, :, ::7] = 0
+    cache.append(k, k, ints(torch, [[1]]), ints(torch, [20]), ints(torch, [0, 20]), k_norm_weight=torch.ones(64, device="cuda"), partial_rotary_factor=0.0)
+    want = k.double() / math.sqrt(1e-6)
+    got = cache.decoded_rows([1], 20)[0].double()
+    scale = cache.key_scales[1, 0].double().repeat_interleave(16)[:20, None, None]
+    step = scale / 2 if fmt == "int8" else torch.maximum(want.abs() * 2.0 ** -4, scale * 2.0 ** -10)
+    # the norm factor is off by a few steps of float32; a decoded value below 2^-126 may be flushed
+    assert bool(((got - want).abs() <= step * (1 + 1e-4) + want.abs() * 2.0 ** -20 + 2.0 ** -126).all())
