@@ -3,7 +3,8 @@ as an operator of its own (er_kv8_*, er_qk_norm_rope in include/er_kv.h).  No co
 
 Inputs are torch CUDA tensors in float32, float16 or bfloat16: [tokens, heads, head_dim], the last dimension contiguous, any 16-byte
 aligned strides before it (so slices of one projection's output go in as they are).  Work is enqueued on `stream`, by default the current
-torch stream of the tensors' device; nothing waits, and every call may be captured into a CUDA graph.  A step over a batch:
+torch stream of the tensors' device; nothing waits, and every call may be captured into a CUDA graph.  With an explicit `stream` the inputs have
+to be ready on it; an output that the call allocates is that stream's memory, kept until the current stream is done with it too.  A step over a batch:
 
     QKNormRopeKernel().encode(q, q, positions, q_norm_weight=qw, rope_theta=theta)       # queries, in place
     cache.append(k, v, block_tables, kv_lens, query_starts, k_norm_weight=kw, rope_theta=theta)
@@ -194,11 +195,20 @@ class BlockScaledKVCache:
                 kp, vp, kt, kh, vt, vh, starts, _weight(k_norm_weight, "k_norm_weight", self.head_dim, index), tokens, kind, rms_eps, rope_theta,
                 rope_scaling, partial_rotary_factor), _stream(stream, index))
 
+    def _empty(self, shape, dtype, stream):
+        """Memory of the stream that the kernel runs on: another stream's block of the caching allocator may still be in use there."""
+        if stream is None:
+            return _torch.empty(shape, dtype=dtype, device=self.device)
+        with _torch.cuda.stream(_torch.cuda.ExternalStream(stream, device=self.device) if isinstance(stream, int) else stream):
+            return _torch.empty(shape, dtype=dtype, device=self.device)
+
     def _attention(self, fn, size_fn, q, out, block_tables, kv_lens, query_starts, query_len, max_query_len, softmax_scale, sliding_window, stream):
         index = self._index
         kind = _type(q, "q")
         if out is None:
-            out = _torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = self._empty(q.shape, q.dtype, stream)
+            if stream is not None:       # the caller's stream will read it
+                out.record_stream(_torch.cuda.current_stream(index))
         qp, qt, qh, tokens, heads = _rows(q, "q", index, None, self.head_dim)
         op, ot, oh, *shape = _rows(out, "out", index, q.dtype, self.head_dim)
         if shape != [tokens, heads]:
@@ -217,11 +227,7 @@ class BlockScaledKVCache:
                 qp, op, qt, qh, ot, oh, starts, tokens, heads, query_len, max_query_len, kind, softmax_scale, sliding_window, 0, 0))
         work = None
         if size:
-            if stream is None:
-                work = _torch.empty(size, dtype=_torch.uint8, device=self.device)
-            else:
-                with _torch.cuda.stream(_torch.cuda.ExternalStream(stream, device=self.device) if isinstance(stream, int) else stream):
-                    work = _torch.empty(size, dtype=_torch.uint8, device=self.device)
+            work = self._empty((size,), _torch.uint8, stream)
         _call(fn, index, view, _ATTENTION.pack(qp, op, qt, qh, ot, oh, starts, tokens, heads, query_len, max_query_len, kind, softmax_scale, sliding_window,
                                                work.data_ptr() if size else 0, size), _stream(stream, index))
         return out

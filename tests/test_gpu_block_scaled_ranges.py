@@ -94,3 +94,19 @@ def test_append_of_tiny_rows(er, torch, fmt, t):  # noqa: F811
     step = scale / 2 if fmt == "int8" else torch.maximum(want.abs() * 2.0 ** -4, scale * 2.0 ** -10)
     # the norm factor is off by a few steps of float32; a decoded value below 2^-126 may be flushed
     assert bool(((got - want).abs() <= step * (1 + 1e-4) + want.abs() * 2.0 ** -20 + 2.0 ** -126).all())
+
+
+def test_the_output_of_a_call_on_another_stream_is_that_streams_memory(er, torch):  # noqa: F811
+    """Without `out` the output comes from the memory of the stream that the kernel runs on: a block of the current stream's may still be in use there."""
+    cache, table, rows = fill(er, torch, "e4m3", [40], 16, 2, 64, 16)
+    other = torch.cuda.Stream()
+    q, starts, lens = torch.randn(1, 4, 64, device="cuda"), ints(torch, [0, 1]), ints(torch, [40])
+    torch.cuda.synchronize()
+    for stream in (other, other.cuda_stream):
+        for out in (cache.attention_decode(q, table, lens, stream=stream), cache.attention_prefill(q, starts, table, lens, stream=stream)):
+            at = out.data_ptr()
+            owner = [s["stream"] for s in torch.cuda.memory_snapshot() if s["address"] <= at < s["address"] + s["total_size"]]
+            assert owner == [other.cuda_stream]
+            other.synchronize()
+            want, big = ref_attention(torch, q, *rows[0], 40, 64 ** -0.5)
+            check_attention(torch, out, want, big, "f32")
