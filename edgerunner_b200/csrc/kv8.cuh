@@ -223,6 +223,9 @@ __device__ __forceinline__ int kv8_find_slot(const int32_t* starts, int num_seqs
     }
     return lo;
 }
+// The first row that a query at position `pos` sees (window 0: all up to it).  A query in front of row 0 has a negative position, and pos - window + 1 need not
+// fit an int then.
+__device__ __forceinline__ int kv8_first_seen(int pos, int window) { return window > 0 && pos >= window ? pos - window + 1 : 0; }
 __device__ __forceinline__ void kv8_report(const Kv8Cache& c, int code) {
     if (c.status != nullptr) atomicExch(c.status, code);
 }

@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     if (tile.rows == 0) return;
     const int past = tile.len - tile.n, last_row = min(tile.rows, tile.row0 + 256) - 1;
     const int hi = min(tile.len, past + last_row / p.group + 1);  // keys below it
-    const int lo = p.window > 0 ? max(0, past + tile.row0 / p.group - p.window + 1) : 0;
+    const int lo = kv8_first_seen(past + tile.row0 / p.group, p.window);
     int t_begin = lo / kTok, tiles = max(0, (hi + kTok - 1) / kTok - t_begin);
     if (parts > 1) {
         const int per = (tiles + parts - 1) / parts, b = min(tiles, part * per);
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             if (lane == 0) mbar_arrive(bars + kBarQ);
         }
         const int limit = min(tile.len - 1, past + qi);
-        const int lower = p.window > 0 ? past + qi - p.window + 1 : 0;
+        const int lower = kv8_first_seen(past + qi, p.window);
         float m = -INFINITY, l = 0.f, LR = -200.f;
         for (int j = 0; j < tiles; ++j) {
             const int t0 = (t_begin + j) * kTok;

@@ -110,3 +110,20 @@ def test_the_output_of_a_call_on_another_stream_is_that_streams_memory(er, torch
             other.synchronize()
             want, big = ref_attention(torch, q, *rows[0], 40, 64 ** -0.5)
             check_attention(torch, out, want, big, "f32")
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("window", [0x7FFFFFFF, 0x7FFFFFFF - 40, 1 << 30])
+def test_windows_wider_than_any_sequence(er, torch, t, window):  # noqa: F811
+    """The same as no window, also for queries in front of row 0."""
+    cache, table, rows = fill(er, torch, "int8", [70, 300], 16, 2, 64, 16)
+    q = torch.randn(120, 4, 64, generator=gen(torch, 2), device="cuda").to(dtype(torch, t))
+    for lens in ([70, 300], [9, 20], [0, 300]):
+        args = (table, ints(torch, lens))
+        starts = ints(torch, [0, 100, 120])
+        assert torch.equal(cache.attention_prefill(q, starts, *args, sliding_window=window), cache.attention_prefill(q, starts, *args))
+        assert torch.equal(cache.attention_decode(q[:32], *args, query_len=16, sliding_window=window), cache.attention_decode(q[:32], *args, query_len=16))
+    got = cache.attention_prefill(q, starts, table, ints(torch, [9, 20]), sliding_window=window)
+    want, big = ref_attention(torch, q[91:100], rows[0][0][:9], rows[0][1][:9], 9, 64 ** -0.5)
+    check_attention(torch, got[91:100], want, big, t)
+    assert bool((got[:91] == 0).all())
