@@ -223,9 +223,6 @@ __device__ __forceinline__ int kv8_find_slot(const int32_t* starts, int num_seqs
     }
     return lo;
 }
-// The first row that a query at position `pos` sees (window 0: all up to it).  A query in front of row 0 has a negative position, and pos - window + 1 need not
-// fit an int then.
-__device__ __forceinline__ int kv8_first_seen(int pos, int window) { return window > 0 && pos >= window ? pos - window + 1 : 0; }
 __device__ __forceinline__ void kv8_report(const Kv8Cache& c, int code) {
     if (c.status != nullptr) atomicExch(c.status, code);
 }
@@ -264,6 +261,12 @@ inline cudaError_t kv8_allow_smem(Kernel kernel, int most, std::atomic<uint64_t>
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e == cudaSuccess && device < 64) devices.fetch_or(1ull << device, std::memory_order_release);
     return e;
+}
+// The window as the kernels take it: 0 (none) where no sequence is longer.  kv8_check_attention keeps position - window, with positions down to -num_tokens
+// for queries in front of row 0, inside an int.
+inline uint64_t kv8_table_rows(const er_kv8_cache* c) { return static_cast<uint64_t>(c->block_table_width) * c->page_size; }
+inline int kv8_window(const er_kv8_cache* c, const er_kv8_attention_params* u) {
+    return u->sliding_window >= kv8_table_rows(c) ? 0 : static_cast<int>(u->sliding_window);
 }
 inline float kv8_scale_log2(float softmax_scale, uint32_t head_dim) {       // scores in units of log2
     return (softmax_scale > 0.f ? softmax_scale : 1.f / std::sqrt(static_cast<float>(head_dim))) * 1.4426950408889634f;

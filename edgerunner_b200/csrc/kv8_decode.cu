@@ -67,7 +67,8 @@ __device__ __forceinline__ SeqRange seq_range(const Kv8Decode& p, int seq) {
     r.row_tiles = (r.n * p.group + p.tile_rows - 1) / p.tile_rows;
     if (p.few_rows > 0 && r.n * p.group > p.few_rows) r.row_tiles = 0;
     r.len = max(0, min(__ldg(p.cache.lens + seq), p.cache.table_width * p.cache.page_size));   // rows behind the table have no page
-    r.first_unit = kv8_first_seen(r.len - r.n, p.window) / kUnit;
+    const int lo = p.window > 0 ? max(0, r.len - r.n - p.window + 1) : 0;
+    r.first_unit = lo / kUnit;
     r.units = max(1, (r.len + kUnit - 1) / kUnit - r.first_unit);
     return r;
 }
@@ -88,7 +89,7 @@ struct Place {        // a position in the list
         return (min(r.n * p.group, (item % r.row_tiles + 1) * p.tile_rows) - 1) / p.group;
     }
     // The first row that the tile sees: pages in front of it may be gone.
-    __device__ __forceinline__ int lowest(const Kv8Decode& p) const { return kv8_first_seen(r.len - r.n + first_query(p), p.window); }
+    __device__ __forceinline__ int lowest(const Kv8Decode& p) const { return p.window > 0 ? max(0, r.len - r.n + first_query(p) - p.window + 1) : 0; }
     // Of the `count` units from `unit` on, those [u0, u1) that the tile sees anything of.
     __device__ __forceinline__ void visible(const Kv8Decode& p, int count, int& u0, int& u1) const {
         const int base = r.first_unit + unit, end = r.len - r.n + last_query(p) + 1;      // rows below `end`
@@ -369,7 +370,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
         const int past = at.r.len - at.r.n;            // position of query 0
         int u0, u1;
         at.visible(p, seg, u0, u1);
-        const int all_see_to = past + at.first_query(p), all_see_from = kv8_first_seen(past + at.last_query(p), p.window);
+        const int all_see_to = past + at.first_query(p), all_see_from = past + at.last_query(p) - p.window + 1;
         // ---- queries of this lane's column g: dims [D/4 t, D/4 (t+1)), scaled to at most 1 by a power of two ----
         uint32_t qh[NT][KK][2], ql[kSplit ? NT : 1][kSplit ? KK : 1][2];
         float qscale[NT][2];        // of the columns 2t, 2t + 1
@@ -459,7 +460,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
                     for (int e = 0; e < 4; ++e) s[h][nt][e] = (s[h][nt][e] + s2[nt][e]) * (kscale[h] * qscale[nt][e & 1]);
             }
             // ---- online softmax; lane's scores: tokens g, g + 8 of each half, of the columns 2t, 2t + 1 ----
-            const bool edge = fminf(kscale[0], kscale[1]) < 0.f || tok0 + kUnit - 1 > all_see_to || tok0 < all_see_from;
+            const bool edge = fminf(kscale[0], kscale[1]) < 0.f || tok0 + kUnit - 1 > all_see_to || (p.window > 0 && tok0 < all_see_from);
             if (edge) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
@@ -468,7 +469,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int tok = tok0 + h * kKv8Unit + g + 8 * (e >> 1), lim = limit[nt][e & 1];
-                            if (kscale[h] < 0.f || tok > lim || tok < kv8_first_seen(lim, p.window)) s[h][nt][e] = -INFINITY;
+                            if (kscale[h] < 0.f || tok > lim || (p.window > 0 && tok <= lim - p.window)) s[h][nt][e] = -INFINITY;
                         }
             }
             bool rise = fmaxf(vscale[0], vscale[1]) > R;
@@ -827,6 +828,8 @@ int32_t kv8_check_attention(const er_kv8_cache* c, const er_kv8_attention_params
     if (!kv8_rows_apart(u->out_token_stride, u->out_head_stride, u->num_tokens, u->num_heads, c->head_dim)) return report_error(ER_ERR_SHAPE, "rows of out overlap");
     if (!(u->softmax_scale >= 0.f && std::isfinite(u->softmax_scale))) return report_error(ER_ERR_INVALID_ARGUMENT, "softmax_scale must be finite and not negative");
     if (u->num_tokens > 0x7FFFFF00u || u->sliding_window > 0x7FFFFFFFu) return report_error(ER_ERR_UNSUPPORTED, "num_tokens or sliding_window beyond 2^31");
+    if (u->sliding_window > 0 && u->sliding_window < kv8_table_rows(c) && kv8_table_rows(c) + u->num_tokens > 0x7FFFFFFFull)
+        return report_error(ER_ERR_UNSUPPORTED, "with a window, num_tokens and the rows that a block table addresses must stay below 2^31 together");
     return ER_OK;
 }
 
@@ -864,7 +867,7 @@ int32_t kv8_launch_decode(const Kv8Cache& cache, const er_kv8_cache* c, const er
     p.num_tokens = static_cast<int>(u->num_tokens);
     p.few_rows = few_rows;
     p.group = static_cast<int>(u->num_heads) / cache.num_kv_heads;
-    p.query_len = static_cast<int>(u->query_len); p.window = static_cast<int>(u->sliding_window);
+    p.query_len = static_cast<int>(u->query_len); p.window = kv8_window(c, u);
     if (!encode_rows(&p.maps[0], cache.codes[0], cache, static_cast<int>(c->head_dim)) || !encode_rows(&p.maps[1], cache.codes[1], cache, static_cast<int>(c->head_dim)))
         return report_error(ER_ERR_CUDA, "cuTensorMapEncodeTiled refused the cache's shape");
     p.scale_log2 = kv8_scale_log2(u->softmax_scale, c->head_dim);

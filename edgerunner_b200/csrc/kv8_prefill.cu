@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     if (tile.rows == 0) return;
     const int past = tile.len - tile.n, last_row = min(tile.rows, tile.row0 + 256) - 1;
     const int hi = min(tile.len, past + last_row / p.group + 1);  // keys below it
-    const int lo = kv8_first_seen(past + tile.row0 / p.group, p.window);
+    const int lo = p.window > 0 ? max(0, past + tile.row0 / p.group - p.window + 1) : 0;
     int t_begin = lo / kTok, tiles = max(0, (hi + kTok - 1) / kTok - t_begin);
     if (parts > 1) {
         const int per = (tiles + parts - 1) / parts, b = min(tiles, part * per);
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             if (lane == 0) mbar_arrive(bars + kBarQ);
         }
         const int limit = min(tile.len - 1, past + qi);
-        const int lower = kv8_first_seen(past + qi, p.window);
+        const int lower = p.window > 0 ? past + qi - p.window + 1 : 0;
         float m = -INFINITY, l = 0.f, LR = -200.f;
         for (int j = 0; j < tiles; ++j) {
             const int t0 = (t_begin + j) * kTok;
@@ -747,7 +747,7 @@ extern "C" int32_t er_kv8_attention_prefill(const er_kv8_cache* cache, const er_
         p.partial = static_cast<float*>(u->workspace);
         p.num_tokens = static_cast<int>(u->num_tokens);
         p.group = static_cast<int>(u->num_heads) / c.num_kv_heads;
-        p.window = static_cast<int>(u->sliding_window);
+        p.window = kv8_window(cache, u);
         p.min_rows = sp.few ? kFewRows + 1 : 0;      // a hint that is wrong costs time, not rows
         p.group_magic = p.group == 1 ? 0 : ~0ull / static_cast<uint64_t>(p.group) + 1;
         p.scale_log2 = kv8_scale_log2(u->softmax_scale, cache->head_dim);

@@ -503,7 +503,8 @@ typedef struct {
 int32_t er_kv8_append(const er_kv8_cache* cache, const er_kv8_append_params* params, void* stream);
 
 /* Attention over the cache: query i of a sequence with n queries sits at position p = kv_lens - n + i and sees the rows
- * max(0, p - sliding_window + 1) .. p (sliding_window 0: 0 .. p).  A query that sees nothing gets zeros.  softmax_scale 0 ->
+ * max(0, p - sliding_window + 1) .. p (sliding_window 0: 0 .. p; a window needs num_tokens and the rows that a block table addresses to
+ * stay below 2^31 together, one that no sequence outgrows is the same as 0).  A query that sees nothing gets zeros.  softmax_scale 0 ->
  * 1 / sqrt(head_dim).  num_heads is a multiple of num_kv_heads, any group.
  * er_kv8_attention_decode: query_len tokens for every sequence (1 to 16; query token s * query_len + i), the work split over the GPU
  * along the rows; accuracy follows the type (float32: queries and probabilities enter the tensor cores as two halves each).

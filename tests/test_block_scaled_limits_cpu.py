@@ -63,3 +63,15 @@ def test_norm_refuses_more_tokens_than_its_counter_holds(er):  # noqa: F811
     import torch
     if not torch.cuda.is_available():
         assert er.lib().er_qk_norm_rope(C.byref(norm(num_tokens=0x7FFF0000)), None) == -8      # past the checks of arguments: no device
+
+
+def test_attention_refuses_windows_whose_arithmetic_leaves_an_int(er):  # noqa: F811
+    """Positions go down to -num_tokens (more queries than rows), and the window is subtracted from them."""
+    wide = dict(block_table_width=0x7FFFFF00 // 32, block_table_stride=0x7FFFFF00 // 32, num_seqs=1)
+    fn = er.lib().er_kv8_attention_prefill
+    assert fn(C.byref(cache(**wide)), C.byref(attention(num_tokens=512, sliding_window=0x7FFFFEFF)), None) == UNSUPPORTED
+    assert fn(C.byref(cache(**wide)), C.byref(attention(num_tokens=512, sliding_window=5)), None) == UNSUPPORTED
+    import torch
+    if not torch.cuda.is_available():       # past the checks of arguments: no device
+        for tokens, window in ((512, 0), (512, 0x7FFFFFFF), (255, 0x7FFFFEFF)):
+            assert fn(C.byref(cache(**wide)), C.byref(attention(num_tokens=tokens, sliding_window=window)), None) == -8
