@@ -3,8 +3,8 @@
 // Mathematics.  With codes c and block scales a (keys) and b (values), row i of a block:  s_i = (q . ck_i) a scale,  o = sum_i p_i b cv_i /
 // sum_i p_i,  p_i = exp(s_i - m).  Codes are exact in fp16, so both contractions run on mma.sync.m16n8k16 with fp16 operands and float32
 // accumulators; the key scale multiplies the score, the value scale the probability.  The probabilities that enter the second product are
-// w = p * b / R with R the largest value scale so far (so w <= 1 whatever the scales are), carried 4096 times so that small ones stay normal
-// fp16 numbers; R and m move together and rarely.
+// w = p * b / R with R the power of two next above the largest value scale that the query has seen so far (so w <= 1 whatever the scales are), carried 4096
+// times so that small ones stay normal fp16 numbers; R and m move together and rarely.
 //
 // Work.  Bound by memory: 2 D bytes a row for 4 D flops a query head.  A persistent CTA per SM; the list of 32-token units of all (sequence, kv head,
 // row tile) items is cut evenly over the CTAs whatever the lengths are, inside a CTA the units of an item go round robin to the warps.  A warp
@@ -32,7 +32,8 @@ namespace {
 
 constexpr int kMinUnits = 8;          // units of a CTA, so that short work stays together
 constexpr int kUnit = 2 * kKv8Unit;   // tokens that a warp takes at a time: two halves, each with a page and scales of its own
-constexpr float kWeightScale = 4096.f;
+constexpr float kWeightScale = 4096.f;    // 2^12
+constexpr float kLift0 = 8.507059173023462e37f;    // 2^126: scales up to 2^-114 need no less
 
 struct Kv8Decode {
     CUtensorMap maps[2];            // codes of the keys, values as [rows][head_dim], boxes of 16 rows
@@ -205,6 +206,13 @@ __device__ __forceinline__ void split_half2(float a, float b, uint32_t& hi, uint
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = half2_bits(a - f.x, b - f.y);
 }
+
+// 2^12 over the power of two next above (or at) a value scale.  Scales from 2^-126 (smaller ones count as 0) to 2^126.
+__device__ __forceinline__ float lift_below(float scale) {
+    const uint32_t b = __float_as_uint(scale), e = min((b >> 23) + ((b & 0x7FFFFFu) != 0u ? 1u : 0u), 253u);
+    return __uint_as_float(min(266u - e, 253u) << 23);
+}
+__device__ __forceinline__ float inverse_lift(float lift) { return __uint_as_float(0x7F000000u - __float_as_uint(lift)); }
 
 // A stage: keys of the two halves, values of the two halves.
 template <int D> struct Stage {
@@ -404,7 +412,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
                 limit[nt][j] = past + min(rr, rows - 1) / p.group;
             }
         }
-        float o[NT][MT][4], m[NT][2], l[NT][2], R = 0.f, inv_R = 0.f;
+        float o[NT][MT][4], m[NT][2], l[NT][2], lift[NT][2];    // lift: 4096 / R, powers of two
         float keep[kSplit ? MT : 1][4];     // float32: the tensor cores' sums are moved here every 8 units (their accumulators round towards zero)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -412,6 +420,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
             for (int i = 0; i < MT; ++i) { o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f; }
             m[nt][0] = m[nt][1] = -INFINITY;
             l[nt][0] = l[nt][1] = 0.f;
+            lift[nt][0] = lift[nt][1] = kLift0;
         }
 #pragma unroll
         for (int i = 0; i < (kSplit ? MT : 1); ++i) keep[i][0] = keep[i][1] = keep[i][2] = keep[i][3] = 0.f;
@@ -472,7 +481,9 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
                             if (kscale[h] < 0.f || tok > lim || (p.window > 0 && tok <= lim - p.window)) s[h][nt][e] = -INFINITY;
                         }
             }
-            bool rise = fmaxf(vscale[0], vscale[1]) > R;
+            bool rise = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) rise |= fmaxf(vscale[0], vscale[1]) * fmaxf(lift[nt][0], lift[nt][1]) > kWeightScale;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -481,7 +492,6 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
             for (int h = 0; h < 2; ++h)
                 if (!(vscale[h] >= 1.17549435e-38f)) vscale[h] = isnan(vscale[h]) ? vscale[h] : 0.f;
             if (__any_sync(0xffffffffu, rise)) {
-                const float R_new = fmaxf(R, fmaxf(vscale[0], vscale[1])), down = R > 0.f ? R / R_new : 0.f;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float corr[2];
@@ -494,7 +504,15 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
                         corr[j] = mx == -INFINITY ? 1.f : fast_exp2(m[nt][j] - mx);
                         m[nt][j] = mx;
                         l[nt][j] *= corr[j];
-                        corr[j] *= down;
+                        float top = 0.f;        // the largest value scale that the column sees: a block that it does not see may be of any size
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int from = tok0 + h * kKv8Unit, lim = limit[nt][j];
+                            if (!edge || (from <= lim && !(p.window > 0 && from + kKv8Unit - 1 <= lim - p.window))) top = fmaxf(top, vscale[h]);
+                        }
+                        const float old = lift[nt][j];
+                        lift[nt][j] = top * old > kWeightScale ? lift_below(top) : old;
+                        corr[j] *= lift[nt][j] * inverse_lift(old);
                     }
 #pragma unroll
                     for (int i = 0; i < MT; ++i) {
@@ -505,13 +523,10 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
                         }
                     }
                 }
-                R = R_new;
-                inv_R = R > 0.f ? 1.f / R : 0.f;
             }
             uint32_t wh[2][NT][2], wl[2][kSplit ? NT : 1][2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float wf = vscale[h] * inv_R * kWeightScale;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float w[4];
@@ -519,7 +534,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
                     for (int e = 0; e < 4; ++e) {
                         const float pr = fast_exp2(s[h][nt][e] - (m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1]));
                         l[nt][e & 1] += pr;
-                        w[e] = pr * wf;
+                        w[e] = pr * (vscale[h] * lift[nt][e & 1]);
                         if (edge && s[h][nt][e] == -INFINITY) w[e] = 0.f;      // a hidden row of a block with a NaN scale weighs nothing
                     }
 #pragma unroll
@@ -595,9 +610,9 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
             load_queries();
         }
         // ---- join the warps of the CTA ----
-        const float out_scale = R * (1.f / kWeightScale);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
+            const float back[2] = {inverse_lift(lift[nt][0]), inverse_lift(lift[nt][1])};
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 4);
@@ -609,7 +624,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if constexpr (kSplit) o[nt][i][e] += keep[i][e];
-                    o[nt][i][e] *= out_scale;
+                    o[nt][i][e] *= back[e & 1];
                 }
             }
         }

@@ -2,9 +2,9 @@
 // block-scaled paged cache.
 //
 // Mathematics.  s = (q . ck) a scale with a the key scale of 16 or more rows, w = 2^(s log2 e - m) b / R with b the value scale and R a power of two near
-// the largest one so far, o = R sum_i w_i cv_i / sum_i (w_i R / b_i).  Codes are exact in fp16, q and w are rounded to it, sums are float32.  Neither scale
-// costs an operation a score: a multiplies the factor inside exp2's argument, log2(b / R) is part of its offset, and the sum of 16 weights is
-// divided by b / R once.
+// the largest one so far of the blocks that the row sees, o = R sum_i w_i cv_i / sum_i (w_i R / b_i).  Codes are exact in fp16, q and w are rounded to
+// it, sums are float32.  Neither scale costs an operation a score: a multiplies the factor inside exp2's argument, log2(b / R) is part of its offset,
+// and the sum of 16 weights is divided by b / R once.
 //
 // One CTA owns two tiles of 128 query rows of a (sequence, kv head): row r is query r / group, head r % group, any group.  The tensor pipe takes 1024
 // clocks for 128 tokens of a tile, exp2 (16 a clock and SM) as long, so the two tiles take turns: while one is in its softmax the products of the other run.
@@ -437,6 +437,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                 vm = fmaxf(vm, sc[8 + g]);
             }
             const bool edge = __any_sync(0xffffffffu, kmin < 0.f || t0 + kTok - 1 > limit || t0 < lower);
+            if (edge) {         // only the blocks that this row sees: one that it does not may be of any size
+                vm = -INFINITY;
+#pragma unroll
+                for (int g = 0; g < 8; ++g)
+                    if (t0 + 16 * g <= limit && t0 + 16 * g + 15 >= lower) vm = fmaxf(vm, sc[8 + g]);
+            }
             // The columns of chunk c0 .. c0 + 32 that this row sees, one bit each.
             auto seen = [&](int c0) {
                 const int from = min(max(lower - t0 - c0, 0), 32), to = min(max(limit + 1 - t0 - c0, 0), 32);

@@ -7,7 +7,7 @@ import math
 
 import pytest
 
-from test_gpu_block_scaled import check_attention, dtype, er, fill, gen, half_step, ints, make_cache, ref_attention, tables, torch  # noqa: F401
+from test_gpu_block_scaled import check_attention, dtype, er, fill, gen, half_step, ints, ref_attention, torch  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -127,3 +127,48 @@ def test_windows_wider_than_any_sequence(er, torch, t, window):  # noqa: F811
     want, big = ref_attention(torch, q[91:100], rows[0][0][:9], rows[0][1][:9], 9, 64 ** -0.5)
     check_attention(torch, got[91:100], want, big, t)
     assert bool((got[:91] == 0).all())
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("op", ["decode", "prefill"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("where", ["later", "left"])
+def test_hidden_blocks_with_large_values(er, torch, t, op, dim, where):  # noqa: F811
+    """A block whose value scale is 2^40 times the others' costs those queries nothing that do not see it: those in front of it, or (`left`) those whose
+    window has left it behind."""
+    if op == "decode":
+        length, n, block, window = (100, 8, 96, 0) if where == "later" else (100, 8, 64, 20)
+    else:
+        length, n, block, window = (300, 200, 272, 0) if where == "later" else (200, 200, 16, 50)
+    cache, table, _ = fill(er, torch, "e4m3", [length], 16, 2, dim, 16)
+    cache.value_scales[int(table[0, block // 16])] *= 2.0 ** 40
+    k, v = rows_of(cache, table[0], length)
+    q = torch.randn(n, 8, dim, generator=gen(torch, 2), device="cuda").to(dtype(torch, t))
+    pos = torch.arange(length - n, length, device="cuda")
+    sees = (pos >= block) & ((pos - window + 1 <= block + 15) if window else True)
+    assert bool(sees.any()) and bool((~sees).any())
+    got = (cache.attention_decode(q, table, ints(torch, [length]), query_len=n, sliding_window=window) if op == "decode" else
+           cache.attention_prefill(q, ints(torch, [0, n]), table, ints(torch, [length]), sliding_window=window))
+    want, big = ref_attention(torch, q, k, v, length, dim ** -0.5, window)
+    check_attention(torch, got[~sees], want[~sees], big[~sees], t)
+    if t != "f16":          # beyond its range
+        check_attention(torch, got[sees], want[sees], big[sees], t)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("op", ["decode", "prefill"])
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_value_scales_over_forty_powers_of_two(er, torch, t, op, fmt):  # noqa: F811
+    """Within float16's range of outputs; the bound is relative to the largest value that the query sees."""
+    length, n = 700, 8 if op == "decode" else 150
+    cache, table, _ = fill(er, torch, fmt, [length], 16, 2, 64, 16)
+    g = gen(torch, 4)
+    cache.value_scales.copy_(torch.exp2(torch.randint(-40, 1, cache.value_scales.shape, generator=g, device="cuda").float()))
+    k, v = rows_of(cache, table[0], length)
+    q = torch.randn(n, 8, 64, generator=g, device="cuda").to(dtype(torch, t))
+    for window in (0, 70):
+        got = (cache.attention_decode(q, table, ints(torch, [length]), query_len=n, sliding_window=window) if op == "decode" else
+               cache.attention_prefill(q, ints(torch, [0, n]), table, ints(torch, [length]), sliding_window=window))
+        want, big = ref_attention(torch, q, k, v, length, 64 ** -0.5, window)
+        assert float(want.abs().max()) < 60000
+        check_attention(torch, got, want, big, t)
