@@ -218,7 +218,7 @@ class BlockScaledKVCache:
         if tokens == 0:
             return out
         # a fresh block of the caching allocator for each call: calls on different streams never share one, and a captured call keeps its own
-        key = (n, block_tables.shape[1], tokens, heads, query_len, max_query_len, kind)
+        key = (n, block_tables.shape[1], tokens, heads, query_len, max_query_len, kind, sliding_window)
         size = self._workspace_bytes.get(key)
         if size is None:
             if len(self._workspace_bytes) > 256:
@@ -227,7 +227,7 @@ class BlockScaledKVCache:
                 qp, op, qt, qh, ot, oh, starts, tokens, heads, query_len, max_query_len, kind, softmax_scale, sliding_window, 0, 0))
         work = None
         if size:
-            work = self._empty((size,), _torch.uint8, stream)
+            work = _torch.empty(size, dtype=_torch.uint8, device=self.device) if stream is None else self._empty((size,), _torch.uint8, stream)
         _call(fn, index, view, _ATTENTION.pack(qp, op, qt, qh, ot, oh, starts, tokens, heads, query_len, max_query_len, kind, softmax_scale, sliding_window,
                                                work.data_ptr() if size else 0, size), _stream(stream, index))
         return out

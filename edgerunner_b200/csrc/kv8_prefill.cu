@@ -38,6 +38,12 @@ constexpr int kTok = 128;                  // tokens of a K / V tile
 constexpr int kSoftWarps = 8, kLoadWarps = 7, kIssueWarp = 12;   // loaders: warps 8-11 and 13-15
 constexpr int kThreads = 512;
 constexpr float kLag = 8.f;                // how far (log2) a row's maximum may rise above the one in use
+// The tensor cores add into their accumulators with truncation, up to 2^-23 of the sum for each 16 keys, which biases a long chain (keys around 500000, values
+// around 1: 3.2e-3 low; 131072 keys: 7.7e-4).  After this many tiles (16384 keys: 1.2e-4 at most, measured 6e-5) a row's O is added to a float32 sum in memory
+// and starts again.  A kernel of its own, for tables and windows that reach that far: the code alone, without a fold, costs a short prompt 12.3 -> 13.4 us,
+// ragged prompts 148 -> 153.
+constexpr int kFold = 128;
+constexpr int kMostFoldSlots = 256;
 constexpr float kCarry = 5.f;              // weights are carried 2^5 times: w <= 2^(8 + 2 + 5) < 65504
 template <int D> __host__ __device__ constexpr int stage_count() { return D == 128 ? 5 : 8; }
 // Slots for the scales of a tile's blocks.  The loader of key tile j waits for the ring entry that it fills, not for the scale slot.  With an even number of
@@ -47,6 +53,8 @@ template <int D> __host__ __device__ constexpr int stage_count() { return D == 1
 template <int D> __host__ __device__ constexpr int scale_slots() { return stage_count<D>() / 2 + 1; }
 constexpr int kMostScaleSlots = 5;
 template <int D> __host__ __device__ constexpr int tile_bytes() { return kTok * D * 2; }   // also a tile of 128 query rows
+// Floats of a CTA's sums: D / 4 groups of columns of 256 rows, then the maximum and the log2 of R that they stand for.
+template <int D> __host__ __device__ constexpr int fold_floats() { return 256 * (D + 2); }
 template <int D> __host__ __device__ constexpr int prefill_smem() { return (stage_count<D>() + 2) * tile_bytes<D>() + 256 + kMostScaleSlots * 32 * 4 + 1024; }
 
 struct Kv8Prefill {
@@ -56,6 +64,8 @@ struct Kv8Prefill {
     int64_t q_token, q_head, out_token, out_head;
     const int32_t* starts;
     float* partial;             // of the split tiles: [index][256 rows][D + 4]: max, sum, -, -, unnormalised row
+    float* fold;                // sums of long contexts: [fold_slots][fold_floats], or nullptr: no CTA has more than kFold tiles
+    int fold_slots;             // as many as CTAs can run at a time
     int num_tokens, group, window, min_rows;    // sequences with fewer query rows are somebody else's
     int slots, split_from, parts;               // CTAs [0, split_from) own a tile pair, the others a part of its keys
     float scale_log2;
@@ -87,6 +97,17 @@ __device__ __forceinline__ Tile find_tile(const Kv8Prefill& p, int slot) {
     t.wrong = t.len > most ? ER_ERR_OUT_OF_PAGES : t.len < 0 ? ER_ERR_SHAPE : 0;
     t.len = max(0, min(t.len, most));
     return t;
+}
+
+// Which of the slots for sums are in use, by the running CTAs of all calls on the device: one fits an SM, so that a slot for each SM is enough, and a call's
+// workspace need not hold one for every CTA of its grid.  A slot decides where a CTA keeps its sums, not what they are.
+__device__ unsigned int fold_claims[kMostFoldSlots / 32];
+__device__ int claim_fold_slot(int slots) {
+    for (int k = 0; k < 4 * slots; ++k) {
+        const int s = (static_cast<int>(blockIdx.x % static_cast<unsigned>(slots)) + k) % slots;
+        if ((atomicOr(&fold_claims[s >> 5], 1u << (s & 31)) >> (s & 31) & 1u) == 0u) return s;
+    }
+    return -1;      // not with a CTA an SM; the sums would stay in tensor memory
 }
 
 // r / group by a multiplication (exact below 2^30)
@@ -139,13 +160,13 @@ __device__ __forceinline__ uint32_t half2_word(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-template <typename T, int D, bool E4M3>
+template <typename T, int D, bool E4M3, bool Fold>
 __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_constant__ Kv8Prefill p) {
     constexpr int kStages = stage_count<D>(), kScaleRing = scale_slots<D>(), kTile = tile_bytes<D>(), kRegion = kTok * 128;   // a region: 128 rows x 64 halves
     constexpr int kBarFull = 0, kBarEmpty = kStages, kBarS = 2 * kStages, kBarP = kBarS + 2, kBarQ = kBarP + 2, kBarO = kBarQ + 1, kBarScale = kBarO + 1,
                   kBarRead = kBarScale + kScaleRing, kNumBars = kBarRead + 2;
     constexpr uint32_t kColO = 256, kColW = D == 128 ? 0 : 384, kStrideW = D == 128 ? 128 : 64;   // tensor-memory columns
-    static_assert(kNumBars * 8 + 8 <= 256, "");
+    static_assert(kNumBars * 8 + 12 <= 256, "");
     static_assert(kScaleRing > kStages / 2 && kScaleRing <= kMostScaleSlots, "scales would be overwritten while the softmax reads them");
     extern __shared__ uint8_t raw[];
     const Kv8Cache& c = p.cache;
@@ -155,6 +176,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     uint64_t* bars = reinterpret_cast<uint64_t*>(q_gen + 2 * kTile);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kNumBars);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* fold_slot = abort_flag + 1;
     float* scale_ring = reinterpret_cast<float*>(q_gen + 2 * kTile + 256);   // [ring][key scale x 8, log2 of the value scale x 8, 1 / it x 8, -]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -190,6 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             mbar_init(bars + i, n);
         }
         *abort_flag = 0;
+        if constexpr (Fold) *fold_slot = tiles > kFold ? claim_fold_slot(p.fold_slots) : -1;
         mbar_init_fence();
     }
     if (warp == kIssueWarp) {
@@ -200,6 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    const int folding = Fold ? *fold_slot : -1;         // negative: not
     const Waiter wait{abort_flag, &c};
     // Codes -> fp16 operand tiles.  The 16-token units of the half tiles (keys of tile 0, values of tile 0, keys of tile 1, ...; eight to a half
     // tile) go round robin to the loader warps, each with the codes of its next unit on the way in registers and the page of the one behind it looked
@@ -334,7 +358,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                 full(vi);
                 wait(bars + kBarP, j & 1);
                 tc_fence_after();
-                outputs(0, vi, j == 0);
+                const bool fresh = Fold && folding >= 0 ? j % kFold == 0 : j == 0;
+                outputs(0, vi, fresh);
                 if (more) {
                     full(ki);
                     read(0, j);
@@ -343,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                 if (two) {
                     wait(bars + kBarP + 1, j & 1);
                     tc_fence_after();
-                    outputs(1, vi, j == 0);
+                    outputs(1, vi, fresh);
                 }
                 release(vi);
                 if (more) {
@@ -426,6 +451,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         const int limit = min(tile.len - 1, past + qi);
         const int lower = p.window > 0 ? past + qi - p.window + 1 : 0;
         float m = -INFINITY, l = 0.f, LR = -200.f;
+        // This thread's row of the sums; what they count now, if they have been begun.
+        float* const sums = p.fold + static_cast<int64_t>(max(folding, 0)) * fold_floats<D>();
+        float4* const sum_row = reinterpret_cast<float4*>(sums) + i * 128 + m_row;
+        float* const sum_max = sums + 256 * D + i * 128 + m_row;
+        auto counts = [&]() {
+            const float was = __ldcg(sum_max);
+            return was == -INFINITY ? 0.f : fast_exp2(was - m) * fast_exp2(__ldcg(sum_max + 256) - LR);
+        };
         for (int j = 0; j < tiles; ++j) {
             const int t0 = (t_begin + j) * kTok;
             wait(bars + kBarScale + j % kScaleRing, (j / kScaleRing) & 1);
@@ -491,6 +524,29 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                 if (c0 > 0) tmem_ld32_nowait(tm_s + 32, b);
             }
             mx *= factor;
+            // ---- after kFold tiles: O joins the sums in memory and begins anew ----
+            const bool fold = Fold && folding >= 0 && j > 0 && j % kFold == 0;
+            if (fold) {
+                const float before = j == kFold ? 0.f : counts();
+#pragma unroll 1
+                for (int c0 = 0; c0 < D; c0 += 32) {
+                    uint32_t o[32];
+                    tmem_ld32_nowait(tm_o + c0, o);
+                    tmem_wait32(o);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        float4* at = sum_row + (c0 / 4 + k) * 256;
+                        float4 v = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
+                        if (j > kFold) {
+                            const float4 w = __ldcg(at);
+                            v = make_float4(fmaf(w.x, before, v.x), fmaf(w.y, before, v.y), fmaf(w.z, before, v.z), fmaf(w.w, before, v.w));
+                        }
+                        __stcg(at, v);
+                    }
+                }
+                __stcg(sum_max, m);
+                __stcg(sum_max + 256, LR);
+            }
             // ---- move to it, if it is far enough above the one in use ----
             const bool grow = vm > LR + 2.f;
             if (__any_sync(0xffffffffu, grow || mx > m + kLag)) {
@@ -500,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                 const float oc = corr * fast_exp2(LR - LR_new);
                 m = m_new;
                 LR = LR_new;
-                if (j > 0) {
+                if (j > 0 && !fold) {
 #pragma unroll 1
                     for (int c0 = 0; c0 < D; c0 += 32) {
                         uint32_t o[32];
@@ -581,6 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             tc_fence_after();
         }
         const float up = fast_exp2(LR - kCarry), f = parts > 1 ? up : (l == 0.f ? 0.f : up / l);
+        const float f_sums = Fold && folding >= 0 ? counts() * f : 0.f;
         float* part_row = parts > 1 ? p.partial + (static_cast<int64_t>(static_cast<int>(blockIdx.x) - p.split_from) * 256 + i * 128 + m_row) * (D + 4) : nullptr;
         if (parts > 1) { part_row[0] = m; part_row[1] = l; }
         // Finished rows leave through shared memory, a bulk copy a row: over the ring of K / V tiles, which every product has read.
@@ -597,6 +654,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             float x[32];
 #pragma unroll
             for (int k = 0; k < 32; ++k) x[k] = tiles > 0 && (parts > 1 || l != 0.f) ? __uint_as_float(o[k]) * f : 0.f;
+            if (Fold && folding >= 0 && (parts > 1 || l != 0.f)) {
+#pragma unroll
+                for (int k = 0; k < 32; k += 4) {
+                    const float4 w = __ldcg(sum_row + (c0 + k) / 4 * 256);
+                    x[k] = fmaf(w.x, f_sums, x[k]);
+                    x[k + 1] = fmaf(w.y, f_sums, x[k + 1]);
+                    x[k + 2] = fmaf(w.z, f_sums, x[k + 2]);
+                    x[k + 3] = fmaf(w.w, f_sums, x[k + 3]);
+                }
+            }
             if (parts > 1) {
 #pragma unroll
                 for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(part_row + 4 + c0 + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
@@ -616,6 +683,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     }
     tc_fence_before();
     __syncthreads();
+    if (Fold && tid == 0 && folding >= 0) {
+        __threadfence();
+        atomicAnd(&fold_claims[folding >> 5], ~(1u << (folding & 31)));
+    }
     if (warp == kIssueWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
@@ -675,15 +746,29 @@ Plan make_plan(const er_kv8_cache* c, const er_kv8_attention_params* u, int sms)
     return pl;
 }
 
-template <typename T, int D, bool E4M3>
-int32_t launch(const Kv8Prefill& p, const Plan& pl, cudaStream_t s) {
+// Bytes of the split pairs' partial rows, and of the sums behind them: none where no CTA can have more than kFold tiles.
+int64_t partial_bytes(const er_kv8_cache* c, const Plan& pl) {
+    return pl.parts > 1 ? static_cast<int64_t>(pl.grid - pl.split_from) * 256 * (c->head_dim + 4) * 4 : 0;
+}
+int64_t fold_bytes(const er_kv8_cache* c, const er_kv8_attention_params* u, int sms) {
+    uint64_t keys = kv8_table_rows(c);
+    if (u->sliding_window > 0) keys = std::min<uint64_t>(keys, static_cast<uint64_t>(u->sliding_window) + 256 + 2 * kTok);   // a pair's queries, both ends of the tiles
+    return keys > static_cast<uint64_t>(kFold) * kTok && sms <= kMostFoldSlots ? static_cast<int64_t>(sms) * 256 * (c->head_dim + 2) * 4 : 0;
+}
+
+template <typename T, int D, bool E4M3, bool Fold>
+int32_t launch_kernel(const Kv8Prefill& p, const Plan& pl, cudaStream_t s) {
     constexpr int kSmem = prefill_smem<D>();
     static_assert(kSmem <= 232448, "prefill kernel exceeds the shared memory of an sm_100 CTA");
     static std::atomic<uint64_t> devices{0};
-    const cudaError_t e = kv8_allow_smem(kv8_prefill_kernel<T, D, E4M3>, kSmem, devices);
+    const cudaError_t e = kv8_allow_smem(kv8_prefill_kernel<T, D, E4M3, Fold>, kSmem, devices);
     if (e != cudaSuccess) return kv8_launched(e, "kv8_prefill_kernel");
-    kv8_prefill_kernel<T, D, E4M3><<<pl.grid, kThreads, kSmem, s>>>(p);
-    const int32_t rc = kv8_launched(cudaGetLastError(), "kv8_prefill_kernel");
+    kv8_prefill_kernel<T, D, E4M3, Fold><<<pl.grid, kThreads, kSmem, s>>>(p);
+    return kv8_launched(cudaGetLastError(), "kv8_prefill_kernel");
+}
+template <typename T, int D, bool E4M3>
+int32_t launch(const Kv8Prefill& p, const Plan& pl, cudaStream_t s) {
+    const int32_t rc = p.fold != nullptr ? launch_kernel<T, D, E4M3, true>(p, pl, s) : launch_kernel<T, D, E4M3, false>(p, pl, s);
     if (rc != ER_OK || pl.parts == 1) return rc;
     kv8_prefill_join_kernel<T, D><<<(pl.grid - pl.split_from) / pl.parts * 32, 256, 0, s>>>(p);
     return kv8_launched(cudaGetLastError(), "kv8_prefill_join_kernel");
@@ -722,7 +807,7 @@ extern "C" int64_t er_kv8_prefill_workspace_bytes(const er_kv8_cache* cache, con
     int64_t bytes = sp.few ? kv8_decode_workspace(cache, u, true) : 0;      // the two kernels run one after the other
     if (sp.many) {
         const Plan pl = make_plan(cache, u, sms);
-        if (pl.parts > 1) bytes = std::max(bytes, static_cast<int64_t>(pl.grid - pl.split_from) * 256 * (cache->head_dim + 4) * 4);
+        bytes = std::max(bytes, partial_bytes(cache, pl) + fold_bytes(cache, u, sms));
     }
     return bytes;
 }
@@ -757,7 +842,12 @@ extern "C" int32_t er_kv8_attention_prefill(const er_kv8_cache* cache, const er_
         p.min_rows = sp.few ? kFewRows + 1 : 0;      // a hint that is wrong costs time, not rows
         p.group_magic = p.group == 1 ? 0 : ~0ull / static_cast<uint64_t>(p.group) + 1;
         p.scale_log2 = kv8_scale_log2(u->softmax_scale, cache->head_dim);
-        const Plan pl = make_plan(cache, u, kv8_sm_count());
+        const int sms = kv8_sm_count();
+        const Plan pl = make_plan(cache, u, sms);
+        if (fold_bytes(cache, u, sms) > 0) {
+            p.fold = p.partial + partial_bytes(cache, pl) / 4;
+            p.fold_slots = sms;
+        }
         p.slots = pl.slots; p.split_from = pl.split_from; p.parts = pl.parts;
         rc = u->type == ER_TYPE_FLOAT16 ? launch_shape<__half>(p, pl, cache->head_dim, e4m3, s) : launch_shape<__nv_bfloat16>(p, pl, cache->head_dim, e4m3, s);
         if (rc != ER_OK) return rc;

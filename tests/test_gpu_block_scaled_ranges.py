@@ -172,3 +172,67 @@ def test_value_scales_over_forty_powers_of_two(er, torch, t, op, fmt):  # noqa: 
         want, big = ref_attention(torch, q, k, v, length, 64 ** -0.5, window)
         assert float(want.abs().max()) < 60000
         check_attention(torch, got, want, big, t)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_sums_over_a_long_context_are_not_biased(er, torch, t, dim):  # noqa: F811
+    """Half a million keys and values around 1: what truncation takes from a running sum would add up.  128 sequences of 10 queries of 4 heads
+    over the same pages are 148 tile pairs, which are not cut along the keys."""
+    length, seqs, n = 500000, 128, 10
+    cache, table, _ = fill(er, torch, "e4m3", [16], 128, 1, dim, 16)
+    g = gen(torch, 6)
+    pages = -(-length // 128)
+    codes = [torch.randn(pages, 1, 128, dim, generator=g, device="cuda").to(torch.float8_e4m3fn).view(torch.uint8),
+             (torch.rand(pages, 1, 128, dim, generator=g, device="cuda") + 0.5).to(torch.float8_e4m3fn).view(torch.uint8)]
+    cache = er.BlockScaledKVCache.from_tensors(*codes, *(torch.full((pages, 1, 8), s, device="cuda") for s in (0.125, 1.0)))
+    table = torch.randperm(pages, generator=g, device="cuda").to(torch.int32)[None]
+    k, v = rows_of(cache, table[0], length)
+    q = torch.randn(seqs * n, 4, dim, generator=g, device="cuda").to(dtype(torch, t))
+    starts = ints(torch, [n * s for s in range(seqs + 1)])
+    got = cache.attention_prefill(q, starts, table.expand(seqs, -1).contiguous(), ints(torch, [length] * seqs), max_query_len=n)
+    for s in (0, 77):
+        want, big = ref_attention(torch, q[n * s:n * (s + 1)], k, v, length, dim ** -0.5)
+        check_attention(torch, got[n * s:n * (s + 1)], want, big, t)
+        # roundings of weights and outputs have no sign: their mean over 40 * dim outputs, each off by at most 2^-8 (bfloat16: half a step) relative, is within
+        # 5 * 2^-8 / sqrt(3 * 40 * dim) in all but one of a million cases for independent ones; a chain of 16384 keys between sums kept in float32
+        # is truncated by at most 1024 * 2^-23
+        mean = float(((got[n * s:n * (s + 1)].double() - want) / want).mean())
+        u = half_step(torch, dtype(torch, t)) + 2.0 ** -11
+        assert abs(mean) <= 5 * u / math.sqrt(3 * 40 * dim) + 1024 * 2.0 ** -23, mean
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("t, dim, seqs, lengths", [("f16", 128, 23, (40000, 16384, 16385, 5000)), ("bf16", 64, 23, (33000, 16513, 100)), ("bf16", 128, 1, (150000,)),
+                                                   ("f16", 64, 1, (280000,))])
+def test_sums_joined_over_a_long_context(er, torch, fmt, t, dim, seqs, lengths):  # noqa: F811
+    """Contexts of several stretches of 16384 keys, on either side of one, and cut along the keys as well (one sequence); maxima that rise and scales
+    that differ from stretch to stretch; windows longer and shorter than one.  Calls on two streams at a time give the bits of calls one by one."""
+    kv_heads, n = (4, 40) if seqs > 1 else (1, 70)
+    heads, longest = 4 * kv_heads, max(lengths)
+    cache, table, _ = fill(er, torch, fmt, [longest], 128, kv_heads, dim, 16, seed=dim)
+    far_apart(torch, cache, 5)
+    order = torch.arange(table.shape[1], device="cuda").float()      # later stretches of 64 pages: larger keys, smaller values
+    at = table[0].clamp(min=0).long()
+    cache.key_scales[at] *= torch.exp2(-3 + 3 * torch.floor(order / 64) / max(1, table.shape[1] // 64))[:, None, None]
+    cache.value_scales[at] *= torch.exp2(-torch.floor(order / 64).clamp(max=10))[:, None, None]
+    k, v = rows_of(cache, table[0], longest)
+    lens = [lengths[s % len(lengths)] for s in range(seqs)]
+    q = torch.randn(n * seqs, heads, dim, generator=gen(torch, 7), device="cuda").to(dtype(torch, t))
+    args = (q, ints(torch, [n * s for s in range(seqs + 1)]), table.expand(seqs, -1).contiguous(), ints(torch, lens))
+    got = {w: cache.attention_prefill(*args, max_query_len=n, sliding_window=w) for w in (0, 3000, 20001)}
+    for w, out in got.items():
+        for s in range(min(seqs, len(lengths))):
+            mine, length = slice(n * s, n * (s + 1)), lens[s]
+            want, big = ref_attention(torch, q[mine], k[:length], v[:length], length, dim ** -0.5, w)
+            check_long(torch, out[mine], want, big, t, 16384)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs[i].append(cache.attention_prefill(*args, max_query_len=n, sliding_window=(0, 20001)[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, got[0]) for x in outs[0]) and all(torch.equal(x, got[20001]) for x in outs[1])
+    assert cache.device_status() == 0
