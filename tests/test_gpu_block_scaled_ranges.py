@@ -174,6 +174,15 @@ def test_value_scales_over_forty_powers_of_two(er, torch, t, op, fmt):  # noqa: 
         check_attention(torch, got, want, big, t)
 
 
+def mean_of_roundings(torch, t, n):
+    """What the roundings of weights and of `n` outputs may add to the mean relative error, in all but one of a million cases.  The outputs here are means of
+    65536 or more values between 0.5 and 1.5 under nearly equal weights: 1 with a deviation of sqrt(1 / 12) / 256 = 0.0011.  float16's steps there are
+    2^-10 and 2^-11, no wider than that, so its roundings have either sign: 5 deviations of a mean of n uniform errors.  A step of bfloat16 is 2^-7 or
+    2^-8, wider than the outputs' spread: all of them may round the same way, and the mean of their errors is bounded by half a step alone."""
+    u = half_step(torch, dtype(torch, t))
+    return 5 * (u + 2.0 ** -11) / math.sqrt(3 * n) if t == "f16" else u + 5 * 2.0 ** -11 / math.sqrt(3 * n)
+
+
 @pytest.mark.parametrize("t", ["f16", "bf16"])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_sums_over_a_long_context_are_not_biased(er, torch, t, dim):  # noqa: F811
@@ -194,12 +203,9 @@ def test_sums_over_a_long_context_are_not_biased(er, torch, t, dim):  # noqa: F8
     for s in (0, 77):
         want, big = ref_attention(torch, q[n * s:n * (s + 1)], k, v, length, dim ** -0.5)
         check_attention(torch, got[n * s:n * (s + 1)], want, big, t)
-        # roundings of weights and outputs have no sign: their mean over 40 * dim outputs, each off by at most 2^-8 (bfloat16: half a step) relative, is within
-        # 5 * 2^-8 / sqrt(3 * 40 * dim) in all but one of a million cases for independent ones; a chain of 16384 keys between sums kept in float32
-        # is truncated by at most 1024 * 2^-23
+        # a chain of 16384 keys between sums kept in float32 is truncated by at most 1024 * 2^-23
         mean = float(((got[n * s:n * (s + 1)].double() - want) / want).mean())
-        u = half_step(torch, dtype(torch, t)) + 2.0 ** -11
-        assert abs(mean) <= 5 * u / math.sqrt(3 * 40 * dim) + 1024 * 2.0 ** -23, mean
+        assert abs(mean) <= mean_of_roundings(torch, t, 40 * dim) + 1024 * 2.0 ** -23, mean
 
 
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
@@ -235,4 +241,26 @@ def test_sums_joined_over_a_long_context(er, torch, fmt, t, dim, seqs, lengths):
                 outs[i].append(cache.attention_prefill(*args, max_query_len=n, sliding_window=(0, 20001)[i]))
     torch.cuda.synchronize()
     assert all(torch.equal(x, got[0]) for x in outs[0]) and all(torch.equal(x, got[20001]) for x in outs[1])
+    assert cache.device_status() == 0
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("dim, heads", [(64, 8), (128, 8), (128, 16)])
+def test_decode_sums_over_millions_of_rows_are_not_biased(er, torch, t, dim, heads):  # noqa: F811
+    """Four million rows a sequence, the same 65536 over and over: their mean is that of the 65536.  148 sequences, so that a CTA walks whole ones."""
+    base, times, seqs = 65536, 64, 148
+    g = gen(torch, 6)
+    pages = base // 128
+    codes = [torch.randn(pages, 1, 128, dim, generator=g, device="cuda").to(torch.float8_e4m3fn).view(torch.uint8),
+             (torch.rand(pages, 1, 128, dim, generator=g, device="cuda") + 0.5).to(torch.float8_e4m3fn).view(torch.uint8)]
+    cache = er.BlockScaledKVCache.from_tensors(*codes, *(torch.full((pages, 1, 8), s, device="cuda") for s in (0.125, 1.0)))
+    order = torch.randperm(pages, generator=g, device="cuda").to(torch.int32)
+    q = torch.randn(seqs, heads, dim, generator=g, device="cuda").to(dtype(torch, t))
+    got = cache.attention_decode(q, order.repeat(times)[None].expand(seqs, -1).contiguous(), ints(torch, [base * times] * seqs))
+    k, v = rows_of(cache, order, base)
+    want, big = (torch.cat(x) for x in zip(*(ref_attention(torch, q[s:s + 1], k, v, base, dim ** -0.5) for s in range(8))))
+    check_attention(torch, got[:8], want, big, t)
+    # eight units of 32 rows between sums kept in float32 are 16 products
+    mean = float(((got[:8].double() - want) / want).mean())
+    assert abs(mean) <= mean_of_roundings(torch, t, 8 * heads * dim) + 16 * 2.0 ** -23, mean
     assert cache.device_status() == 0
