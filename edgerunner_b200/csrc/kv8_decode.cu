@@ -33,9 +33,12 @@ namespace {
 constexpr int kMinUnits = 8;          // units of a CTA, so that short work stays together
 constexpr int kUnit = 2 * kKv8Unit;   // tokens that a warp takes at a time: two halves, each with a page and scales of its own
 // The tensor cores add into their accumulators with truncation: a product of 16 keys takes up to 2^-23 from the sum, half of that on average, and a warp adds every
-// 8th or 12th of a visit.  float32 rows move their sums out every 8 units.  16-bit rows do so where a query may see more rows than this: up to there the loss
-// stays below 1.3e-4 (measured 1.7e-4 at 500000 rows of one CTA), a quarter of half a float16 step; the registers that it takes leave room for eight warps.
+// 8th or 12th of a visit (one CTA over 500000 rows: 1.7e-4 low, 4 million rows: 1.4e-3).  float32 rows move their sums to registers every 8 units.  16-bit rows
+// have no registers for that: where a query may see more rows than kPlainRows they add them to a float32 sum in memory every kSumUnits units of a warp, that is
+// every 196608 rows of a CTA's visit (1.2e-4 at most, measured 7e-5).  A kernel of its own, since the count alone costs the loop (64 ragged sequences: 231 us
+// without, 236 with it, 262 with eight warps that keep the sums in registers).
 constexpr uint64_t kPlainRows = 1u << 18;
+constexpr int kSumUnits = 512;
 constexpr float kWeightScale = 4096.f;    // 2^12
 constexpr float kLift0 = 8.507059173023462e37f;    // 2^126: scales up to 2^-114 need no less
 
@@ -46,6 +49,7 @@ struct Kv8Decode {
     void* out;
     int64_t q_token, q_head, out_token, out_head;
     float* partial;
+    float4* sums;                   // of long visits: [CTA][warp][NT][D / 16 + 1][lane]: accumulators, then the maxima and lifts that they stand for
     const int32_t* starts;          // tokens of the sequences, or nullptr: query_len each
     int num_tokens, group, query_len, window, tile_rows;
     int few_rows;                   // > 0: sequences with more query rows are somebody else's
@@ -230,16 +234,16 @@ template <int D> struct Stage {
 template <int NT> __host__ __device__ constexpr int decode_rows() { return 8 * NT; }
 // Warps of a CTA.  A unit costs a warp about 570 instructions, most of them in chains: with two warps to a scheduler it waits for itself a
 // quarter of the time.  Three fit where 168 registers do: one column tile of 16-bit rows (64 ragged sequences: 237 -> 226 us).
-template <typename T, int NT, bool Keep> __host__ __device__ constexpr int decode_warps() { return sizeof(T) == 2 && NT == 1 && !Keep ? 12 : 8; }
+template <typename T, int NT> __host__ __device__ constexpr int decode_warps() { return sizeof(T) == 2 && NT == 1 ? 12 : 8; }
 // Warps that meet in shared memory at the end of an item; those beyond hand theirs to a partner first.
-template <typename T, int NT, bool Keep> __host__ __device__ constexpr int join_warps() { return decode_warps<T, NT, Keep>() / 2; }
-template <typename T, int D, int NT, bool Keep> __host__ __device__ constexpr int decode_stages() {
-    constexpr int n = decode_warps<T, NT, Keep>() == 12 ? 2 : NT == 1 ? 3 : 2;
+template <typename T, int NT> __host__ __device__ constexpr int join_warps() { return decode_warps<T, NT>() / 2; }
+template <typename T, int D, int NT> __host__ __device__ constexpr int decode_stages() {
+    constexpr int n = decode_warps<T, NT>() == 12 ? 2 : NT == 1 ? 3 : 2;
     return D == 128 ? n : 2 * n;
 }
-template <typename T, int D, int NT, bool Keep> __host__ __device__ constexpr int join_floats() { return join_warps<T, NT, Keep>() * 8 * NT * (D + 4); }
-template <typename T, int D, int NT, bool Keep> __host__ __device__ constexpr int decode_smem() {
-    return decode_warps<T, NT, Keep>() * decode_stages<T, D, NT, Keep>() * (Stage<D>::kBytes + 16 + 8) + (join_floats<T, D, NT, Keep>() + join_warps<T, NT, Keep>() * 8 * NT * 2) * 4 + static_cast<int>(sizeof(ListScratch)) + 16 + 1024;
+template <typename T, int D, int NT> __host__ __device__ constexpr int join_floats() { return join_warps<T, NT>() * 8 * NT * (D + 4); }
+template <typename T, int D, int NT> __host__ __device__ constexpr int decode_smem() {
+    return decode_warps<T, NT>() * decode_stages<T, D, NT>() * (Stage<D>::kBytes + 16 + 8) + (join_floats<T, D, NT>() + join_warps<T, NT>() * 8 * NT * 2) * 4 + static_cast<int>(sizeof(ListScratch)) + 16 + 1024;
 }
 // One partial: max, sum, -, - and the unnormalised row.
 template <int D> __host__ __device__ constexpr int partial_stride() { return D + 4; }
@@ -261,11 +265,11 @@ __device__ __forceinline__ void bounded_wait(uint64_t* bar, uint32_t parity, vol
     }
 }
 
-template <typename T, int D, bool E4M3, int NT, bool Keep>
-__global__ void __launch_bounds__(decode_warps<T, NT, Keep>() * 32, 1) kv8_decode_kernel(const __grid_constant__ Kv8Decode p) {
+template <typename T, int D, bool E4M3, int NT, bool Long>
+__global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kernel(const __grid_constant__ Kv8Decode p) {
     constexpr bool kSplit = sizeof(T) == 4;      // float32: queries and weights as a high and a low half
-    static_assert(!Keep || NT == 1, "");
-    constexpr int kRows = decode_rows<NT>(), kStages = decode_stages<T, D, NT, Keep>(), kWarps = decode_warps<T, NT, Keep>(), kThreads = kWarps * 32, kJoin = join_warps<T, NT, Keep>();
+    static_assert(!kSplit || (NT == 1 && !Long), "");
+    constexpr int kRows = decode_rows<NT>(), kStages = decode_stages<T, D, NT>(), kWarps = decode_warps<T, NT>(), kThreads = kWarps * 32, kJoin = join_warps<T, NT>();
     constexpr int KK = D / 16, MT = D / 16, kWords = D / 16;   // k-steps of the scores; m-tiles of the outputs; 4-byte words of a lane's part of a key row
     constexpr int kOwn = D / 8;                                 // dims of a lane g in the outputs
     constexpr int kJoinRow = D + 4;
@@ -273,7 +277,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT, Keep>() * 32, 1) kv8_decod
     uint8_t* stages = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);     // the swizzle goes by the address
     float* stage_scales = reinterpret_cast<float*>(stages + kWarps * kStages * Stage<D>::kBytes);
     float* join = stage_scales + kWarps * kStages * 4;
-    float* join_ml = join + join_floats<T, D, NT, Keep>();
+    float* join_ml = join + join_floats<T, D, NT>();
     uint64_t* bars = reinterpret_cast<uint64_t*>(join_ml + kJoin * kRows * 2);
     ListScratch* scratch = reinterpret_cast<ListScratch*>(bars + kWarps * kStages);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(scratch + 1);
@@ -417,7 +421,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT, Keep>() * 32, 1) kv8_decod
             }
         }
         float o[NT][MT][4], m[NT][2], l[NT][2], lift[NT][2];    // lift: 4096 / R, powers of two
-        float keep[Keep ? MT : 1][4];       // the tensor cores' sums are moved here every 8 units (their accumulators round towards zero)
+        float keep[kSplit ? MT : 1][4];     // float32: the tensor cores' sums are moved here every 8 units (their accumulators round towards zero)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -427,8 +431,29 @@ __global__ void __launch_bounds__(decode_warps<T, NT, Keep>() * 32, 1) kv8_decod
             lift[nt][0] = lift[nt][1] = kLift0;
         }
 #pragma unroll
-        for (int i = 0; i < (Keep ? MT : 1); ++i) keep[i][0] = keep[i][1] = keep[i][2] = keep[i][3] = 0.f;
+        for (int i = 0; i < (kSplit ? MT : 1); ++i) keep[i][0] = keep[i][1] = keep[i][2] = keep[i][3] = 0.f;
         int since = 0;
+        // Long visits: this lane's sums in memory, once they have been begun, are added to the accumulators, which then go there and start again.
+        bool begun = false;
+        float4* const sums = Long ? p.sums + static_cast<int64_t>(cta * kWarps + warp) * (NT * (MT + 1) * 32) + lane : nullptr;
+        auto add_sums = [&]() {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const float4 was = __ldcg(sums + (nt * (MT + 1) + MT) * 32);
+                const float was_m[2] = {was.x, was.y}, was_lift[2] = {was.z, was.w};
+                float f[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) f[j] = was_m[j] == -INFINITY ? 0.f : fast_exp2(was_m[j] - m[nt][j]) * (lift[nt][j] * inverse_lift(was_lift[j]));
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    const float4 v = __ldcg(sums + (nt * (MT + 1) + i) * 32);
+                    o[nt][i][0] = fmaf(v.x, f[0], o[nt][i][0]);
+                    o[nt][i][1] = fmaf(v.y, f[1], o[nt][i][1]);
+                    o[nt][i][2] = fmaf(v.z, f[0], o[nt][i][2]);
+                    o[nt][i][3] = fmaf(v.w, f[1], o[nt][i][3]);
+                }
+            }
+        };
 
         for (int u = u0 + warp; u < u1; u += kWarps) {
             cp_async_wait<kStages - 2>();
@@ -523,7 +548,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT, Keep>() * 32, 1) kv8_decod
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             o[nt][i][e] *= corr[e & 1];
-                            if constexpr (Keep) keep[i][e] *= corr[e & 1];
+                            if constexpr (kSplit) keep[i][e] *= corr[e & 1];
                         }
                     }
                 }
@@ -593,7 +618,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT, Keep>() * 32, 1) kv8_decod
                     }
                 }
             }
-            if constexpr (Keep) {
+            if constexpr (kSplit) {
                 if (++since == 8) {
                     since = 0;
 #pragma unroll
@@ -603,10 +628,27 @@ __global__ void __launch_bounds__(decode_warps<T, NT, Keep>() * 32, 1) kv8_decod
                     }
                 }
             }
+            if constexpr (Long) {
+                if (++since == kSumUnits) {
+                    since = 0;
+                    if (begun) add_sums();
+                    begun = true;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) {
+                            __stcg(sums + (nt * (MT + 1) + i) * 32, make_float4(o[nt][i][0], o[nt][i][1], o[nt][i][2], o[nt][i][3]));
+                            o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+                        }
+                        __stcg(sums + (nt * (MT + 1) + MT) * 32, make_float4(m[nt][0], m[nt][1], lift[nt][0], lift[nt][1]));
+                    }
+                }
+            }
             cstage = cstage + 1 == kStages ? 0 : cstage + 1;
             cphase ^= cstage == 0 ? 1 : 0;
         }
 
+        if (Long && begun) add_sums();
         const Place done = at;
         left -= seg;
         if (left > 0) {
@@ -627,7 +669,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT, Keep>() * 32, 1) kv8_decod
             for (int i = 0; i < MT; ++i) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    if constexpr (Keep) o[nt][i][e] += keep[i][e];
+                    if constexpr (kSplit) o[nt][i][e] += keep[i][e];
                     o[nt][i][e] *= back[e & 1];
                 }
             }
@@ -781,13 +823,13 @@ int kv8_sm_count() {
     return sms;
 }
 namespace {
-// Two columns of eight query rows where they are needed and fit: float32 rows take two operands each and stay at eight.
-int tiles_of(bool keep, int rows) { return !keep && rows > 8 ? 2 : 1; }
-bool keeps_sums(const er_kv8_cache* c, const er_kv8_attention_params* u) {
-    if (u->type == ER_TYPE_FLOAT32) return true;
+bool long_visits(const er_kv8_cache* c, const er_kv8_attention_params* u) {
+    if (u->type == ER_TYPE_FLOAT32) return false;
     const uint64_t rows = kv8_table_rows(c);
     return (u->sliding_window > 0 ? std::min<uint64_t>(rows, static_cast<uint64_t>(u->sliding_window) + 64) : rows) > kPlainRows;
 }
+// Two columns of eight query rows where they are needed and fit: float32 rows take two operands each and stay at eight.
+int tiles_of(uint32_t type, int rows) { return type != ER_TYPE_FLOAT32 && rows > 8 ? 2 : 1; }
 
 // Codes as a 2-D tensor of bytes, swizzled as the kernel reads them: rows of 128 (64) bytes, 16-byte chunk c of row r at c ^ (r % 8) (c ^ (r / 2 % 4)).
 bool encode_rows(CUtensorMap* map, const uint8_t* codes, const Kv8Cache& c, int head_dim) {
@@ -800,15 +842,15 @@ bool encode_rows(CUtensorMap* map, const uint8_t* codes, const Kv8Cache& c, int 
               head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int D, bool E4M3, int NT, bool Keep>
+template <typename T, int D, bool E4M3, int NT, bool Long>
 int32_t launch(Kv8Decode& p, int most_rows, int sms, cudaStream_t s) {
-    constexpr int kSmem = decode_smem<T, D, NT, Keep>();
+    constexpr int kSmem = decode_smem<T, D, NT>();
     static_assert(kSmem <= 232448, "decode kernel exceeds the shared memory of an sm_100 CTA");
     p.tile_rows = 8 * NT;
     static std::atomic<uint64_t> devices{0};
-    cudaError_t e = kv8_allow_smem(kv8_decode_kernel<T, D, E4M3, NT, Keep>, kSmem, devices);
+    cudaError_t e = kv8_allow_smem(kv8_decode_kernel<T, D, E4M3, NT, Long>, kSmem, devices);
     if (e != cudaSuccess) return kv8_launched(e, "kv8_decode_kernel");
-    kv8_decode_kernel<T, D, E4M3, NT, Keep><<<sms, decode_warps<T, NT, Keep>() * 32, kSmem, s>>>(p);
+    kv8_decode_kernel<T, D, E4M3, NT, Long><<<sms, decode_warps<T, NT>() * 32, kSmem, s>>>(p);
     const int32_t rc = kv8_launched(cudaGetLastError(), "kv8_decode_kernel");
     if (rc != ER_OK) return rc;
     cudaLaunchConfig_t cfg{};
@@ -824,16 +866,18 @@ int32_t launch(Kv8Decode& p, int most_rows, int sms, cudaStream_t s) {
     return kv8_launched(e, "kv8_decode_join_kernel");
 }
 template <typename T, int D, bool E4M3>
-int32_t launch_rows(Kv8Decode& p, int most_rows, bool keep, int sms, cudaStream_t s) {
+int32_t launch_rows(Kv8Decode& p, int most_rows, int sms, cudaStream_t s) {
     if constexpr (sizeof(T) == 2) {
-        if (!keep) return tiles_of(keep, most_rows) == 2 ? launch<T, D, E4M3, 2, false>(p, most_rows, sms, s) : launch<T, D, E4M3, 1, false>(p, most_rows, sms, s);
+        const bool two = tiles_of(ER_TYPE_FLOAT16, most_rows) == 2;
+        if (p.sums != nullptr) return two ? launch<T, D, E4M3, 2, true>(p, most_rows, sms, s) : launch<T, D, E4M3, 1, true>(p, most_rows, sms, s);
+        if (two) return launch<T, D, E4M3, 2, false>(p, most_rows, sms, s);
     }
-    return launch<T, D, E4M3, 1, true>(p, most_rows, sms, s);
+    return launch<T, D, E4M3, 1, false>(p, most_rows, sms, s);
 }
 template <typename T>
-int32_t launch_shape(Kv8Decode& p, int most_rows, int head_dim, bool e4m3, bool keep, int sms, cudaStream_t s) {
-    if (head_dim == 128) return e4m3 ? launch_rows<T, 128, true>(p, most_rows, keep, sms, s) : launch_rows<T, 128, false>(p, most_rows, keep, sms, s);
-    return e4m3 ? launch_rows<T, 64, true>(p, most_rows, keep, sms, s) : launch_rows<T, 64, false>(p, most_rows, keep, sms, s);
+int32_t launch_shape(Kv8Decode& p, int most_rows, int head_dim, bool e4m3, int sms, cudaStream_t s) {
+    if (head_dim == 128) return e4m3 ? launch_rows<T, 128, true>(p, most_rows, sms, s) : launch_rows<T, 128, false>(p, most_rows, sms, s);
+    return e4m3 ? launch_rows<T, 64, true>(p, most_rows, sms, s) : launch_rows<T, 64, false>(p, most_rows, sms, s);
 }
 
 }  // namespace
@@ -864,10 +908,14 @@ static int most_rows_of(const er_kv8_cache* c, const er_kv8_attention_params* u,
     return static_cast<int>(std::min<uint64_t>(n * (u->num_heads / c->num_kv_heads), 1u << 30));
 }
 
+// Bytes of the partial rows of a grid of `sms` CTAs, and behind them of the sums of long visits (12 warps at most).
+static int64_t partial_bytes(const er_kv8_cache* c, const er_kv8_attention_params* u, int sms, int most_rows) {
+    return static_cast<int64_t>(sms) * 2 * 8 * tiles_of(u->type, most_rows) * (c->head_dim + 4) * 4;
+}
 int64_t kv8_decode_workspace(const er_kv8_cache* c, const er_kv8_attention_params* u, bool ragged) {
-    const int sms = kv8_sm_count();
+    const int sms = kv8_sm_count(), most_rows = most_rows_of(c, u, ragged), tiles = tiles_of(u->type, most_rows);
     if (sms == 0) return report_error(ER_ERR_CUDA, "no CUDA device (no CPU fallback)");
-    return static_cast<int64_t>(sms) * 2 * 8 * tiles_of(keeps_sums(c, u), most_rows_of(c, u, ragged)) * (c->head_dim + 4) * 4;
+    return partial_bytes(c, u, sms, most_rows) + (long_visits(c, u) ? static_cast<int64_t>(sms) * (tiles == 1 ? 12 : 8) * tiles * (c->head_dim / 16 + 1) * 32 * 16 : 0);
 }
 
 int32_t kv8_check_workspace(const er_kv8_attention_params* u, int64_t need) {
@@ -881,7 +929,7 @@ int32_t kv8_check_workspace(const er_kv8_attention_params* u, int64_t need) {
 // The kernel over a checked call.  ragged: queries by query_starts, of the sequences with up to `few_rows` query rows (0: all).
 int32_t kv8_launch_decode(const Kv8Cache& cache, const er_kv8_cache* c, const er_kv8_attention_params* u, bool ragged, int few_rows, cudaStream_t s) {
     const int most_rows = few_rows > 0 ? std::min(few_rows, most_rows_of(c, u, ragged)) : most_rows_of(c, u, ragged);
-    const bool e4m3 = c->format == ER_KV8_E4M3, keep = keeps_sums(c, u);
+    const bool e4m3 = c->format == ER_KV8_E4M3;
     Kv8Decode p{};
     p.cache = cache;
     p.q = u->q; p.out = u->out;
@@ -896,10 +944,11 @@ int32_t kv8_launch_decode(const Kv8Cache& cache, const er_kv8_cache* c, const er
         return report_error(ER_ERR_CUDA, "cuTensorMapEncodeTiled refused the cache's shape");
     p.scale_log2 = kv8_scale_log2(u->softmax_scale, c->head_dim);
     const int sms = kv8_sm_count(), d = static_cast<int>(c->head_dim);
+    if (long_visits(c, u)) p.sums = reinterpret_cast<float4*>(static_cast<uint8_t*>(u->workspace) + partial_bytes(c, u, sms, most_rows_of(c, u, ragged)));
     switch (u->type) {
-        case ER_TYPE_FLOAT32: return launch_shape<float>(p, most_rows, d, e4m3, keep, sms, s);
-        case ER_TYPE_FLOAT16: return launch_shape<__half>(p, most_rows, d, e4m3, keep, sms, s);
-        default: return launch_shape<__nv_bfloat16>(p, most_rows, d, e4m3, keep, sms, s);
+        case ER_TYPE_FLOAT32: return launch_shape<float>(p, most_rows, d, e4m3, sms, s);
+        case ER_TYPE_FLOAT16: return launch_shape<__half>(p, most_rows, d, e4m3, sms, s);
+        default: return launch_shape<__nv_bfloat16>(p, most_rows, d, e4m3, sms, s);
     }
 }
 
