@@ -40,7 +40,7 @@ constexpr int kUnit = 2 * kKv8Unit;   // tokens that a warp takes at a time: two
 constexpr uint64_t kPlainRows = 1u << 18;
 constexpr int kSumUnits = 512;
 constexpr float kWeightScale = 4096.f;    // 2^12
-constexpr float kLift0 = 8.507059173023462e37f;    // 2^126: scales up to 2^-114 need no less
+constexpr float kLift0 = 8.507059173023462e37f;    // 2^126, while no scale above 2^-114 has been seen
 
 struct Kv8Decode {
     CUtensorMap maps[2];            // codes of the keys, values as [rows][head_dim], boxes of 16 rows

@@ -17,7 +17,8 @@
 //                    until O_i += W_i V has been executed (head size 128; with 64 there is room for W beside S).
 // Tensor memory: S_0, S_1 at columns 0, 128; O_0, O_1 from 256 on, D columns each; W_i over S_i, or (head size 64) W_0, W_1 at 384, 448.  Shared
 // memory: Q (2 x 128 rows), a ring of K / V tiles of 128 tokens, scales.
-// Every wait is bounded (2 s): then the status word is set, the rest of the waits are skipped, tensor memory is freed, the kernel returns.
+// Every wait is bounded (2 s): then the status word is set, the rest of the waits are skipped, the products that have been issued are waited for (3 s), tensor
+// memory is freed, the kernel returns.
 //
 // Measured (B200, 32 query / 8 kv heads of 128): a chunk of 2048 tokens at 32768, int8, float16: 1.28 ms = 835 TFLOP/s = 0.50 of the library's bf16
 // product; the same without the softmax arithmetic 0.80 ms, without the conversion besides 0.63 ms.  A tile's softmax takes 3400 clocks of a period
@@ -381,6 +382,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             }
             if (leader) umma_commit(smem_u32(bars + kBarO));
             __syncwarp();
+            // After a wait that ran out nobody else waits for the products, which read this CTA's memory and write the tensor memory that is freed below.
+            const uint64_t start = global_timer_ns();
+            while (!mbar_try_wait(bars + kBarO, 0) && global_timer_ns() - start < 3000000000ull) {}
         }
     } else {
         // ================= softmax =================
