@@ -259,7 +259,10 @@ class BlockScaledKVCache:
         return tuple(out)
 
     def device_status(self):
-        """The sticky status word as an ER_ERR_* code, 0 when nothing was skipped (waits for the device); clear_device_status() resets it."""
+        """The sticky status word as an ER_ERR_* code, 0 when nothing was skipped (waits for the device, calls on every stream); clear_device_status()
+        resets it, in the order of the current stream."""
+        import torch
+        torch.cuda.synchronize(self.device)
         return int(self._status.item())
 
     def clear_device_status(self):

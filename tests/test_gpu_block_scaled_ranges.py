@@ -264,3 +264,18 @@ def test_decode_sums_over_millions_of_rows_are_not_biased(er, torch, t, dim, hea
     mean = float(((got[:8].double() - want) / want).mean())
     assert abs(mean) <= mean_of_roundings(torch, t, 8 * heads * dim) + 1024 * 2.0 ** -23, mean
     assert cache.device_status() == 0
+
+
+def test_the_status_waits_for_every_stream(er, torch):  # noqa: F811
+    """device_status() tells what a call on any stream has met, also one that is still running when it is asked."""
+    cache = er.BlockScaledKVCache(2, 16, 1, 64)
+    k = torch.ones(1, 1, 64, device="cuda")
+    table, lens, other = ints(torch, [[-1]]), ints(torch, [1]), torch.cuda.Stream()
+    cache.append(k, k, table, lens, partial_rotary_factor=0.0)
+    assert cache.device_status() == -10
+    cache.clear_device_status()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(other):
+        torch.cuda._sleep(200_000_000)          # 0.1 s
+        cache.append(k, k, table, lens, partial_rotary_factor=0.0)
+    assert cache.device_status() == -10
