@@ -40,7 +40,7 @@ int32_t kv8_check_device(const void* buffer) {
 }
 
 int32_t kv8_check(const er_kv8_cache* c, Kv8Cache* out) {
-    if (!c->keys || !c->values || !c->key_scales || !c->value_scales || !c->block_tables || !c->kv_lens)
+    if (!c->keys || !c->values || !c->key_scales || !c->value_scales || (!c->block_tables && c->block_table_width > 0) || !c->kv_lens)
         return report_error(ER_ERR_INVALID_ARGUMENT, "null buffer in er_kv8_cache");
     if (c->format != ER_KV8_E4M3 && c->format != ER_KV8_INT8) return report_error(ER_ERR_INVALID_ARGUMENT, "format must be ER_KV8_E4M3 or ER_KV8_INT8");
     if (c->head_dim != 64 && c->head_dim != 128) return report_error(ER_ERR_UNSUPPORTED, "head_dim of an 8-bit cache must be 64 or 128");

@@ -475,7 +475,7 @@ typedef struct {
     uint8_t* values;
     float* key_scales;           /* device [num_pages][num_kv_heads][page_size / scale_block] */
     float* value_scales;
-    const int32_t* block_tables; /* device [num_seqs][block_table_stride]: page ids, one per page_size tokens; negative = no page */
+    const int32_t* block_tables; /* device [num_seqs][block_table_stride]: page ids, one per page_size tokens; negative = no page; NULL with width 0 */
     const int32_t* kv_lens;      /* device [num_seqs]: rows of the sequence, the call's own tokens included */
     int32_t* status;             /* device word, set to ER_ERR_OUT_OF_PAGES / ER_ERR_SHAPE by a kernel that skipped something; NULL = none */
     uint32_t num_pages, page_size, scale_block;  /* page_size a multiple of scale_block; scale_block 16, 32, 64 or 128 */

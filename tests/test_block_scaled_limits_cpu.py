@@ -75,3 +75,13 @@ def test_attention_refuses_windows_whose_arithmetic_leaves_an_int(er):  # noqa: 
     if not torch.cuda.is_available():       # past the checks of arguments: no device
         for tokens, window in ((512, 0), (512, 0x7FFFFFFF), (255, 0x7FFFFEFF)):
             assert fn(C.byref(cache(**wide)), C.byref(attention(num_tokens=tokens, sliding_window=window)), None) == -8
+
+
+def test_tables_without_columns_need_no_buffer(er):  # noqa: F811
+    """No pages yet: an empty table has no address.  With columns it needs one."""
+    import torch
+    none = dict(block_tables=0, block_table_width=0, block_table_stride=0)
+    for fn, p in ((er.lib().er_kv8_attention_decode, attention()), (er.lib().er_kv8_attention_prefill, attention()), (er.lib().er_kv8_append, append())):
+        assert fn(C.byref(cache(block_tables=0)), C.byref(p), None) == INVALID
+        if not torch.cuda.is_available():       # past the checks of arguments: no device
+            assert fn(C.byref(cache(**none)), C.byref(p), None) == -8

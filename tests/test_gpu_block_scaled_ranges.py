@@ -279,3 +279,15 @@ def test_the_status_waits_for_every_stream(er, torch):  # noqa: F811
         torch.cuda._sleep(200_000_000)          # 0.1 s
         cache.append(k, k, table, lens, partial_rotary_factor=0.0)
     assert cache.device_status() == -10
+
+
+def test_tables_without_pages(er, torch):  # noqa: F811
+    """A batch of empty sequences whose table has no column yet: nothing to see, and nowhere to write."""
+    cache = er.BlockScaledKVCache(2, 16, 1, 64)
+    q = torch.randn(2, 2, 64, device="cuda")
+    table, lens = torch.empty(2, 0, dtype=torch.int32, device="cuda"), ints(torch, [0, 0])
+    assert bool((cache.attention_decode(q, table, lens) == 0).all())
+    assert bool((cache.attention_prefill(q, ints(torch, [0, 1, 2]), table, lens) == 0).all())
+    assert cache.device_status() == 0
+    cache.append(q[:, :1], q[:, :1], table, ints(torch, [1, 1]), partial_rotary_factor=0.0)
+    assert cache.device_status() == -10
