@@ -16,7 +16,7 @@ import struct
 from ._lib import check, lib, stream_ptr
 
 # The parameter structures of include/er_kv.h as packed bytes: one call instead of some thirty attribute writes, which cost more than a
-# small kernel runs for.  Field order as in the header (tests compare the sizes with the compiler's).
+# small kernel runs for.  Field order as in the header (a test compares sizes and every field's place with the compiler's).
 _NORM_ROPE = struct.Struct("@4P8q3P5I4f4x")
 _CACHE = struct.Struct("@7P9I4x")
 _APPEND = struct.Struct("@2P4q2P2I4f")

@@ -85,3 +85,31 @@ def test_tables_without_columns_need_no_buffer(er):  # noqa: F811
         assert fn(C.byref(cache(block_tables=0)), C.byref(p), None) == INVALID
         if not torch.cuda.is_available():       # past the checks of arguments: no device
             assert fn(C.byref(cache(**none)), C.byref(p), None) == -8
+
+
+def test_packed_structures_are_the_headers(er):  # noqa: F811
+    """The calls hand their structures over as packed bytes: size and every field's place against the C compiler's layout of the header."""
+    import os
+    import subprocess
+    import tempfile
+    from edgerunner_b200 import _lib
+    from edgerunner_b200 import block_scaled_cache as b
+    pairs = [("er_qk_norm_rope_params", b._NORM_ROPE), ("er_kv8_cache", b._CACHE), ("er_kv8_append_params", b._APPEND), ("er_kv8_attention_params", b._ATTENTION)]
+    prints = ["printf(\"%%zu \", sizeof(%s));" % n + "".join("printf(\"%%zu \", offsetof(%s, %s));" % (n, f[0]) for f in getattr(_lib, n)._fields_) for n, _ in pairs]
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    with tempfile.TemporaryDirectory() as d:
+        src = os.path.join(d, "s.c")
+        with open(src, "w") as f:
+            f.write("#include <stddef.h>\n#include <stdio.h>\n#include \"er_kv.h\"\nint main(void) { %s return 0; }\n" % " ".join(prints))
+        subprocess.run(["gcc", "-I", os.path.join(root, "include"), src, "-o", os.path.join(d, "s")], check=True)
+        got = [int(x) for x in subprocess.run([os.path.join(d, "s")], capture_output=True, text=True, check=True).stdout.split()]
+    for name, packed in pairs:
+        kind = getattr(_lib, name)
+        fields = [f[0] for f in kind._fields_]
+        size, offsets, got = got[0], got[1:1 + len(fields)], got[1 + len(fields):]
+        assert size == packed.size == C.sizeof(kind)
+        assert offsets == [getattr(kind, f).offset for f in fields]
+        values = list(range(1, len(fields) + 1))          # a value of its own for each field, in the header's order
+        back = kind.from_buffer_copy(packed.pack(*values))
+        assert [getattr(back, f) for f in fields] == values, name
+    assert got == []
