@@ -203,6 +203,8 @@ class BlockScaledKVCache:
             return _torch.empty(shape, dtype=dtype, device=self.device)
 
     def _attention(self, fn, size_fn, q, out, block_tables, kv_lens, query_starts, query_len, max_query_len, softmax_scale, sliding_window, stream):
+        if sliding_window < 0 or max_query_len < 0:
+            raise ValueError("sliding_window and max_query_len must not be negative (0: none, not known)")
         index = self._index
         kind = _type(q, "q")
         if out is None:

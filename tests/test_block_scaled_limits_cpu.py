@@ -113,3 +113,16 @@ def test_packed_structures_are_the_headers(er):  # noqa: F811
         back = kind.from_buffer_copy(packed.pack(*values))
         assert [getattr(back, f) for f in fields] == values, name
     assert got == []
+
+
+def test_python_layer_refuses_negative_counts(er):  # noqa: F811
+    """A window or a hint below zero is a ValueError that names it, like every other argument the layer refuses."""
+    import torch
+    cache_ = object.__new__(er.BlockScaledKVCache)
+    q, n = torch.zeros(1, 2, 128), torch.ones(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="sliding_window"):
+        cache_.attention_decode(q, n[None], n, sliding_window=-1)
+    with pytest.raises(ValueError, match="sliding_window"):
+        cache_.attention_prefill(q, n, n[None], n, sliding_window=-1)
+    with pytest.raises(ValueError, match="max_query_len"):
+        cache_.attention_prefill(q, n, n[None], n, max_query_len=-2)
