@@ -469,7 +469,8 @@ typedef struct {
 } er_qk_norm_rope_params;
 int32_t er_qk_norm_rope(const er_qk_norm_rope_params* params, void* stream);
 
-/* A batch's view of an 8-bit paged cache.  Element = code * scale; scale >= 0, one per (page, kv head, block of scale_block tokens). */
+/* A batch's view of an 8-bit paged cache.  Element = code * scale; scale >= 0, one per (page, kv head, block of scale_block tokens).
+ * er_kv8_append writes no E4M3 code of a NaN; where rows come from elsewhere, a query in front of such a code may be NaN as well. */
 typedef struct {
     uint8_t* keys;               /* device [num_pages][num_kv_heads][page_size][head_dim] codes */
     uint8_t* values;
@@ -488,7 +489,8 @@ typedef struct {
  * Keys are normed and rotated at that position on the way (as in er_qk_norm_rope).  The scale of a block is what its largest
  * magnitude needs; where a block holds earlier rows its scale only grows, and when it does the earlier rows' codes are
  * re-encoded (int8: another rounding of at most half a step).  Rows behind the newest one stay as they were.  An infinity or a
- * NaN makes its block's scale NaN.  A page that two sequences share must not be written by either.
+ * NaN makes its block's scale NaN.  A page that two sequences share must not be written by either, and no block of tokens twice by
+ * one call (a table that names a page again, as a ring of pages does, takes no more new tokens at a time than the ring has rows).
  * query_starts NULL: one token per sequence (num_tokens = num_seqs). */
 typedef struct {
     const void* k;               /* device [num_tokens][num_kv_heads][head_dim] */
@@ -506,8 +508,11 @@ int32_t er_kv8_append(const er_kv8_cache* cache, const er_kv8_append_params* par
  * max(0, p - sliding_window + 1) .. p (sliding_window 0: 0 .. p; a window needs num_tokens and the rows that a block table addresses to
  * stay below 2^31 together, one that no sequence outgrows is the same as 0).  A query that sees nothing gets zeros.  softmax_scale 0 ->
  * 1 / sqrt(head_dim).  num_heads is a multiple of num_kv_heads, any group.
+ * out does not overlap q, the cache or the workspace.  Errors are relative to the largest value that a query sees: 16-bit types round each
+ * weight (probability times value scale) once to float16, 2^-11 of it, and sums of more than 16384 keys (prefill) or 196608 rows (decode)
+ * are continued in float32; float32 keeps 22 bits of queries and weights.
  * er_kv8_attention_decode: query_len tokens for every sequence (1 to 16; query token s * query_len + i), the work split over the GPU
- * along the rows; accuracy follows the type (float32: queries and probabilities enter the tensor cores as two halves each).
+ * along the rows.
  * er_kv8_attention_prefill: a ragged batch; max_query_len bounds the longest sequence's tokens (0 = num_tokens does).
  * workspace: device memory of er_kv8_*_workspace_bytes, 16-byte aligned, no particular contents; two calls that may overlap on the
  * GPU need two. */
