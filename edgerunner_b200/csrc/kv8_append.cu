@@ -478,11 +478,14 @@ int32_t launch_norm_rope(NormRope& p, cudaStream_t s) {
     const int vecs = p.head_dim / 2 / Act<T>::kVec;
     p.lanes = 1;
     while (p.lanes < vecs) p.lanes *= 2;
-    // A warp a token when that gives each SM 16 warps of work, else the heads of a token over two, four, eight warps; up to four CTAs an SM walk the tokens.
+    // Two CTAs fit an SM by their registers, and each begins with the frequencies: more of them cost a second start (4000 tokens in 500 CTAs 22.0 us, in 296 that
+    // walk the tokens 20.6).  Few tokens spread their heads over two, four or eight warps each, as long as the CTAs fit at a time (300 tokens on
+    // eight warps each, 300 CTAs: 9.9 us, on four, 150 CTAs: 6.5; on one, 38 CTAs: 7.5).
+    const int most = 2 * kv8_sm_count();
     p.warps_per_token = 1;
-    while (p.warps_per_token < 8 && static_cast<int64_t>(p.num_tokens) * p.warps_per_token < 148 * 16) p.warps_per_token *= 2;
+    while (p.warps_per_token < 8 && static_cast<int64_t>(p.num_tokens) * p.warps_per_token * 2 <= most * (kThreads / 32)) p.warps_per_token *= 2;
     const int tokens_per_cta = (kThreads / 32) / p.warps_per_token;
-    const int grid = std::min((p.num_tokens + tokens_per_cta - 1) / tokens_per_cta, 148 * 4);
+    const int grid = std::min((p.num_tokens + tokens_per_cta - 1) / tokens_per_cta, std::max(most, 1));
     const size_t smem = ((p.rotated + 1) & ~1) * sizeof(double) + (kThreads / 32) * (p.head_dim / 2) * sizeof(float2);
     qk_norm_rope_kernel<T><<<grid, kThreads, smem, s>>>(p);
     return kv8_launched(cudaGetLastError(), "qk_norm_rope_kernel");
@@ -494,7 +497,11 @@ int32_t launch_append(const Kv8Append& p, cudaStream_t s) {
     const unsigned blocks = p.starts == nullptr ? p.cache.num_seqs : p.num_tokens / sb + 2u * p.cache.num_seqs;
     const int threads = sb == 128 ? 512 : 256;
     const int groups = threads / 32 / (sb / kWarpRows), steps = (2 * p.cache.num_kv_heads + groups - 1) / groups;
-    const dim3 grid(blocks, blocks >= 592 ? 1 : steps);   // 592: four CTAs' worth of blocks for each SM
+    // The pairs of a block are spread over as many CTAs as make two an SM with the blocks that have rows: each CTA works out its block's turns, so that more of
+    // them cost more than they hide (blocks of 64, one CTA a step against this: 64 single tokens 16.5 / 11.5 us, 16 x 2048 tokens 189 / 65 us; one CTA a
+    // block: a single token 22.2 / 4.3 us).
+    const int64_t filled = p.starts == nullptr ? p.cache.num_seqs : p.num_tokens / sb + static_cast<int64_t>(p.cache.num_seqs);
+    const dim3 grid(blocks, static_cast<unsigned>(std::min<int64_t>(steps, std::max<int64_t>(1, 2 * kv8_sm_count() / filled))));
     const size_t smem = D / 2 * sizeof(double) + static_cast<size_t>(sb) * (D / 2) * sizeof(float2) + threads / 32 * kAppendSlots * kWarpRows * D * sizeof(T);
     if (smem > 48 * 1024) {
         constexpr int kMost = D / 2 * 8 + 128 * (D / 2) * 8 + 16 * kAppendSlots * kWarpRows * D * static_cast<int>(sizeof(T));
