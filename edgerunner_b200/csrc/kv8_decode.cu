@@ -4,7 +4,8 @@
 // sum_i p_i,  p_i = exp(s_i - m).  Codes are exact in fp16, so both contractions run on mma.sync.m16n8k16 with fp16 operands and float32
 // accumulators; the key scale multiplies the score, the value scale the probability.  The probabilities that enter the second product are
 // w = p * b / R with R the power of two next above the largest value scale that the query has seen so far (so w <= 1 whatever the scales are), carried 4096
-// times so that small ones stay normal fp16 numbers; R and m move together and rarely.
+// times so that small ones stay normal fp16 numbers; R and m move together and rarely.  bfloat16 rows round w to fp16; float32 and float16 rows carry a second
+// half with what that leaves (64 ragged sequences in float16: 226 -> 236 us with up to four query rows a kv head, 193 -> 208 us with 16).
 //
 // Work.  Bound by memory: 2 D bytes a row for 4 D flops a query head.  A persistent CTA per SM; the list of 32-token units of all (sequence, kv head,
 // row tile) items is cut evenly over the CTAs whatever the lengths are, inside a CTA the units of an item go round robin to the warps.  A warp
@@ -23,6 +24,7 @@
 // four token rows, turned into token pairs by byte permutes.  Stage layout: 16-byte chunks XORed so that both reads are free of bank conflicts.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "kv8.cuh"
 #include "tmap.h"
@@ -265,9 +267,14 @@ __device__ __forceinline__ void bounded_wait(uint64_t* bar, uint32_t parity, vol
     }
 }
 
-template <typename T, int D, bool E4M3, int NT, bool Long>
+template <typename T, int D, bool E4M3, int NT, bool Long, bool Pairs>
 __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kernel(const __grid_constant__ Kv8Decode p) {
-    constexpr bool kSplit = sizeof(T) == 4;      // float32: queries and weights as a high and a low half
+    constexpr bool kSplit = sizeof(T) == 4;      // float32: queries as a high and a low half
+    // Weights as a high and a low half: one rounding to fp16 is seen beside float16's own (131072 rows: 3.3e-4 from 64 bits instead of 2.2e-4), not beside bfloat16's.
+    // The low halves are a second product, or (Pairs: up to four query rows) take the four free columns, whose queries are the first four's over again.
+    constexpr bool kSplitW = !std::is_same<T, __nv_bfloat16>::value && !Pairs;
+    static_assert(!Pairs || (NT == 1 && std::is_same<T, __half>::value), "");
+    constexpr int kColumn = Pairs ? 3 : 7;       // column c of a tile is query row c & kColumn
     static_assert(!kSplit || (NT == 1 && !Long), "");
     constexpr int kRows = decode_rows<NT>(), kStages = decode_stages<T, D, NT>(), kWarps = decode_warps<T, NT>(), kThreads = kWarps * 32, kJoin = join_warps<T, NT>();
     constexpr int KK = D / 16, MT = D / 16, kWords = D / 16;   // k-steps of the scores; m-tiles of the outputs; 4-byte words of a lane's part of a key row
@@ -370,7 +377,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
         const int head = at.item / at.r.row_tiles, first_row = at.item % at.r.row_tiles * kRows;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const int r = first_row + nt * 8 + g, qi = r / p.group;
+            const int r = first_row + nt * 8 + (g & kColumn), qi = r / p.group;
             const T* src = static_cast<const T*>(p.q) + static_cast<int64_t>(at.r.begin + qi) * p.q_token + (head * p.group + r - qi * p.group) * p.q_head + (D / 4) * t;
 #pragma unroll
             for (int i = 0; i < kVecs; ++i) ahead[nt][i] = r < at.r.n * p.group ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
@@ -416,7 +423,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 qscale[nt][j] = __shfl_sync(0xffffffffu, f, (2 * t + j) * 4);
-                const int rr = rt * kRows + nt * 8 + 2 * t + j;
+                const int rr = rt * kRows + nt * 8 + ((2 * t + j) & kColumn);
                 limit[nt][j] = past + min(rr, rows - 1) / p.group;
             }
         }
@@ -553,7 +560,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
                     }
                 }
             }
-            uint32_t wh[2][NT][2], wl[2][kSplit ? NT : 1][2];
+            uint32_t wh[2][NT][2], wl[2][kSplitW ? NT : 1][2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -568,11 +575,15 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
                     }
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        if constexpr (kSplit) {
+                        if constexpr (kSplitW) {
                             uint32_t hi, lo;
                             split_half2(w[2 * x], w[2 * x + 1], hi, lo);
                             wh[h][nt][x] = transpose8x8(hi);
                             wl[h][nt][x] = transpose8x8(lo);
+                        } else if constexpr (Pairs) {
+                            uint32_t hi, lo;
+                            split_half2(w[2 * x], w[2 * x + 1], hi, lo);
+                            wh[h][nt][x] = transpose8x8(t < 2 ? hi : lo);
                         } else {
                             wh[h][nt][x] = transpose8x8(half2_bits(w[2 * x], w[2 * x + 1]));
                         }
@@ -613,7 +624,7 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             mma16816(o[nt][2 * i + x], a0, a1, a2, a3, wh[h][nt][0], wh[h][nt][1]);
-                            if constexpr (kSplit) mma16816(o[nt][2 * i + x], a0, a1, a2, a3, wl[h][nt][0], wl[h][nt][1]);
+                            if constexpr (kSplitW) mma16816(o[nt][2 * i + x], a0, a1, a2, a3, wl[h][nt][0], wl[h][nt][1]);
                         }
                     }
                 }
@@ -726,7 +737,11 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
 #pragma unroll
             for (int w = 0; w < kJoin; ++w) {
                 const float f = fast_exp2(join_ml[(w * kRows + col) * 2] - M0);
-                const float2 v = *reinterpret_cast<const float2*>(join + (w * kRows + col) * kJoinRow + pos);
+                float2 v = *reinterpret_cast<const float2*>(join + (w * kRows + col) * kJoinRow + pos);
+                if constexpr (Pairs) {
+                    const float2 low = *reinterpret_cast<const float2*>(join + (w * kRows + col + 4) * kJoinRow + pos);
+                    v = make_float2(v.x + low.x, v.y + low.y);
+                }
                 L = fmaf(f, join_ml[(w * kRows + col) * 2 + 1], L);
                 x = fmaf(f, v.x, x);
                 y = fmaf(f, v.y, y);
@@ -842,15 +857,15 @@ bool encode_rows(CUtensorMap* map, const uint8_t* codes, const Kv8Cache& c, int 
               head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int D, bool E4M3, int NT, bool Long>
+template <typename T, int D, bool E4M3, int NT, bool Long, bool Pairs>
 int32_t launch(Kv8Decode& p, int most_rows, int sms, cudaStream_t s) {
     constexpr int kSmem = decode_smem<T, D, NT>();
     static_assert(kSmem <= 232448, "decode kernel exceeds the shared memory of an sm_100 CTA");
-    p.tile_rows = 8 * NT;
+    p.tile_rows = Pairs ? 4 : 8 * NT;
     static std::atomic<uint64_t> devices{0};
-    cudaError_t e = kv8_allow_smem(kv8_decode_kernel<T, D, E4M3, NT, Long>, kSmem, devices);
+    cudaError_t e = kv8_allow_smem(kv8_decode_kernel<T, D, E4M3, NT, Long, Pairs>, kSmem, devices);
     if (e != cudaSuccess) return kv8_launched(e, "kv8_decode_kernel");
-    kv8_decode_kernel<T, D, E4M3, NT, Long><<<sms, decode_warps<T, NT>() * 32, kSmem, s>>>(p);
+    kv8_decode_kernel<T, D, E4M3, NT, Long, Pairs><<<sms, decode_warps<T, NT>() * 32, kSmem, s>>>(p);
     const int32_t rc = kv8_launched(cudaGetLastError(), "kv8_decode_kernel");
     if (rc != ER_OK) return rc;
     cudaLaunchConfig_t cfg{};
@@ -869,10 +884,14 @@ template <typename T, int D, bool E4M3>
 int32_t launch_rows(Kv8Decode& p, int most_rows, int sms, cudaStream_t s) {
     if constexpr (sizeof(T) == 2) {
         const bool two = tiles_of(ER_TYPE_FLOAT16, most_rows) == 2;
-        if (p.sums != nullptr) return two ? launch<T, D, E4M3, 2, true>(p, most_rows, sms, s) : launch<T, D, E4M3, 1, true>(p, most_rows, sms, s);
-        if (two) return launch<T, D, E4M3, 2, false>(p, most_rows, sms, s);
+        if constexpr (std::is_same<T, __half>::value) {
+            if (p.starts == nullptr && most_rows <= 4)
+                return p.sums != nullptr ? launch<T, D, E4M3, 1, true, true>(p, most_rows, sms, s) : launch<T, D, E4M3, 1, false, true>(p, most_rows, sms, s);
+        }
+        if (p.sums != nullptr) return two ? launch<T, D, E4M3, 2, true, false>(p, most_rows, sms, s) : launch<T, D, E4M3, 1, true, false>(p, most_rows, sms, s);
+        if (two) return launch<T, D, E4M3, 2, false, false>(p, most_rows, sms, s);
     }
-    return launch<T, D, E4M3, 1, false>(p, most_rows, sms, s);
+    return launch<T, D, E4M3, 1, false, false>(p, most_rows, sms, s);
 }
 template <typename T>
 int32_t launch_shape(Kv8Decode& p, int most_rows, int head_dim, bool e4m3, int sms, cudaStream_t s) {

@@ -508,9 +508,9 @@ int32_t er_kv8_append(const er_kv8_cache* cache, const er_kv8_append_params* par
  * max(0, p - sliding_window + 1) .. p (sliding_window 0: 0 .. p; a window needs num_tokens and the rows that a block table addresses to
  * stay below 2^31 together, one that no sequence outgrows is the same as 0).  A query that sees nothing gets zeros.  softmax_scale 0 ->
  * 1 / sqrt(head_dim).  num_heads is a multiple of num_kv_heads, any group.
- * out does not overlap q, the cache or the workspace.  Errors are relative to the largest value that a query sees: 16-bit types round each
- * weight (probability times value scale) once to float16, 2^-11 of it, and sums of more than 16384 keys (prefill) or 196608 rows (decode)
- * are continued in float32; float32 keeps 22 bits of queries and weights.
+ * out does not overlap q, the cache or the workspace.  Errors are relative to the largest value that a query sees: bfloat16, and float16 in
+ * prefill, round each weight (probability times value scale) once to float16, 2^-11 of it; float16 in decode and float32 keep 22 bits of the
+ * weights, float32 22 bits of the queries.  Sums of more than 16384 keys (prefill) or 196608 rows (decode) are continued in float32.
  * er_kv8_attention_decode: query_len tokens for every sequence (1 to 16; query token s * query_len + i), the work split over the GPU
  * along the rows.
  * er_kv8_attention_prefill: a ragged batch; max_query_len bounds the longest sequence's tokens (0 = num_tokens does).

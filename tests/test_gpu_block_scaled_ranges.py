@@ -291,3 +291,20 @@ def test_tables_without_pages(er, torch):  # noqa: F811
     assert cache.device_status() == 0
     cache.append(q[:, :1], q[:, :1], table, ints(torch, [1, 1]), partial_rotary_factor=0.0)
     assert cache.device_status() == -10
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dim, heads, kv_heads, query_len", [(128, 4, 1, 1), (64, 6, 2, 1), (128, 8, 1, 1), (64, 2, 2, 4), (128, 16, 1, 1), (128, 14, 2, 2), (64, 32, 4, 3), (128, 3, 1, 1)])
+def test_float16_decode_is_as_exact_as_its_outputs(er, torch, fmt, dim, heads, kv_heads, query_len):  # noqa: F811
+    """What is left against 64 bits is the rounding of the outputs to float16.  With y = want + d before it, |round(y) - want| <= |round(want) - want| + 2 |d|
+    (round(y) is no farther from y than round(want) is), and so are the norms.  d is float32's share: 22 bits of the weights, scores of exact products,
+    sums of some thousand terms, less than 2^-17 = 7.6e-6 of the output all together."""
+    lens = [9000, 20001]
+    cache, table, rows = fill(er, torch, fmt, lens, 128, kv_heads, dim, 16)
+    q = (0.3 * torch.randn(2 * query_len, heads, dim, generator=gen(torch, 2), device="cuda")).half()
+    got = cache.attention_decode(q, table, ints(torch, lens), query_len=query_len)
+    for s, n in enumerate(lens):
+        mine = slice(s * query_len, (s + 1) * query_len)
+        want, _ = ref_attention(torch, q[mine], *rows[s], n, dim ** -0.5)
+        best = float((want.half().double() - want).norm())
+        assert float((got[mine].double() - want).norm()) <= best + 2 * 2.0 ** -17 * float(want.norm())
