@@ -235,10 +235,11 @@ __device__ __forceinline__ double rope_frequency(int pair, int half, double log2
 }
 __device__ __forceinline__ float2 rope_turn(int position, double frequency) {
     double u = static_cast<double>(position) * frequency * 0.15915494309189533577;   // whole turns
-    u -= rint(u);
+    u = 2.0 * (u - rint(u));
+    const float half_turns = static_cast<float>(u), rest = static_cast<float>(u - half_turns) * 3.14159265f;   // what float32 leaves of the angle: up to 1e-7 radians
     float s, c;
-    sincospif(static_cast<float>(2.0 * u), &s, &c);
-    return make_float2(c, s);
+    sincospif(half_turns, &s, &c);
+    return make_float2(fmaf(-s, rest, c), fmaf(c, rest, s));
 }
 
 // ---- host ----

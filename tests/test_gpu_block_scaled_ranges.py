@@ -308,3 +308,18 @@ def test_float16_decode_is_as_exact_as_its_outputs(er, torch, fmt, dim, heads, k
         want, _ = ref_attention(torch, q[mine], *rows[s], n, dim ** -0.5)
         best = float((want.half().double() - want).norm())
         assert float((got[mine].double() - want).norm()) <= best + 2 * 2.0 ** -17 * float(want.norm())
+
+
+@pytest.mark.parametrize("theta, scaling", [(1e4, 1.0), (5e5, 8.0)])
+def test_turns_are_right_where_they_are_small(er, torch, theta, scaling):  # noqa: F811
+    """Pairs (1, 0) come out as (cos, sin).  Each is off by one step of the function, half a step of the correction's addition (2^-23 and 2^-24 of itself) and the angle:
+    64 bits over up to 2^20 / (2 pi) turns, 3 roundings, 4e-10 radians.  An angle rounded to 32 bits alone would be off by up to 9e-8."""
+    g = gen(torch, 2)
+    pos = torch.randint(0, 1 << 20, (4096,), generator=g, device="cuda", dtype=torch.int32)
+    x = torch.zeros(4096, 1, 128, device="cuda")
+    x[..., :64] = 1
+    y = torch.empty_like(x)
+    er.QKNormRopeKernel().encode(x, y, pos, rope_theta=theta, rope_scaling=scaling)
+    angle = pos.double()[:, None] * (theta ** (-torch.arange(64, device="cuda", dtype=torch.float64) / 64) / scaling)
+    want = torch.cat([angle.cos(), angle.sin()], dim=-1)[:, None]
+    assert bool(((y.double() - want).abs() <= want.abs() * 1.5 * 2.0 ** -23 + 1e-9).all())
