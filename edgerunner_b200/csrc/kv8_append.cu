@@ -6,8 +6,8 @@
 // some 150 instructions of a slow pipe) once a CTA, the (cos, sin) of a token once for all of its heads, in shared memory in the order in which the
 // lanes read them: 16 bytes (two pairs) a lane, lane beside lane.
 //
-// Measured (B200, bfloat16): norm + rotation of 32768 tokens of 32 + 8 heads of 128: 123 us = 5.46 TB/s = 0.83 of the copy bandwidth (157 us with the turns
-// read from shared memory for every head); append of 16 x 2048 tokens of 8 kv heads, E4M3, blocks of 32: 60 us = 3.4 TB/s = 0.51: half of its issue
+// Measured (B200, bfloat16): norm + rotation of 32768 tokens of 32 + 8 heads of 128: 126 us = 5.33 TB/s = 0.81 of the copy bandwidth (157 us with the turns
+// read from shared memory for every head); append of 16 x 2048 tokens of 8 kv heads, E4M3, blocks of 32: 61 us = 3.3 TB/s = 0.50: half of its issue
 // slots are busy, and without the arithmetic (norm, rotation, maximum, encoding) the same copies take 40 us.
 #include <algorithm>
 #include <cmath>

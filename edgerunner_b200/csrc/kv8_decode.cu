@@ -14,8 +14,8 @@
 // rows), so eight query rows fill a tile and K is an A operand as it lies in memory.  The warps of a CTA are joined in shared memory at the end of an
 // item, the CTAs that share an item by a second small launch that overlaps this one's tail.
 //
-// Measured (B200, head size 128, 32 query / 8 kv heads): 64 sequences of 1024 .. 16384 rows in 16-row pages, E4M3, bfloat16: 215 to 229 us = 5.1 to 5.4 TB/s = 0.77 to 0.82 of
-// the copy bandwidth; one sequence of 131072 int8 rows: 57 us = 4.7 TB/s.  With the arithmetic taken out the first takes 207 us, with the copies
+// Measured (B200, head size 128, 32 query / 8 kv heads): 64 sequences of 1024 .. 16384 rows in 16-row pages, E4M3, bfloat16: 227 to 234 us = 5.0 to 5.1 TB/s = 0.76 to 0.78 of
+// the copy bandwidth; one sequence of 131072 int8 rows, float16: 58 to 61 us = 4.4 to 4.6 TB/s.  With the arithmetic taken out the first takes 207 us, with the copies
 // taken out 173 us: what is left is their overlap at the ends of items (4.5 a CTA), the start and the joining launch.  32 tokens at a time instead of 16
 // brought 312 -> 237 us (the bookkeeping of a unit was half of its instructions); cp.async instead of TMA measured the same.
 //

@@ -3,7 +3,7 @@
 //
 // Mathematics.  s = (q . ck) a scale with a the key scale of 16 or more rows, w = 2^(s log2 e - m) b / R with b the value scale and R a power of two near
 // the largest one so far of the blocks that the row sees, o = R sum_i w_i cv_i / sum_i (w_i R / b_i).  Codes are exact in fp16, q and w are rounded to
-// it, sums are float32.  Neither scale costs an operation a score: a multiplies the factor inside exp2's argument, log2(b / R) is part of its offset,
+// it (float16 outputs 3.0e-4 from 64 bits instead of 2.1e-4; a second half of w would lengthen the softmax, which bounds the kernel), sums are float32.  Neither scale costs an operation a score: a multiplies the factor inside exp2's argument, log2(b / R) is part of its offset,
 // and the sum of 16 weights is divided by b / R once.
 //
 // One CTA owns two tiles of 128 query rows of a (sequence, kv head): row r is query r / group, head r % group, any group.  The tensor pipe takes 1024
@@ -20,11 +20,11 @@
 // Every wait is bounded (2 s): then the status word is set, the rest of the waits are skipped, the products that have been issued are waited for (3 s), tensor
 // memory is freed, the kernel returns.
 //
-// Measured (B200, 32 query / 8 kv heads of 128): a chunk of 2048 tokens at 32768, int8, float16: 1.28 ms = 835 TFLOP/s = 0.50 of the library's bf16
-// product; the same without the softmax arithmetic 0.80 ms, without the conversion besides 0.63 ms.  A tile's softmax takes 3400 clocks of a period
+// Measured (B200, 32 query / 8 kv heads of 128): a chunk of 2048 tokens at 32768, int8, float16: 1.29 to 1.31 ms = 810 to 826 TFLOP/s = 0.49 to 0.50 of the library's
+// bf16 product; before long sums were folded, without the softmax arithmetic 0.80 ms, without the conversion besides 0.63 ms.  A tile's softmax takes 3400 clocks of a period
 // of 4500: 2400 for the weights (1890 alone; 1024 of them exp2), 550 for the maximum.  What changed it on the way: loops over 64 columns instead of
 // straight-line code, which had the warps wait for instructions (2.20 -> 1.39 ms); seven loader warps, packed arithmetic, no divisions (1.29); scores of half
-// a tile kept in registers between the passes (1.21, before products were ordered by commits: +1 %).  Tried and dropped: part of the exponentials as
+// a tile kept in registers between the passes (1.21; 1.26 to 1.29 since products are ordered by commits).  Tried and dropped: part of the exponentials as
 // polynomials on the FMA pipe (the same or slower), weights in one pass against the old maximum (registers spill).
 #include <algorithm>
 #include <type_traits>
