@@ -337,7 +337,8 @@ __global__ void __launch_bounds__(decode_warps<T, NT>() * 32, 1) kv8_decode_kern
             pu += warp;
         }
         const int tok = pp.token(pu) + half * kKv8Unit;
-        ppage = tok < pp.r.len ? kv8_page(c, pp.seq, tok) : -1;
+        // blocks in front of the window are not fetched: their pages may be gone or somebody else's
+        ppage = tok < pp.r.len && (p.window == 0 || tok + kKv8Unit > pp.lowest(p)) ? kv8_page(c, pp.seq, tok) : -1;
     };
     int pstage = 0, produced = 0;
     auto produce = [&]() {          // the next unit, if there is one: lanes 0-15 see to half 0, 16-31 to half 1

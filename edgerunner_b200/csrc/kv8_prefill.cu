@@ -241,7 +241,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         const int64_t src_lane = static_cast<int64_t>(r8) * D + c4 * 16;
         const int total = 16 * tiles;
         auto token_of = [&](int q) { return (t_begin + (q >> 4)) * kTok + (q & 7) * 16; };
-        auto look_up = [&](Unit& x, int q) { x.page = q < total && token_of(q) < tile.len ? kv8_page(c, tile.seq, token_of(q)) : -1; };
+        // blocks in front of the window are not fetched: their pages may be gone or somebody else's
+        auto look_up = [&](Unit& x, int q) { x.page = q < total && token_of(q) < tile.len && token_of(q) + kKv8Unit > lo ? kv8_page(c, tile.seq, token_of(q)) : -1; };
         auto fetch = [&](Unit& x, int q) {
             const int side = (q >> 3) & 1, tok = token_of(q), valid = x.page >= 0 ? tile.len - tok : 0;
             const int64_t row = kv8_row(c, max(x.page, 0), head, kv8_in_page(c, tok));

@@ -506,7 +506,8 @@ int32_t er_kv8_append(const er_kv8_cache* cache, const er_kv8_append_params* par
 
 /* Attention over the cache: query i of a sequence with n queries sits at position p = kv_lens - n + i and sees the rows
  * max(0, p - sliding_window + 1) .. p (sliding_window 0: 0 .. p; a window needs num_tokens and the rows that a block table addresses to
- * stay below 2^31 together, one that no sequence outgrows is the same as 0).  A query that sees nothing gets zeros.  softmax_scale 0 ->
+ * stay below 2^31 together, one that no sequence outgrows is the same as 0; pages wholly in front of the window of every query may be gone or
+ * belong to somebody else).  A query that sees nothing gets zeros.  softmax_scale 0 ->
  * 1 / sqrt(head_dim).  num_heads is a multiple of num_kv_heads, any group.
  * out does not overlap q, the cache or the workspace.  Errors are relative to the largest value that a query sees: bfloat16, and float16 in
  * prefill, round each weight (probability times value scale) once to float16, 2^-11 of it; float16 in decode and float32 keep 22 bits of the

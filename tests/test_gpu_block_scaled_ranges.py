@@ -323,3 +323,29 @@ def test_turns_are_right_where_they_are_small(er, torch, theta, scaling):  # noq
     angle = pos.double()[:, None] * (theta ** (-torch.arange(64, device="cuda", dtype=torch.float64) / 64) / scaling)
     want = torch.cat([angle.cos(), angle.sin()], dim=-1)[:, None]
     assert bool(((y.double() - want).abs() <= want.abs() * 1.5 * 2.0 ** -23 + 1e-9).all())
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_pages_in_front_of_the_window_may_be_somebody_elses(er, torch, t, dim):  # noqa: F811
+    """A freed page whose id is still in the table: whatever lies there now, bytes that are codes of NaN and scales that are not finite among it, is not read
+    as anything."""
+    lens, window = [16 * 23 + 5, 700], 100
+    cache, table, rows = fill(er, torch, "e4m3", lens, 16, 2, dim, 16)
+    other = int(torch.arange(cache.num_pages, device="cuda")[~torch.isin(torch.arange(cache.num_pages, device="cuda"), table)][0])
+    cache.keys[other], cache.values[other] = 0x7F, 0xFF                    # NaN in every row
+    cache.key_scales[other], cache.value_scales[other] = math.nan, math.inf
+    q = torch.randn(2 * 70, 4, dim, generator=gen(torch, 3), device="cuda").to(dtype(torch, t))
+    for n in (1, 3, 70):
+        stale = table.clone()
+        for s in range(2):
+            stale[s, :(lens[s] - n - window + 1) // 16] = other
+        mine = torch.cat([q[:n], q[70:70 + n]])
+        got = [cache.attention_prefill(mine, ints(torch, [0, n, 2 * n]), stale, ints(torch, lens), sliding_window=window)]
+        if n <= 16:
+            got.append(cache.attention_decode(mine, stale, ints(torch, lens), query_len=n, sliding_window=window))
+        for out in got:
+            for s in range(2):
+                want, big = ref_attention(torch, mine[s * n:(s + 1) * n], *rows[s], lens[s], dim ** -0.5, window)
+                check_attention(torch, out[s * n:(s + 1) * n], want, big, t)
+    assert cache.device_status() == 0
