@@ -349,3 +349,37 @@ def test_pages_in_front_of_the_window_may_be_somebody_elses(er, torch, t, dim): 
                 want, big = ref_attention(torch, mine[s * n:(s + 1) * n], *rows[s], lens[s], dim ** -0.5, window)
                 check_attention(torch, out[s * n:(s + 1) * n], want, big, t)
     assert cache.device_status() == 0
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("columns", [100, 2100, 17000])
+def test_tables_wider_than_the_sequences(er, torch, t, columns):  # noqa: F811
+    """A server's tables have a fixed width: 1600, 33600 and 272000 rows here, beyond what either kernel keeps in its accumulators.  Prompts beside single tokens,
+    eager and as a captured graph that sees other lengths at its replay."""
+    lens, new = [400, 90, 0, 1030], [400, 1, 0, 130]
+    cache, table, rows = fill(er, torch, "e4m3", lens, 16, 2, 128, 16)
+    wide = torch.full((4, columns), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    starts = [sum(new[:s]) for s in range(5)]
+    q = torch.randn(starts[-1], 8, 128, generator=gen(torch, 3), device="cuda").to(dtype(torch, t))
+    one = q[:4].contiguous()
+    n, st = ints(torch, lens), ints(torch, starts)
+
+    def check(out, dec, now):
+        for s in range(4):
+            if new[s]:
+                want, big = ref_attention(torch, q[starts[s]:starts[s + 1]], rows[s][0][:now[s]], rows[s][1][:now[s]], now[s], 128 ** -0.5)
+                check_attention(torch, out[starts[s]:starts[s + 1]], want, big, t)
+            if now[s]:
+                want, big = ref_attention(torch, one[s:s + 1], rows[s][0][:now[s]], rows[s][1][:now[s]], now[s], 128 ** -0.5)
+                check_attention(torch, dec[s:s + 1], want, big, t)
+
+    check(cache.attention_prefill(q, st, wide, n, max_query_len=400), cache.attention_decode(one, wide, n), lens)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, dec = cache.attention_prefill(q, st, wide, n, max_query_len=400), cache.attention_decode(one, wide, n)
+    for now in (lens, [400, 60, 0, 500]):
+        n.copy_(ints(torch, now))
+        graph.replay()
+        check(out, dec, now)
+    assert cache.device_status() == 0
